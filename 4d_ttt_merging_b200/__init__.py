@@ -28,6 +28,7 @@ from .ops import (
     similarity_topk,
     streaming_top4,
 )
+from .streaming import PagedCache, attention_ranges, masked_attention, paged_attention
 from .token_plan import TokenPlan, WeightedBilinearTokenPlan
 from .planners import build_fastvggt_plan, build_ttt_protected_uniform_convex_plan, build_uniform_convex_plan
 from .attention_block import GlobalAttention, compute_attention
@@ -36,7 +37,9 @@ from . import parallel, ttt_kernels
 
 __all__ = [
     "GlobalAttention",
+    "PagedCache",
     "PlanCSR",
+    "attention_ranges",
     "build_fastvggt_plan",
     "build_ttt_protected_uniform_convex_plan",
     "build_uniform_convex_plan",
@@ -53,7 +56,9 @@ __all__ = [
     "library_path",
     "mass_bias_attention",
     "mass_bias_attention_into",
+    "masked_attention",
     "merge_argmax",
+    "paged_attention",
     "row_gather",
     "row_normalize_bf16",
     "similarity_topk",

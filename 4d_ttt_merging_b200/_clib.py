@@ -25,6 +25,27 @@ _c_size = ctypes.c_size_t
 _c_float = ctypes.c_float
 _p_i64 = ctypes.POINTER(ctypes.c_int64)
 
+
+
+class ScoreMods(ctypes.Structure):
+    """``vb200_score_mods``: what the masked and the paged attention add to the plain scores."""
+
+    _fields_ = [("key_bias", _c_vp), ("key_bias_sb", _c_i64), ("key_range", _c_vp), ("key_range_sb", _c_i64),
+                ("slope", _c_vp), ("q_position", _c_vp), ("q_position_sb", _c_i64), ("k_position", _c_vp),
+                ("k_position_sb", _c_i64), ("scale", _c_float), ("softcap", _c_float)]
+
+
+class CacheHandle(ctypes.Structure):
+    """``vb200_paged_cache``."""
+
+    _fields_ = [("k", _c_vp), ("v", _c_vp), ("log_mass", _c_vp), ("table", _c_vp), ("length", _c_vp),
+                ("references", _c_vp), ("pages", _c_i64), ("page_size", _c_i64), ("kv_heads", _c_i64),
+                ("slots", _c_i64), ("max_pages", _c_i64)]
+
+
+_p_mods = ctypes.POINTER(ScoreMods)
+_p_cache = ctypes.POINTER(CacheHandle)
+
 # name -> (restype, argtypes)
 _SIGNATURES = {
     "vb200_version": (_c_int, []),
@@ -45,6 +66,26 @@ _SIGNATURES = {
         [_c_int, _c_vp, _c_vp, _c_vp, _c_vp, _c_int, _c_vp, _c_i64, _c_i64, _c_i64, _c_i64, _c_i64,
          _p_i64, _p_i64, _p_i64, _p_i64, _c_vp],
     ),
+    "vb200_masked_attention": (
+        _c_int,
+        [_c_int, _c_vp, _c_vp, _c_vp, _c_vp, _c_i64, _c_i64, _c_i64, _c_i64, _c_i64, _c_i64, _p_i64, _p_i64, _p_i64,
+         _p_i64, _p_mods, _c_vp],
+    ),
+    "vb200_paged_attention": (
+        _c_int,
+        [_c_int, _c_vp, _c_vp, _c_i64, _c_i64, _c_i64, _p_i64, _p_i64, _p_cache, _c_vp, _c_vp, _c_i64, _c_int, _p_mods,
+         _c_vp],
+    ),
+    "vb200_cache_append_workspace_size": (_c_size, [_c_i64, _c_i64, _c_i64]),
+    "vb200_cache_append": (
+        _c_int,
+        [_p_cache, _c_int, _c_vp, _c_vp, _c_i64, _c_vp, _c_vp, _c_vp, _c_i64, _p_i64, _p_i64, _c_vp, _c_size, _c_vp],
+    ),
+    "vb200_cache_fork_workspace_size": (_c_size, [_c_i64, _c_i64, _c_i64]),
+    "vb200_cache_fork": (_c_int, [_p_cache, _c_int, _c_vp, _c_vp, _c_i64, _c_vp, _c_size, _c_vp]),
+    "vb200_cache_free": (_c_int, [_p_cache, _c_int, _c_vp, _c_i64, _c_vp]),
+    "vb200_cache_compact_workspace_size": (_c_size, [_c_i64]),
+    "vb200_cache_compact": (_c_int, [_p_cache, _c_int, _c_vp, _c_vp, _c_size, _c_vp]),
     "vb200_exp2_poly": (_c_int, [_c_vp, _c_vp, _c_i64, _c_vp]),
     "vb200_plan_csr_workspace_size": (_c_size, [_c_i64, _c_i64, _c_i64]),
     "vb200_plan_csr_build": (
@@ -211,7 +252,7 @@ def require_cuda(t: torch.Tensor, what: str) -> None:
 
 def device_error_flags(clear: bool = True) -> int:
     """OR of the kernels' device error words (bit 0: a bounded wait ran out; bit 1: an index
-    outside its range).  Synchronises the device."""
+    outside its range; bit 2: a cache append found too few free pages).  Synchronises the device."""
     flags = ctypes.c_uint(0)
     check(lib().vb200_device_error_flags(ctypes.byref(flags), int(clear)), "vb200_device_error_flags")
     return int(flags.value)

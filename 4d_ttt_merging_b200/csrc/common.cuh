@@ -25,6 +25,7 @@ namespace vb200 {
 enum DeviceError : unsigned {
   kErrWaitTimeout = 1u << 0,   // an mbarrier wait gave up
   kErrBadArgument = 1u << 1,   // a kernel found an index outside its declared range
+  kErrCacheFull = 1u << 2,     // an append found too few free pages, or a table row too short
 };
 
 __device__ __forceinline__ uint64_t global_timer_ns() {

@@ -28,6 +28,8 @@ unsigned projection_error_word(int clear);
 unsigned merge_error_word(int clear);
 unsigned plan_error_word(int clear);
 unsigned peer_error_word(int clear);
+unsigned masked_error_word(int clear);
+unsigned cache_error_word(int clear);
 
 inline size_t align_up(size_t v, size_t a) { return (v + a - 1) / a * a; }
 

@@ -1,0 +1,145 @@
+// Entry points of the masked and the paged attention: argument checks and the choice of kernel.
+#include <cmath>
+#include <initializer_list>
+
+#include "attention_view.cuh"
+#include "host_common.h"
+#include "masked_host.h"
+
+namespace vb200 {
+namespace {
+
+static __device__ unsigned g_masked_err;
+
+int error_word_address(unsigned** p) {
+  // resolved for the current device at every call: the address differs per device
+  VB200_CHECK_CUDA(cudaGetSymbolAddress(reinterpret_cast<void**>(p), g_masked_err), "cudaGetSymbolAddress(g_masked_err)");
+  return VB200_OK;
+}
+
+int fill_mods(const vb200_score_mods* m, AttnView& a) {
+  VB200_REQUIRE(std::isfinite(m->scale), "attention: scale must be finite");
+  VB200_REQUIRE(m->softcap >= 0.f && std::isfinite(m->softcap), "attention: softcap must be 0 (none) or positive and finite");
+  a.range = m->key_range;
+  a.range_sb = m->key_range_sb;
+  a.slope = m->slope;
+  if (m->softcap > 0.f) {
+    a.scale = m->scale / m->softcap;
+    a.cap = m->softcap * kLog2E;
+    VB200_REQUIRE(std::isfinite(a.scale) && std::isfinite(a.cap), "attention: softcap out of range");
+  } else {
+    a.scale = m->scale * kLog2E;
+    a.cap = 0.f;
+  }
+  return VB200_OK;
+}
+
+// 16-byte rows: base address and the strides of dimensions longer than one
+bool aligned(const void* p, const int64_t* s, std::initializer_list<int64_t> sizes, int es) {
+  bool ok = (reinterpret_cast<uintptr_t>(p) & 15u) == 0;
+  int i = 0;
+  for (int64_t n : sizes) {
+    ok = ok && (n <= 1 || (s[i] * es) % 16 == 0);
+    ++i;
+  }
+  return ok;
+}
+
+}  // namespace
+
+int sm_count_of_device() {
+  int dev = 0, n = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess) return 0;
+  if (cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess) return 0;
+  return n;
+}
+
+unsigned masked_error_word(int clear) {
+  unsigned v = 0;
+  cudaMemcpyFromSymbol(&v, g_masked_err, sizeof(v));
+  if (clear) {
+    const unsigned z = 0;
+    cudaMemcpyToSymbol(g_masked_err, &z, sizeof(z));
+  }
+  return v;
+}
+
+}  // namespace vb200
+
+using namespace vb200;
+
+extern "C" int vb200_masked_attention(int dtype, const void* q, const void* k, const void* v, void* out, int64_t B, int64_t H,
+                                      int64_t Hkv, int64_t Nq, int64_t Nk, int64_t D, const int64_t* qs, const int64_t* ks,
+                                      const int64_t* vs, const int64_t* os, const vb200_score_mods* mods, void* stream) {
+  VB200_REQUIRE(dtype == VB200_BF16 || dtype == VB200_F16 || dtype == VB200_F32, "masked_attention: unsupported dtype code %d", dtype);
+  VB200_REQUIRE(D == kHeadDim, "masked_attention supports head_dim=64 only (got %lld)", (long long)D);
+  VB200_REQUIRE(B >= 1 && H >= 1 && Hkv >= 1 && H % Hkv == 0 && Nq >= 0 && Nk >= 1,
+                "masked_attention: invalid sizes B=%lld H=%lld Hkv=%lld Nq=%lld Nk=%lld", (long long)B, (long long)H, (long long)Hkv,
+                (long long)Nq, (long long)Nk);
+  VB200_REQUIRE(Nk < (1ll << 31) - 128 && B * H < 65536 && Nq * (H / Hkv) < (1ll << 31) - 256,
+                "masked_attention: sizes exceed the kernels' index range");
+  VB200_REQUIRE(mods != nullptr, "masked_attention: null mods");
+  if (Nq == 0) return VB200_OK;
+  VB200_REQUIRE(q && k && v && out && qs && ks && vs && os, "masked_attention: null pointer argument");
+  const int es = dtype == VB200_F32 ? 4 : 2;
+  VB200_REQUIRE(aligned(q, qs, {B, H, Nq}, es) && aligned(k, ks, {B, Hkv, Nk}, es) && aligned(v, vs, {B, Hkv, Nk}, es) &&
+                    aligned(out, os, {B, H, Nq}, es),
+                "masked_attention: rows must be 16-byte aligned");
+  AttnView a{};
+  int rc = fill_mods(mods, a);
+  if (rc != VB200_OK) return rc;
+  if ((rc = check_sm100()) != VB200_OK || (rc = error_word_address(&a.err)) != VB200_OK) return rc;
+  a.q = q, a.k = k, a.v = v, a.out = out;
+  a.q_sb = qs[0], a.q_sh = qs[1], a.q_sn = qs[2];
+  a.k_sb = ks[0], a.k_sh = ks[1], a.k_sn = ks[2];
+  a.v_sb = vs[0], a.v_sh = vs[1], a.v_sn = vs[2];
+  a.o_sb = os[0], a.o_sh = os[1], a.o_sn = os[2];
+  a.B = static_cast<int>(B), a.H = static_cast<int>(H), a.Hkv = static_cast<int>(Hkv), a.group = static_cast<int>(H / Hkv);
+  a.Nq = static_cast<int>(Nq), a.Nk = static_cast<int>(Nk);
+  a.bias = mods->key_bias, a.bias_sb = mods->key_bias_sb;
+  a.qpos = mods->q_position, a.qpos_sb = mods->q_position_sb;
+  a.kpos = mods->k_position, a.kpos_sb = mods->k_position_sb;
+  return rows_attention(dtype, false, a, Nk, static_cast<cudaStream_t>(stream));
+}
+
+extern "C" int vb200_paged_attention(int dtype, const void* q, void* out, int64_t rows, int64_t H, int64_t D, const int64_t* qs,
+                                     const int64_t* os, const vb200_paged_cache* cache, const int32_t* sequence, const int32_t* offsets,
+                                     int64_t n, int causal, const vb200_score_mods* mods, void* stream) {
+  VB200_REQUIRE(dtype == VB200_BF16 || dtype == VB200_F16 || dtype == VB200_F32, "paged_attention: unsupported dtype code %d", dtype);
+  VB200_REQUIRE(D == kHeadDim, "paged_attention supports head_dim=64 only (got %lld)", (long long)D);
+  VB200_REQUIRE(cache != nullptr && mods != nullptr, "paged_attention: null handle or mods");
+  VB200_REQUIRE(cache->page_size == 16 || cache->page_size == 32 || cache->page_size == 64 || cache->page_size == 128,
+                "paged_attention: pages of 16, 32, 64 or 128 tokens (got %lld)", (long long)cache->page_size);
+  VB200_REQUIRE(H >= 1 && H < 65536 && cache->kv_heads >= 1 && H % cache->kv_heads == 0, "paged_attention: H=%lld is no multiple of %lld key heads",
+                (long long)H, (long long)cache->kv_heads);
+  VB200_REQUIRE(n >= 0 && n < (1ll << 24) && rows >= 0 && rows * (H / cache->kv_heads) < (1ll << 31) - 256 && cache->pages >= 1 &&
+                    cache->pages < (1ll << 30) && cache->slots >= 1 && cache->slots < (1ll << 30) && cache->max_pages >= 1 &&
+                    cache->max_pages * cache->page_size < (1ll << 31) - 128,
+                "paged_attention: sizes exceed the kernels' index range");
+  if (n == 0 || rows == 0) return VB200_OK;
+  VB200_REQUIRE(q && out && qs && os && offsets && cache->k && cache->v && cache->table && cache->length, "paged_attention: null pointer argument");
+  VB200_REQUIRE(sequence != nullptr || n <= cache->slots, "paged_attention: more sequences than slots");
+  const int es = dtype == VB200_F32 ? 4 : 2;
+  VB200_REQUIRE(aligned(q, qs, {H, rows}, es) && aligned(out, os, {H, rows}, es) && aligned(cache->k, nullptr, {}, es) &&
+                    aligned(cache->v, nullptr, {}, es),
+                "paged_attention: rows must be 16-byte aligned");
+  AttnView a{};
+  int rc = fill_mods(mods, a);
+  if (rc != VB200_OK) return rc;
+  if ((rc = check_sm100()) != VB200_OK || (rc = error_word_address(&a.err)) != VB200_OK) return rc;
+  a.q = q, a.k = cache->k, a.v = cache->v, a.out = out;
+  a.q_sh = qs[0], a.q_sn = qs[1], a.o_sh = os[0], a.o_sn = os[1];
+  a.Hkv = static_cast<int>(cache->kv_heads);
+  a.k_sh = a.v_sh = kHeadDim;
+  a.k_sn = a.v_sn = static_cast<long long>(a.Hkv) * kHeadDim;
+  a.k_sb = a.v_sb = a.k_sn * cache->page_size;
+  a.B = 1, a.H = static_cast<int>(H), a.group = static_cast<int>(H / cache->kv_heads);
+  a.Nq = static_cast<int>(rows), a.Nk = 0;
+  a.bias = cache->log_mass;
+  a.table = cache->table, a.length = cache->length, a.sequence = sequence, a.offsets = offsets;
+  a.table_stride = cache->max_pages;
+  a.n_seq = static_cast<int>(n), a.slots = static_cast<int>(cache->slots), a.pages = static_cast<int>(cache->pages);
+  a.page_shift = cache->page_size == 16 ? 4 : cache->page_size == 32 ? 5 : cache->page_size == 64 ? 6 : 7;
+  a.max_pages = static_cast<int>(cache->max_pages), a.causal = causal;
+  return rows_attention(dtype, true, a, cache->max_pages * cache->page_size, static_cast<cudaStream_t>(stream));
+}

@@ -46,8 +46,8 @@ VB200_API int vb200_version(void);
 VB200_API const char* vb200_last_error(void);
 /* Number of kernels this library has launched in the process (all devices, all threads). */
 VB200_API unsigned long long vb200_launch_count(void);
-/* OR of the error words that kernels write when a bounded wait runs out (bit 0) or an index
- * is out of range (bit 1).  Synchronises the current device; clears the words when clear!=0. */
+/* OR of the error words that kernels write when a bounded wait runs out (bit 0), an index
+ * is out of range (bit 1) or an append found too few free pages (bit 2).  Synchronises the current device; clears the words when clear!=0. */
 VB200_API int vb200_device_error_flags(unsigned* flags, int clear);
 
 /* ---- a1/a2/a3: mass-bias attention --------------------------------------------------------
@@ -113,6 +113,78 @@ VB200_API int vb200_mass_bias_attention_noalloc(int dtype, const void* q, const 
  * [-125, 64]; below -125 the result is about 2^-125).  Device arrays of n floats.  Test and
  * inspection entry point; no counterpart in the reference. */
 VB200_API int vb200_exp2_poly(const float* x, float* y, int64_t n, void* stream);
+
+/* ---- masked and paged attention -------------------------------------------------------------
+ * x_ij = scale q_i.k_j;  softcap c > 0: x = c tanh(x / c);  + key_bias_j;
+ * - slope_h |q_position_i - k_position_j|
+ * out_i = sum_j e^{x_ij} v_j / sum_j e^{x_ij} over the keys j in [begin_i, end_i) of the row; a row
+ * without keys gives 0.  What the other keys hold (infinities, NaN) never reaches the row.  Forward only.
+ * head_dim 64; H is a multiple of Hkv, query head h reads key head h / (H / Hkv).  BF16 / F16 run on
+ * tcgen05 (or the FMA pipe for few rows per key head), F32 on the FMA pipe; statistics and sums in fp32,
+ * in 16 bits the probabilities are rounded to the value type before the PV product.
+ * No reference counterpart: the reference's global attention sees one clip at a time, all of it. */
+typedef struct {
+  const float* key_bias;     /* natural log, added to the score; NULL: none.  Dense calls only:    */
+  int64_t key_bias_sb;       /*   [B][Nk] with this batch stride (0: one row for all)               */
+  const int32_t* key_range;  /* [B][Nq][2] (dense) or [rows][2] (paged): begin, end; NULL: all keys */
+  int64_t key_range_sb;      /*   batch stride in elements (0: one table for all)                   */
+  const float* slope;        /* [H] distance slopes, NULL: none                                     */
+  const float* q_position;   /* [B][Nq], NULL: Nk - Nq + i (the queries are the last tokens)        */
+  int64_t q_position_sb;
+  const float* k_position;   /* [B][Nk], NULL: j                                                    */
+  int64_t k_position_sb;
+  float scale;               /* usually 1 / 8                                                       */
+  float softcap;             /* 0: none                                                             */
+} vb200_score_mods;
+/* q, k, v, out with strides {batch, head, token}, channel stride 1; rows 16-byte aligned.  mods may be
+ * NULL only through its fields: pass a struct with scale set. */
+VB200_API int vb200_masked_attention(int dtype, const void* q, const void* k, const void* v, void* out, int64_t B, int64_t H,
+                                     int64_t Hkv, int64_t Nq, int64_t Nk, int64_t D, const int64_t* q_strides,
+                                     const int64_t* k_strides, const int64_t* v_strides, const int64_t* o_strides,
+                                     const vb200_score_mods* mods, void* stream);
+
+/* ---- paged cache of streamed keys and values ---------------------------------------------------
+ * The handle: contiguous pools k, v [pages][page_size][kv_heads][64] and log_mass [pages][page_size] (or NULL),
+ * table [slots][max_pages] of page numbers (-1: none), length [slots], references [pages] (0: free).
+ * page_size is 16, 32, 64 or 128.  Calls on one handle are ordered by their stream. */
+typedef struct {
+  void* k;
+  void* v;
+  float* log_mass;
+  int32_t* table;
+  int32_t* length;
+  int32_t* references;
+  int64_t pages, page_size, kv_heads, slots, max_pages;
+} vb200_paged_cache;
+/* Attention of ragged chunks over the cache: rows offsets[i] .. offsets[i+1] of q (strides {head, row}) are the
+ * last tokens of slot sequence[i] (NULL: slot i), already appended.  Without mods->key_range a row sees all
+ * keys of its slot, or with causal != 0 those up to its own.  Positions are token indices (q_position, k_position
+ * and key_bias of mods are not used: the bias is the cache's log_mass).  Rows outside every chunk are not written. */
+VB200_API int vb200_paged_attention(int dtype, const void* q, void* out, int64_t rows, int64_t H, int64_t D,
+                                    const int64_t* q_strides, const int64_t* o_strides, const vb200_paged_cache* cache,
+                                    const int32_t* sequence, const int32_t* offsets, int64_t n, int causal,
+                                    const vb200_score_mods* mods, void* stream);
+/* Appends rows offsets[i] .. offsets[i+1] of k, v (strides {token, head}) and log_mass [tokens] (NULL: 0) behind
+ * the tokens of slot sequence[i].  New pages are the lowest free ones in the order of the call; a shared, partly
+ * filled last page is copied first.  All or nothing: with too few pages (error bit 2) or offsets that
+ * do not ascend (bit 1) nothing changes.  A slot out of range or named before is left out (bit 1).
+ * Scratch: vb200_cache_append_workspace_size bytes, not shared by calls that may overlap. */
+VB200_API size_t vb200_cache_append_workspace_size(int64_t n, int64_t slots, int64_t pages);
+VB200_API int vb200_cache_append(const vb200_paged_cache* cache, int dtype, const int32_t* sequence, const int32_t* offsets,
+                                 int64_t n, const void* k, const void* v, const float* log_mass, int64_t tokens,
+                                 const int64_t* k_strides, const int64_t* v_strides, void* workspace, size_t workspace_bytes,
+                                 void* stream);
+/* Slots target[i] share the pages and the length of source[i], and give back what they held.  All sources are read
+ * before any target is written; of several pairs with one target the last counts. */
+VB200_API size_t vb200_cache_fork_workspace_size(int64_t n, int64_t slots, int64_t max_pages);
+VB200_API int vb200_cache_fork(const vb200_paged_cache* cache, int dtype, const int32_t* source, const int32_t* target, int64_t n,
+                               void* workspace, size_t workspace_bytes, void* stream);
+/* Empties slots; a page whose last reference goes is free. */
+VB200_API int vb200_cache_free(const vb200_paged_cache* cache, int dtype, const int32_t* sequence, int64_t n, void* stream);
+/* Moves the used pages to the front of the pool (contents, references, table entries); used[0] = pages in use. */
+VB200_API size_t vb200_cache_compact_workspace_size(int64_t pages);
+VB200_API int vb200_cache_compact(const vb200_paged_cache* cache, int dtype, int32_t* used, void* workspace,
+                                  size_t workspace_bytes, void* stream);
 
 /* ---- a7/a8: plan preprocessing --------------------------------------------------------------
  * Groups the S*corners (source, corner) pairs of a weighted plan by compact parent so that

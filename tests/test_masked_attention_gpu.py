@@ -1,0 +1,255 @@
+"""Masked attention on the GPU against its definition in 64 bits (``oracle.streaming``): types, head layouts, masks that
+leave rows empty, caps, distances, biases, strides, values that must not reach a row, graphs and streams.
+
+The tolerance of every element is the oracle's bound, counted from the roundings that the kernels make."""
+from __future__ import annotations
+
+import numpy as np
+import pytest
+import torch
+
+from helpers import TORCH_DTYPE, to_np
+
+pytestmark = pytest.mark.gpu
+
+
+def make(seed, B, H, Hkv, Nq, Nk, dtype, oracle, q_scale=2.0):
+    rng = np.random.default_rng(seed)
+    q = rng.standard_normal((B, H, Nq, 64)).astype(np.float32) * q_scale
+    k = rng.standard_normal((B, Hkv, Nk, 64)).astype(np.float32)
+    v = rng.standard_normal((B, Hkv, Nk, 64)).astype(np.float32)
+    return rng, *(oracle.round_to(t, dtype) for t in (q, k, v))
+
+
+def gpu(t, device, dtype=None):
+    return None if t is None else torch.from_numpy(np.ascontiguousarray(t)).to(device=device, dtype=dtype)
+
+
+def check(got, ref, bound):
+    got = to_np(got) if isinstance(got, torch.Tensor) else got
+    over = np.abs(got - ref) - bound
+    assert np.isfinite(got).all(), f"{np.sum(~np.isfinite(got))} values are not finite"
+    assert over.max(initial=-1.0) <= 0, f"{np.sum(over > 0)} values off by up to {over.max():.3e} more than their bound"
+
+
+def run(pkg, oracle, device, dtype, q, k, v, bias=None, ranges=None, slope=None, qpos=None, kpos=None, **kw):
+    td = TORCH_DTYPE[dtype]
+    out = pkg.masked_attention(gpu(q, device, td), gpu(k, device, td), gpu(v, device, td), gpu(bias, device),
+                               key_range=gpu(ranges, device), distance_slope=gpu(slope, device), query_position=gpu(qpos, device),
+                               key_position=gpu(kpos, device), **kw)
+    assert out.dtype == td and out.shape == q.shape
+    ref, bound = oracle.streaming.masked_attention(q, k, v, bias, ranges, slope=slope, qpos=qpos, kpos=kpos, dtype=dtype, **kw)
+    check(out, ref, bound)
+    assert pkg.device_error_flags() == 0
+    return out
+
+
+SHAPES = [  # B, H, Hkv, Nq, Nk
+    (1, 1, 1, 1, 1),
+    (1, 4, 1, 2, 7),      # eight row x head pairs over a few keys
+    (2, 2, 2, 1, 1000),   # single rows, keys split
+    (1, 6, 2, 9, 129),
+    (2, 4, 2, 130, 257),  # a second query tile with two rows, ragged tails
+    (1, 3, 3, 300, 300),
+    (1, 2, 1, 17, 1041),
+]
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f16", "f32"])
+@pytest.mark.parametrize("shape", SHAPES, ids=lambda s: "x".join(map(str, s)))
+def test_plain(pkg, oracle, cuda_device, dtype, shape):
+    _, q, k, v = make(sum(shape), *shape, dtype, oracle)
+    run(pkg, oracle, cuda_device, dtype, q, k, v)
+
+
+MASKS = {
+    "causal": dict(step=1),
+    "frames": dict(step=17),
+    "documents": dict(documents=[0, 5, 5, 140, 141, 333]),
+    "document frames prefix": dict(documents=[0, 100, 333], step=30, prefix=7),
+    "prefix": dict(step=1, prefix=130),
+    "window": dict(step=1, window=3),
+    "window of a document": dict(documents=[0, 128, 333], window=150),
+}
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f16", "f32"])
+@pytest.mark.parametrize("mask", sorted(MASKS))
+@pytest.mark.parametrize("queries", [333, 5])
+def test_masks(pkg, oracle, cuda_device, dtype, mask, queries):
+    spec = dict(MASKS[mask])
+    if "documents" in spec:
+        spec["documents"] = torch.tensor(spec["documents"], device=cuda_device)
+    ranges = pkg.attention_ranges(queries, 333, device=cuda_device, **spec).cpu().numpy()
+    rng, q, k, v = make(3, 1, 4, 2, queries, 333, dtype, oracle)
+    mass = np.log(rng.integers(1, 50, 333)).astype(np.float32)
+    run(pkg, oracle, cuda_device, dtype, q, k, v, mass, ranges)
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f16", "f32"])
+@pytest.mark.parametrize("queries", [200, 3])
+def test_empty_and_odd_ranges(pkg, oracle, cuda_device, dtype, queries):
+    """Rows that see nothing, ranges beyond the keys, reversed ones, a hole between the rows' keys, per batch entry."""
+    rng, q, k, v = make(4, 2, 2, 2, queries, 700, dtype, oracle)
+    r = np.sort(rng.integers(-5, 720, (2, queries, 2)), axis=2).astype(np.int32)
+    r[:, ::7] = 50
+    r[:, 1::11] = [300, 20]
+    r[:, 2::13] = [690, 5000]
+    r[0, queries // 2:] = [600, 640]
+    out = run(pkg, oracle, cuda_device, dtype, q, k, v, None, r)
+    empty = torch.from_numpy(np.minimum(r[..., 1], 700) <= np.maximum(r[..., 0], 0)).to(cuda_device)
+    assert bool(empty.any()) and bool((out.transpose(1, 2)[empty] == 0).all())
+    r[:] = 5
+    out = run(pkg, oracle, cuda_device, dtype, q, k, v, None, r)  # no row sees a key
+    assert (out == 0).all()
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f16", "f32"])
+@pytest.mark.parametrize("queries", [180, 2])
+@pytest.mark.parametrize("softcap,dist,mass", [(20.0, False, False), (None, True, False), (5.0, True, True), (100.0, False, True)])
+def test_scores(pkg, oracle, cuda_device, dtype, queries, softcap, dist, mass):
+    rng, q, k, v = make(5, 2, 4, 4, queries, 400, dtype, oracle, q_scale=6.0)
+    bias = np.log(rng.integers(1, 50, (2, 400))).astype(np.float32) if mass else None
+    slope = np.array([0.5, 0.25, 0.01, -0.003], np.float32) if dist else None
+    kpos = np.sort(rng.uniform(0, 60, (2, 400))).astype(np.float32) if dist and mass else None
+    qpos = rng.uniform(0, 60, queries).astype(np.float32) if dist and mass else None
+    r = pkg.attention_ranges(queries, 400, step=1, device=cuda_device).cpu().numpy()
+    run(pkg, oracle, cuda_device, dtype, q, k, v, bias, r, slope=slope, qpos=qpos, kpos=kpos, softcap=softcap, scale=0.2)
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f16", "f32"])
+@pytest.mark.parametrize("queries", [150, 2])
+def test_extreme_biases(pkg, oracle, cuda_device, dtype, queries):
+    """Masses of zero (bias -inf) hide a key; the type's lowest value outweighs every score but not another such key."""
+    rng, q, k, v = make(6, 3, 2, 2, queries, 300, dtype, oracle)
+    bias = np.zeros((3, 300), np.float32)
+    bias[0, ::2] = -np.inf
+    bias[0, 1::4] = np.finfo(np.float32).min
+    bias[1] = np.finfo(np.float32).min
+    bias[2] = -np.inf
+    v[2] = np.nan
+    v[0, :, ::2] = np.nan
+    k[0, :, ::4] = np.inf
+    out = run(pkg, oracle, cuda_device, dtype, q, k, v, bias)
+    assert (out[2] == 0).all()
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f16", "f32"])
+@pytest.mark.parametrize("queries", [333, 4])
+def test_hidden_values_do_not_reach_a_row(pkg, oracle, cuda_device, dtype, queries):
+    """NaN and infinities in keys and values that a row does not see, in the tiles that it reads."""
+    docs = torch.tensor([0, 20, 150, 151, 333], device=cuda_device)
+    r = pkg.attention_ranges(queries, 333, documents=docs, step=1, device=cuda_device).cpu().numpy()
+    _, q, k, v = make(7, 1, 2, 2, queries, 333, dtype, oracle)
+    clean = run(pkg, oracle, cuda_device, dtype, q, k, v, None, r)
+    td = TORCH_DTYPE[dtype]
+    bad_k, bad_v = k.copy(), v.copy()
+    bad_k[:, :, 332], bad_v[:, :, 332] = np.nan, np.inf   # the last key: only the last row sees it
+    bad_v[:, 0, 25, 3] = -np.inf                            # a key of document 1: its rows from 25 on see it
+    bad_k[:, 1, 7] = np.inf
+    got = pkg.masked_attention(gpu(q, cuda_device, td), gpu(bad_k, cuda_device, td), gpu(bad_v, cuda_device, td),
+                               key_range=gpu(r, cuda_device))
+    sees = np.zeros((1, 2, queries), bool)
+    for h, j in ((0, 332), (1, 332), (0, 25), (1, 7)):
+        sees[0, h] |= (r[:, 0] <= j) & (j < r[:, 1])
+    sees = torch.from_numpy(sees).to(cuda_device)
+    same = (got == clean).all(-1) | sees
+    assert bool(same.all()) or torch.allclose(got[~sees].float(), clean[~sees].float(), rtol=2.0 ** -7, atol=2.0 ** -8)
+    assert bool(torch.isfinite(got[~sees]).all()) and not bool(torch.isfinite(got[sees]).all(-1).any())
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+def test_strides(pkg, oracle, cuda_device, dtype):
+    """Views of a packed q | k | v buffer, a broadcast batch of keys, rows that are not 16-byte aligned, a given output."""
+    td = TORCH_DTYPE[dtype]
+    rng = np.random.default_rng(8)
+    x = oracle.round_to(rng.standard_normal((2, 150, 3 * 4 * 64)).astype(np.float32), dtype)
+    t = gpu(x, cuda_device, td).view(2, 150, 3, 4, 64)
+    q, k, v = (t[:, :, i].transpose(1, 2) for i in range(3))
+    npy = [to_np(y) for y in (q, k, v)]
+    ref, bound = oracle.streaming.masked_attention(*npy, dtype=dtype)
+    buf = torch.full((2, 152, 4, 64), 7.0, device=cuda_device, dtype=td)
+    out = buf[:, 1:151].transpose(1, 2)
+    assert pkg.masked_attention(q, k, v, out=out) is out
+    check(out, ref, bound)
+    assert bool((buf[:, 0] == 7).all()) and bool((buf[:, 151] == 7).all())  # what lies beside is left as it was
+    kb, vb = k[:1].expand(2, -1, -1, -1), v[:1].expand(2, -1, -1, -1)
+    ref, bound = oracle.streaming.masked_attention(npy[0], npy[1][[0, 0]], npy[2][[0, 0]], dtype=dtype)
+    check(pkg.masked_attention(q, kb, vb), ref, bound)
+    odd = torch.empty(2 * 4 * 150 * 65, device=cuda_device, dtype=td)[1:1 + 2 * 4 * 150 * 64].view(2, 4, 150, 64)
+    odd.copy_(q)
+    ref, bound = oracle.streaming.masked_attention(*npy, dtype=dtype)
+    check(pkg.masked_attention(odd, k, v), ref, bound)
+
+
+@pytest.mark.parametrize("dtype,queries", [("bf16", 40), ("bf16", 2), ("f32", 2)])
+def test_offsets_beyond_32_bits(pkg, oracle, cuda_device, dtype, queries):
+    """Keys whose rows lie more than 2^32 bytes (and elements) apart."""
+    td = TORCH_DTYPE[dtype]
+    Nk, stride = 200, (1 << 32) // 192 // 64 * 64
+    base = torch.zeros(Nk * stride + 64, device=cuda_device, dtype=td)
+    _, q, k, v = make(9, 1, 1, 1, queries, Nk, dtype, oracle)
+    kk = base.as_strided((1, 1, Nk, 64), (0, 0, stride, 1))
+    kk.copy_(gpu(k, cuda_device, td))
+    ref, bound = oracle.streaming.masked_attention(q, k, v, dtype=dtype)
+    check(pkg.masked_attention(gpu(q, cuda_device, td), kk, gpu(v, cuda_device, td)), ref, bound)
+    check(pkg.masked_attention(gpu(q, cuda_device, td), gpu(k, cuda_device, td), kk), *oracle.streaming.masked_attention(q, k, k, dtype=dtype))
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+def test_no_rows_and_no_keys(pkg, cuda_device, dtype):
+    td = TORCH_DTYPE[dtype]
+    z = lambda *s: torch.ones(s, device=cuda_device, dtype=td)  # noqa: E731
+    assert pkg.masked_attention(z(1, 2, 0, 64), z(1, 2, 5, 64), z(1, 2, 5, 64)).shape == (1, 2, 0, 64)
+    assert bool((pkg.masked_attention(z(1, 2, 3, 64), z(1, 2, 0, 64), z(1, 2, 0, 64)) == 0).all())
+    assert pkg.masked_attention(z(0, 2, 3, 64), z(0, 2, 5, 64), z(0, 2, 5, 64)).numel() == 0
+
+
+@pytest.mark.parametrize("queries", [300, 3])
+def test_repeatable_graph_and_stream(pkg, cuda_device, queries):
+    """The same bits from a second call, from a replayed graph with refilled inputs, from another stream and from two
+    graphs replayed at once."""
+    g = torch.Generator(device=cuda_device).manual_seed(1)
+    new = lambda n: torch.randn(1, 4, n, 64, generator=g, device=cuda_device).bfloat16()  # noqa: E731
+    q, k, v = new(queries), new(900), new(900)
+    mass = torch.rand(900, generator=g, device=cuda_device)
+    r = pkg.attention_ranges(queries, 900, step=64, device=cuda_device)
+    call = lambda: pkg.masked_attention(q, k, v, mass, key_range=r, softcap=30.0)  # noqa: E731
+    a, b = call(), call()
+    assert torch.equal(a, b)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        c = call()
+    torch.cuda.current_stream().wait_stream(side)
+    assert torch.equal(a, c)
+    graphs, outs = [], []
+    for _ in range(2):
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            outs.append(call())
+        graphs.append(graph)
+    q.copy_(new(queries))
+    k.copy_(new(900))
+    ref = call()
+    torch.cuda.synchronize()
+    with torch.cuda.stream(side):
+        for _ in range(3):
+            graphs[0].replay()
+    for _ in range(3):
+        graphs[1].replay()
+    torch.cuda.synchronize()
+    assert torch.equal(outs[0], ref) and torch.equal(outs[1], ref)
+    assert pkg.device_error_flags() == 0
+
+
+def test_refusals_on_the_gpu(pkg, cuda_device):
+    q = torch.zeros(1, 2, 4, 64, device=cuda_device, dtype=torch.bfloat16)
+    with pytest.raises(RuntimeError, match="no backward"):
+        pkg.masked_attention(q.clone().requires_grad_(), q, q)
+    with torch.no_grad():
+        pkg.masked_attention(q.clone().requires_grad_(), q, q)
+    with pytest.raises(ValueError, match="tensors are on"):
+        pkg.masked_attention(q, q, q, torch.zeros(4))
+    with pytest.raises(ValueError, match="out must"):
+        pkg.masked_attention(q, q, q, out=torch.empty(1, 2, 4, 65, device=cuda_device, dtype=torch.bfloat16)[..., :64])

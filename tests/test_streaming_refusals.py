@@ -1,0 +1,155 @@
+"""Argument checks of the masked and paged attention and of the cache that need no GPU, the key intervals of the masks, and
+the oracle of the cache."""
+from __future__ import annotations
+
+import ctypes
+
+import numpy as np
+import pytest
+import torch
+
+
+def test_masked_attention_refusals(pkg):
+    q = torch.zeros(1, 4, 3, 64)
+    k = torch.zeros(1, 2, 5, 64)
+    f = pkg.masked_attention
+    with pytest.raises(ValueError, match="head_dim=64"):
+        f(q[..., :32], k[..., :32], k[..., :32])
+    with pytest.raises(ValueError, match="batch, heads"):
+        f(q[0], k, k)
+    with pytest.raises(ValueError, match="incompatible"):
+        f(q, torch.zeros(1, 3, 5, 64), torch.zeros(1, 3, 5, 64))
+    with pytest.raises(ValueError, match="incompatible"):
+        f(q, k, k[:, :, :4])
+    with pytest.raises(ValueError, match="one dtype"):
+        f(q, k.half(), k.half())
+    with pytest.raises(ValueError, match="unsupported dtype"):
+        f(q.double(), k.double(), k.double())
+    for cap in (0.0, -1.0, float("nan"), float("inf")):
+        with pytest.raises(ValueError, match="softcap"):
+            f(q, k, k, softcap=cap)
+    with pytest.raises(ValueError, match="scale"):
+        f(q, k, k, scale=float("inf"))
+    with pytest.raises(ValueError, match="distance_slope"):
+        f(q, k, k, distance_slope=torch.zeros(2))
+    with pytest.raises(ValueError, match="positions are used"):
+        f(q, k, k, key_position=torch.zeros(5))
+    with pytest.raises(ValueError, match="key_range"):
+        f(q, k, k, key_range=torch.zeros(3, 2))
+    with pytest.raises(ValueError, match="key_range"):
+        f(q, k, k, key_range=torch.zeros(2, 2, dtype=torch.int32))
+    with pytest.raises(ValueError, match="out must"):
+        f(q, k, k, out=torch.zeros(1, 4, 2, 64))
+    with pytest.raises(RuntimeError, match="CUDA"):
+        f(q, k, k)
+
+
+def test_cache_refusals(pkg):
+    with pytest.raises(RuntimeError, match="CUDA"):
+        pkg.PagedCache.empty(1, 4, 4, device="cpu")
+    with pytest.raises(ValueError, match="pages hold"):
+        pkg.PagedCache.empty(1, 4, 4, page_size=48, device="cpu")
+    with pytest.raises(ValueError, match="at least 1"):
+        pkg.PagedCache.empty(0, 4, 4, device="cpu")
+    k = torch.zeros(4, 16, 2, 64)
+    ints = lambda *s: torch.zeros(s, dtype=torch.int32)  # noqa: E731
+    make = pkg.PagedCache
+    with pytest.raises(ValueError, match="cache pools"):
+        make(torch.zeros(4, 24, 2, 64), k, None, ints(1, 2), ints(1), ints(4))
+    with pytest.raises(ValueError, match="one shape"):
+        make(k, k.half(), None, ints(1, 2), ints(1), ints(4))
+    with pytest.raises(ValueError, match="log_mass"):
+        make(k, k, torch.zeros(4, 8), ints(1, 2), ints(1), ints(4))
+    with pytest.raises(ValueError, match="table"):
+        make(k, k, None, ints(1, 2), ints(2), ints(4))
+    with pytest.raises(ValueError, match="int32"):
+        make(k, k, None, ints(1, 2).long(), ints(1), ints(4))
+    with pytest.raises(ValueError, match="contiguous"):
+        make(k, torch.zeros(4, 16, 64, 2).transpose(2, 3), None, ints(1, 2), ints(1), ints(4))
+
+
+def test_c_entry_points_refuse_bad_arguments(pkg):
+    lib, C = pkg.load_library(), pkg._clib
+    s = (ctypes.c_int64 * 3)(64, 64, 64)
+    mods = C.ScoreMods(scale=0.125)
+    dense = lambda dt=1, q=16, B=1, H=4, Hkv=2, Nq=3, Nk=5, D=64, st=s, m=mods: lib.vb200_masked_attention(  # noqa: E731
+        dt, q, 16, 16, 16, B, H, Hkv, Nq, Nk, D, st, s, s, s, m, None)
+    for kw, word in ((dict(dt=7), b"dtype"), (dict(D=32), b"head_dim"), (dict(Hkv=3), b"sizes"), (dict(Nk=0), b"sizes"),
+                     (dict(Nk=1 << 31), b"range"), (dict(q=None), b"null"), (dict(q=8), b"aligned"),
+                     (dict(st=(ctypes.c_int64 * 3)(64, 64, 60)), b"aligned"), (dict(m=C.ScoreMods(scale=float("nan"))), b"scale"),
+                     (dict(m=C.ScoreMods(scale=1.0, softcap=-1.0)), b"softcap"), (dict(m=None), b"mods")):
+        assert dense(**kw) == C.EINVAL and word in lib.vb200_last_error(), (kw, lib.vb200_last_error())
+    assert dense(Nq=0) == 0
+    cache = lambda **k: C.CacheHandle(**dict(dict(k=16, v=16, table=16, length=16, references=16, pages=4, page_size=16,  # noqa: E731
+                                                  kv_heads=2, slots=2, max_pages=4), **k))
+    two = (ctypes.c_int64 * 2)(64, 64)
+    paged = lambda c, H=4, rows=2, n=1, q=16, seq=16: lib.vb200_paged_attention(1, q, 16, rows, H, 64, two, two, c, seq, 16, n, 1,  # noqa: E731
+                                                                               mods, None)
+    for c, kw, word in ((cache(page_size=24), {}, b"pages of"), (cache(), dict(H=3), b"multiple"), (cache(pages=0), {}, b"range"),
+                        (cache(k=None), {}, b"null"), (cache(), dict(q=None), b"null"), (cache(), dict(n=3, seq=None), b"slots"),
+                        (cache(k=24), {}, b"aligned")):
+        assert paged(c, **kw) == C.EINVAL and word in lib.vb200_last_error(), (kw, lib.vb200_last_error())
+    assert paged(cache(), n=0) == 0 and paged(cache(), rows=0) == 0
+    size = lib.vb200_cache_append_workspace_size(1, 2, 4)
+    app = lambda c, ws=16, size=size, mass=None, k=16: lib.vb200_cache_append(c, 1, 16, 16, 1, k, 16, mass, 2, two, two, ws, size, None)  # noqa: E731
+    for c, kw, word in ((cache(page_size=8), {}, b"pages of"), (cache(), dict(size=16), b"workspace"), (cache(), dict(mass=16), b"log-mass"),
+                        (cache(), dict(k=24), b"aligned"), (cache(references=None), {}, b"null")):
+        assert app(c, **kw) == C.EINVAL and word in lib.vb200_last_error(), (kw, lib.vb200_last_error())
+    assert lib.vb200_cache_fork(cache(), 1, 16, None, 1, 16, 1 << 20, None) == C.EINVAL
+    assert lib.vb200_cache_fork(cache(), 1, 16, 16, 1, 16, 4, None) == C.EINVAL
+    assert lib.vb200_cache_free(cache(), 1, None, 1, None) == C.EINVAL
+    assert lib.vb200_cache_compact(cache(), 1, None, 16, 1 << 20, None) == C.EINVAL
+    assert lib.vb200_cache_compact(cache(), 1, 16, 16, 4, None) == C.EINVAL
+
+
+def test_attention_ranges(pkg):
+    f = pkg.attention_ranges
+    assert f(3).tolist() == [[0, 3]] * 3 and f(0).shape == (0, 2)
+    assert f(2, 4, step=1).tolist() == [[0, 3], [0, 4]]
+    assert f(5, step=2).tolist() == [[0, 2], [0, 2], [0, 4], [0, 4], [0, 5]]
+    docs = torch.tensor([0, 2, 2, 5])
+    assert f(5, documents=docs).tolist() == [[0, 2], [0, 2], [2, 5], [2, 5], [2, 5]]
+    assert f(5, documents=docs, step=1, prefix=2).tolist() == [[0, 2], [0, 2], [2, 4], [2, 4], [2, 5]]
+    assert f(4, step=1, window=2).tolist() == [[0, 1], [0, 2], [1, 3], [2, 4]]
+    assert f(4, documents=torch.tensor([0, 2, 4]), window=1).tolist() == [[0, 2], [1, 2], [2, 4], [3, 4]]
+    for bad in (dict(keys=1), dict(step=0), dict(window=0), dict(prefix=-1), dict(documents=torch.tensor([0])),
+                dict(documents=torch.zeros(3))):
+        with pytest.raises(ValueError):
+            f(2, **bad)
+
+
+def test_oracle_against_plain_softmax(oracle):
+    rng = np.random.default_rng(0)
+    q, k, v = rng.standard_normal((3, 1, 2, 6, 64))
+    out, _ = oracle.streaming.masked_attention(q, k, v)
+    ref = torch.softmax(torch.from_numpy(q @ k.swapaxes(-1, -2) / 8), -1).numpy() @ v
+    assert np.abs(out - ref).max() < 1e-12
+
+
+def test_oracle_cache_keeps_tokens(oracle):
+    """Appends, forks and compactions leave every slot's tokens what was written, and the references what the tables hold."""
+    rng = np.random.default_rng(1)
+    c = oracle.streaming.Cache(np.zeros((20, 4, 1, 2)), np.zeros((20, 4, 1, 2)), np.zeros((20, 4)), np.full((3, 10), -1), [0] * 3, [0] * 20)
+    want = {0: [], 1: [], 2: []}
+    for _ in range(200):
+        what = rng.integers(4)
+        a, b = rng.integers(0, 3, 2)
+        if what == 0:
+            n = int(rng.integers(1, 6))
+            x = rng.standard_normal((n, 1, 2))
+            if c.append([a], [0, n], x, -x, x[:, 0, 0]):
+                want[a] = want[a] + list(x)
+        elif what == 1:
+            c.fork([a], [b])
+            want[b] = list(want[a])
+        elif what == 2:
+            c.free([a])
+            want[a] = []
+        else:
+            used = c.compact()
+            assert used == sum(r > 0 for r in c.refs) and all(r == 0 for r in c.refs[used:])
+        for s in range(3):
+            k, v, m = c.tokens(s)
+            assert len(k) == len(want[s]) and all((x == y).all() for x, y in zip(k, want[s])) and (v == -k).all()
+        count = np.bincount([p for row in c.held for p in row], minlength=20)
+        assert count.tolist() == c.refs
