@@ -45,6 +45,10 @@ bool aligned(const void* p, const int64_t* s, std::initializer_list<int64_t> siz
   return ok;
 }
 
+// fp32, or at most 8 (row, head) pairs per key head: the FMA kernel.  A tile of the tensor-core kernel has 128 rows
+// of one head, so below that its tiles are nearly empty and the heads of a group read their keys one by one.
+bool few_rows(int dtype, int64_t rows, int group) { return dtype == VB200_F32 || rows * group <= 8; }
+
 }  // namespace
 
 int sm_count_of_device() {
@@ -99,7 +103,8 @@ extern "C" int vb200_masked_attention(int dtype, const void* q, const void* k, c
   a.bias = mods->key_bias, a.bias_sb = mods->key_bias_sb;
   a.qpos = mods->q_position, a.qpos_sb = mods->q_position_sb;
   a.kpos = mods->k_position, a.kpos_sb = mods->k_position_sb;
-  return rows_attention(dtype, false, a, Nk, static_cast<cudaStream_t>(stream));
+  if (few_rows(dtype, Nq, a.group)) return rows_attention(dtype, false, a, Nk, static_cast<cudaStream_t>(stream));
+  return tile_attention(dtype, false, a, Nk, static_cast<cudaStream_t>(stream));
 }
 
 extern "C" int vb200_paged_attention(int dtype, const void* q, void* out, int64_t rows, int64_t H, int64_t D, const int64_t* qs,
@@ -141,5 +146,7 @@ extern "C" int vb200_paged_attention(int dtype, const void* q, void* out, int64_
   a.n_seq = static_cast<int>(n), a.slots = static_cast<int>(cache->slots), a.pages = static_cast<int>(cache->pages);
   a.page_shift = cache->page_size == 16 ? 4 : cache->page_size == 32 ? 5 : cache->page_size == 64 ? 6 : 7;
   a.max_pages = static_cast<int>(cache->max_pages), a.causal = causal;
-  return rows_attention(dtype, true, a, cache->max_pages * cache->page_size, static_cast<cudaStream_t>(stream));
+  const int64_t most = cache->max_pages * cache->page_size;
+  if (few_rows(dtype, (rows + n - 1) / n, a.group)) return rows_attention(dtype, true, a, most, static_cast<cudaStream_t>(stream));
+  return tile_attention(dtype, true, a, most, static_cast<cudaStream_t>(stream));
 }

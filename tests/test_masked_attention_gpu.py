@@ -159,6 +159,25 @@ def test_hidden_values_do_not_reach_a_row(pkg, oracle, cuda_device, dtype, queri
 
 
 @pytest.mark.parametrize("dtype", ["bf16", "f32"])
+@pytest.mark.parametrize("queries", [300, 4])
+def test_hidden_values_of_any_size(pkg, oracle, cuda_device, dtype, queries):
+    """Hidden keys and values near the largest finite number, beside rows whose scores are far below zero."""
+    r = pkg.attention_ranges(queries, 300, step=1, window=40, device=cuda_device).cpu().numpy()
+    rng, q, k, v = make(12, 1, 2, 2, queries, 300, dtype, oracle)
+    bias = np.where(np.arange(300) % 3 == 0, -np.inf, -300.0).astype(np.float32)
+    v[:, :, ::3] = 3e38
+    k[:, :, ::6] = 3e38
+    run(pkg, oracle, cuda_device, dtype, q, k, v, bias, r)
+    first = 300 - queries
+    r[:] = [0, first + 1]
+    r[1:, 1] = first  # only the first row sees the key at its own place
+    v[:, :, first] = 3e38
+    bias[first] = -np.inf if dtype == "f32" else 0.0
+    out = run(pkg, oracle, cuda_device, dtype, q[:, :, 1:], k, v, bias, r[1:]) if queries > 4 else None
+    assert out is None or bool((out.abs() < 100).all())
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
 def test_strides(pkg, oracle, cuda_device, dtype):
     """Views of a packed q | k | v buffer, a broadcast batch of keys, rows that are not 16-byte aligned, a given output."""
     td = TORCH_DTYPE[dtype]
