@@ -1,31 +1,46 @@
 // Masked and paged attention on the tensor cores (bf16, fp16); the mathematics is in attention_view.cuh.
 //
-// One CTA per 256 query rows of one sequence and head (two tiles of 128 rows), one CTA per SM, 12 warps:
-//   warps 0-7   two softmax warpgroups, one per query tile, one thread per row (its TMEM lane).  A row's
-//               scores of a key tile sit in one thread's registers, so the cap, the bias, the distance and the
-//               mask are applied once, and the row's maximum needs no exchange.
-//   warp 8      TMA producer: Q once; K and V tiles of 128 keys into a ring (dense: one box; paged: a box per page,
-//               pages outside the sequence read a coordinate outside the pool and fill with zeros).
-//   warp 9      TMEM and the MMA stream: S_t = Q_t K_j^T one tile ahead, O_t += P_t V_j, as the softmax releases them.
-//   warp 10     per key: bias and position of the tile, into the ring (only when there are any).
+// One CTA per 256 query rows of one sequence and head (two tiles of 128 rows that share every K and V tile), one
+// CTA per SM, 12 warps:
+//   warps 0-7    two softmax warpgroups, one per query tile, one thread per row (its TMEM lane).  A row's scores sit
+//                in one thread's registers, so the cap, the bias, the distance and the mask are applied once, and
+//                the row's maximum needs no exchange.  A tile of 128 keys is taken in two halves of 64.
+//   warp 8       TMA producer: Q once; K and V tiles of 128 keys into a ring (dense: one box; paged: a box per page,
+//                pages outside the sequence read a coordinate outside the pool and fill with zeros).
+//   warps 9, 10  one MMA stream per query tile: S(j + 1) = Q K_{j+1}^T as soon as S(j) is in registers, then
+//                O += P(j) V_j.
+//   warp 11      per key: bias and position of the tile, into the ring (only when there are any).  Without a cap the
+//                bias rides in the QK product: an extra K=16 chunk holds 1, 1, 1 in columns 0 to 2 of every query
+//                row and bias / scale, split into three 16-bit values that add up to its 24 bits, in those of the
+//                key row.  A tile with a bias that does not fit (infinite, the type's lowest value) gets it in the
+//                softmax instead.
 // TMEM: S_t at 128 t, P_t at 256 + 64 t (16-bit, the A operand of PV), O_t at 384 + 64 t.
 //
-// Work that is skipped: key tiles outside the union of a query tile's intervals.  Masks are evaluated in the tiles
-// that some row of a warp sees in part only.  A hidden key has probability 0; what its value holds still meets that
-// 0 in the PV product, so a row that comes out with a value that is not finite is computed again, key by key, by its
+// The two warps of an SM sub-partition compute their exponentials at the same time and leave the unit idle at the same time
+// (3200 clocks per 256 x 128 scores, 2100 of them in exponentials); making them take turns measured 8% slower, starting one
+// half a tile later 6%, and part of the exponentials on the FMA pipe 4%.
+//
+// Why this shape: a wait costs 50 to 100 clocks even when what it waits for is long there, a tile's arithmetic 510
+// (two warps per SM sub-partition, bound by the exponential unit) per 64 keys.  64-key steps with a wait for each
+// product spent as long in waits as in arithmetic (890 clocks a step, two CTAs of 128 rows); so the softmax waits
+// twice per 128 keys.  Two query tiles per CTA because two CTAs of 128 rows load K and V twice, 24 bytes per SM clock
+// and more, near what L2 gives.
+//
+// Work that is skipped: key tiles outside the union of the rows' intervals.  Masks are evaluated in the tiles that
+// some row of a warp sees in part only.  A hidden key has probability 0; what its value holds still meets that 0 in
+// the PV product, so a row that comes out with a value that is not finite is computed again, key by key, by its
 // warp (exact_row): rows are right whatever the hidden values are, and finite inputs pay one test per row.
 //
 // When the blocks do not fill the GPU, the key tiles of each are split over a cluster of 2, 4 or 8 CTAs;
 // (O, maximum, sum) of the parts meet in distributed shared memory and are joined in rank order (no workspace, no second
 // launch, the same bits at every run).
 //
-// The running maximum is lazy: O_t is rescaled only when a row's maximum grows by more than 2^8.  Probabilities are
+// The running maximum is lazy: O is rescaled only when a row's maximum grows by more than 2^8.  Probabilities are
 // rounded to the value type for the PV product; sums, maxima and O are fp32.
 #include <cudaTypedefs.h>
 
 #include <atomic>
 
-#include "attention_mma.cuh"
 #include "attention_view.cuh"
 #include "host_common.h"
 #include "masked_host.h"
@@ -33,39 +48,39 @@
 namespace vb200 {
 namespace {
 
-constexpr int kBM = 128, kQT = 2, kBN = 128;
+constexpr int kBM = 128, kQT = 2, kBN = 128, kHalf = 64;
 constexpr int kStages = 4;
-constexpr int kTileBytes = kBM * kHeadDim * 2;
+constexpr int kTileBytes = kBN * kHeadDim * 2;  // 16 KB: a Q, K or V tile
 constexpr int kSoftmaxWarps = 8;
-constexpr int kWarpProducer = 8, kWarpMma = 9, kWarpKeys = 10;
+constexpr int kWarpProducer = 8, kWarpMma = 9, kWarpKeys = 11;
 constexpr int kThreads = 12 * 32;
-// Register split: the block launches with 168 a thread (64512 of the SM's 65536); the softmax warpgroups rise to
-// 200, the third drops to 104.  The host refuses to launch a build with another count.
-constexpr int kLaunchRegs = 168, kRegsHigh = 200, kRegsLow = 104;
-static_assert(kSoftmaxWarps * 32 * kRegsHigh + 128 * kRegsLow == kThreads * kLaunchRegs, "register split");
 constexpr float kRescale = 8.f;  // P stays <= 2^8
-constexpr int kPolyPairs = 1;    // of every 8 exponent pairs, those on the FMA pipe
 
 constexpr int kOffQ = 0;
 constexpr int kOffStage = kQT * kTileBytes;
-constexpr int kOffKeys = kOffStage + kStages * 2 * kTileBytes;  // [stage][2][128] fp32: bias, position
+// The bias chunk of a tile: 128 rows x 16 columns, no swizzle: [16 row groups][2 column halves][8 rows][16 bytes]
+constexpr int kExtraBytes = 4096;
+constexpr int kOffExtra = kOffStage + kStages * 2 * kTileBytes;   // the query rows' chunk, then one per stage
+constexpr int kOffKeys = kOffExtra + (1 + kStages) * kExtraBytes;  // [stage][2][128] fp32: bias, position
 constexpr int kOffBar = kOffKeys + kStages * 2 * kBN * 4;
-constexpr int kBarQ = 0, kBarFull = 1, kBarEmpty = kBarFull + kStages, kBarS = kBarEmpty + kStages, kBarP = kBarS + kQT,
-              kBarO = kBarP + kQT, kBarSFree = kBarO + kQT, kNumBars = kBarSFree + kQT;
-constexpr int kOffMisc = kOffBar + kNumBars * 8;  // tmem slot, abort flag, per tile: first and last key
-constexpr int kSmemBytes = kOffMisc + 32 + 1024;
+constexpr int kBarQ = 0, kBarFull = 1, kBarEmpty = kBarFull + kStages, kBarS = kBarEmpty + kStages, kBarSFree = kBarS + kQT,
+              kBarP = kBarSFree + kQT, kBarO = kBarP + kQT, kNumBars = kBarO + kQT;
+constexpr int kOffMisc = kOffBar + kNumBars * 8;  // TMEM base; per query tile: first and last key; per stage: bias in the softmax
+constexpr int kSmemBytes = kOffMisc + 48 + 1024;
 constexpr int kPartStride = kHeadDim + 4;  // floats; parts of a split overlay Q and the ring
 constexpr int kOffPartMl = kQT * kBM * kPartStride * 4;
 static_assert(kOffPartMl + kQT * kBM * 8 <= kOffKeys, "the parts fit");
 constexpr uint32_t kTmemCols = 512, kTmemP = 256, kTmemO = 384;
 
-// S_t = Q_t K^T: four K=16 steps of head_dim 64; the first overwrites.
-__device__ __forceinline__ void issue_qk(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t bar) {
+// S = Q K^T: four K=16 steps of head_dim 64, the first overwrites, and with use_x the bias chunk (xa, xb).
+__device__ __forceinline__ void issue_qk(uint32_t d, uint64_t a, uint64_t b, uint64_t xa, uint64_t xb, uint32_t use_x, uint32_t idesc,
+                                         uint32_t bar) {
   asm volatile(
-      "{\n\t.reg .pred e, pf, pt;\n\t.reg .b64 a1, a2, a3, b1, b2, b3;\n\t"
+      "{\n\t.reg .pred e, pf, pt, px;\n\t.reg .b64 a1, a2, a3, b1, b2, b3;\n\t"
       "elect.sync _|e, 0xffffffff;\n\t"
       "setp.ne.b32 pf, 0, 0;\n\t"
       "setp.eq.b32 pt, 0, 0;\n\t"
+      "setp.ne.and.b32 px, %7, 0, e;\n\t"
       "add.s64 a1, %1, 2;\n\tadd.s64 b1, %2, 2;\n\t"
       "add.s64 a2, %1, 4;\n\tadd.s64 b2, %2, 4;\n\t"
       "add.s64 a3, %1, 6;\n\tadd.s64 b3, %2, 6;\n\t"
@@ -73,8 +88,39 @@ __device__ __forceinline__ void issue_qk(uint32_t d, uint64_t a, uint64_t b, uin
       "@e tcgen05.mma.cta_group::1.kind::f16 [%0], a1, b1, %3, pt;\n\t"
       "@e tcgen05.mma.cta_group::1.kind::f16 [%0], a2, b2, %3, pt;\n\t"
       "@e tcgen05.mma.cta_group::1.kind::f16 [%0], a3, b3, %3, pt;\n\t"
+      "@px tcgen05.mma.cta_group::1.kind::f16 [%0], %5, %6, %3, pt;\n\t"
       "@e tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%4];\n\t}" ::"r"(d),
-      "l"(a), "l"(b), "r"(idesc), "r"(bar)
+      "l"(a), "l"(b), "r"(idesc), "r"(bar), "l"(xa), "l"(xb), "r"(use_x)
+      : "memory");
+}
+
+// O (+)= P V over a key tile: eight K=16 steps; P in TMEM (8 columns of packed pairs a step), V MN-major (2048 bytes a
+// step).  Commits to both barriers.
+__device__ __forceinline__ void issue_pv(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t acc_first, uint32_t bar,
+                                         uint32_t bar2) {
+  asm volatile(
+      "{\n\t.reg .pred e, pf, pt;\n\t.reg .b64 b1, b2, b3, b4, b5, b6, b7;\n\t.reg .b32 a1, a2, a3, a4, a5, a6, a7;\n\t"
+      "elect.sync _|e, 0xffffffff;\n\t"
+      "setp.ne.b32 pf, %4, 0;\n\t"
+      "setp.eq.b32 pt, 0, 0;\n\t"
+      "add.s32 a1, %1, 8;\n\tadd.s64 b1, %2, 128;\n\t"
+      "add.s32 a2, %1, 16;\n\tadd.s64 b2, %2, 256;\n\t"
+      "add.s32 a3, %1, 24;\n\tadd.s64 b3, %2, 384;\n\t"
+      "add.s32 a4, %1, 32;\n\tadd.s64 b4, %2, 512;\n\t"
+      "add.s32 a5, %1, 40;\n\tadd.s64 b5, %2, 640;\n\t"
+      "add.s32 a6, %1, 48;\n\tadd.s64 b6, %2, 768;\n\t"
+      "add.s32 a7, %1, 56;\n\tadd.s64 b7, %2, 896;\n\t"
+      "@e tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, pf;\n\t"
+      "@e tcgen05.mma.cta_group::1.kind::f16 [%0], [a1], b1, %3, pt;\n\t"
+      "@e tcgen05.mma.cta_group::1.kind::f16 [%0], [a2], b2, %3, pt;\n\t"
+      "@e tcgen05.mma.cta_group::1.kind::f16 [%0], [a3], b3, %3, pt;\n\t"
+      "@e tcgen05.mma.cta_group::1.kind::f16 [%0], [a4], b4, %3, pt;\n\t"
+      "@e tcgen05.mma.cta_group::1.kind::f16 [%0], [a5], b5, %3, pt;\n\t"
+      "@e tcgen05.mma.cta_group::1.kind::f16 [%0], [a6], b6, %3, pt;\n\t"
+      "@e tcgen05.mma.cta_group::1.kind::f16 [%0], [a7], b7, %3, pt;\n\t"
+      "@e tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%5];\n\t"
+      "@e tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%6];\n\t}" ::"r"(d),
+      "r"(a), "l"(b), "r"(idesc), "r"(acc_first), "r"(bar), "r"(bar2)
       : "memory");
 }
 
@@ -145,12 +191,142 @@ __device__ __noinline__ void exact_row(const AttnView& a, AttnSeq s, int i, int 
   out[1] = from_f32<T>(l == 0.f ? 0.f : o1 / l);
 }
 
+// Both 16-bit halves of x times f.
+template <typename T>
+__device__ __forceinline__ uint32_t scale2(uint32_t x, float f) {
+  const T* h = reinterpret_cast<const T*>(&x);
+  const float lo = to_f32<T>(h[0]) * f, hi = to_f32<T>(h[1]) * f;
+  return std::is_same<T, __nv_bfloat16>::value ? pack_bf16x2(lo, hi) : pack_f16x2(lo, hi);
+}
+
 template <typename T>
 __device__ __forceinline__ uint32_t pack2(float lo, float hi) {
   return sizeof(T) == 2 && std::is_same<T, __nv_bfloat16>::value ? pack_bf16x2(lo, hi) : pack_f16x2(lo, hi);
 }
 
-template <typename T, bool kPaged>
+// tanh(y) / y for y^2 <= 1 as a polynomial in y^2, fitted here for minimum maximum relative error (least squares
+// reweighted to equal ripples: 6e-7, 7e-7 evaluated in fp32).
+constexpr float kTanh0 = 0.9999994039535522f, kTanh1 = -0.3332904279232025f, kTanh2 = 0.13281433284282684f,
+                kTanh3 = -0.051605671644210815f, kTanh4 = 0.016743112355470657f, kTanh5 = -0.0030670592095702887f;
+
+__device__ __forceinline__ float max_of(const uint32_t (&r)[kHalf]) {
+  float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+  for (int c = 0; c < kHalf; c += 8) {
+#pragma unroll
+    for (int u = 0; u < 4; ++u) mx[u] = fmax3(mx[u], u2f(r[c + 2 * u]), u2f(r[c + 2 * u + 1]));
+  }
+  return fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
+}
+
+// r <- tanh(r s).  On the FMA pipe while no score of the warp is beyond the cap (eight packed instructions a pair, as long
+// as the exponential unit takes for the probabilities), else two uses of the exponential unit per score.
+__device__ __forceinline__ void cap_scores(uint32_t (&r)[kHalf], float s) {
+  float far = 0.f;
+#pragma unroll
+  for (int c = 0; c < kHalf; c += 2) far = fmax3(far, fabsf(u2f(r[c])), fabsf(u2f(r[c + 1])));
+  if (__all_sync(0xffffffffu, far * fabsf(s) <= 1.f)) {
+    const uint64_t s2 = pk2(s, s);
+#pragma unroll
+    for (int c = 0; c < kHalf; c += 2) {
+      const uint64_t y = fmul2(pk2(u2f(r[c]), u2f(r[c + 1])), s2), z = fmul2(y, y);
+      uint64_t f = ffma2(pk2(kTanh5, kTanh5), z, pk2(kTanh4, kTanh4));
+      f = ffma2(f, z, pk2(kTanh3, kTanh3));
+      f = ffma2(f, z, pk2(kTanh2, kTanh2));
+      f = ffma2(f, z, pk2(kTanh1, kTanh1));
+      f = ffma2(f, z, pk2(kTanh0, kTanh0));
+      float x0, x1;
+      upk2(fmul2(f, y), x0, x1);
+      r[c] = f2u(x0);
+      r[c + 1] = f2u(x1);
+    }
+  } else {
+#pragma unroll
+    for (int c = 0; c < kHalf; ++c) r[c] = f2u(tanh_fast(u2f(r[c]) * s));
+  }
+}
+
+// The scores of 64 keys: products in r -> scores of which mul times is the log2 domain, hidden keys at -inf.  kFull: with
+// the cap, the distance and, with add, biases that are in `keys` and not in the product (always with a cap).
+template <bool kFull>
+__device__ __forceinline__ float form_scores(uint32_t (&r)[kHalf], const AttnView& a, const float* keys, bool add, float slope, float pos,
+                                             int lo, int hi, bool partly) {
+  float mul = a.scale;
+  if constexpr (kFull) {
+    if (a.cap != 0.f) {
+      cap_scores(r, a.scale);
+      mul = a.cap;
+    }
+    if (add || a.slope != nullptr) {
+      // the ring holds zeros for biases that are in the product
+      const uint64_t sc = pk2(mul, mul);
+#pragma unroll
+      for (int c = 0; c < kHalf; c += 4) {
+        const float4 y = *reinterpret_cast<const float4*>(keys + c);
+        float x0, x1;
+        upk2(ffma2(pk2(u2f(r[c]), u2f(r[c + 1])), sc, pk2(y.x, y.y)), x0, x1);
+        r[c] = f2u(x0);
+        r[c + 1] = f2u(x1);
+        upk2(ffma2(pk2(u2f(r[c + 2]), u2f(r[c + 3])), sc, pk2(y.z, y.w)), x0, x1);
+        r[c + 2] = f2u(x0);
+        r[c + 3] = f2u(x1);
+      }
+      mul = 1.f;
+    }
+    if (a.slope != nullptr) {
+#pragma unroll
+      for (int c = 0; c < kHalf; c += 4) {
+        const float4 y = *reinterpret_cast<const float4*>(keys + kBN + c);
+        r[c] = f2u(fmaf(-slope, fabsf(pos - y.x), u2f(r[c])));
+        r[c + 1] = f2u(fmaf(-slope, fabsf(pos - y.y), u2f(r[c + 1])));
+        r[c + 2] = f2u(fmaf(-slope, fabsf(pos - y.z), u2f(r[c + 2])));
+        r[c + 3] = f2u(fmaf(-slope, fabsf(pos - y.w), u2f(r[c + 3])));
+      }
+    }
+  }
+  if (partly) {
+    lo = min(max(lo, 0), kHalf);
+    hi = min(max(hi, 0), kHalf);
+#pragma unroll
+    for (int w = 0; w < kHalf / 32; ++w) {
+      // bits [lo, hi) of this word of 32 columns
+      const int l0 = min(max(lo - 32 * w, 0), 32), h0 = min(max(hi - 32 * w, 0), 32);
+      const uint32_t up = h0 >= 32 ? 0xffffffffu : (1u << h0) - 1u;
+      const uint32_t dn = l0 >= 32 ? 0u : 0xffffffffu << l0;
+      const uint32_t see = up & dn;
+#pragma unroll
+      for (int c = 0; c < 32; ++c)
+        if (!((see >> c) & 1u)) r[32 * w + c] = f2u(-INFINITY);
+    }
+  }
+  return mul;
+}
+
+// p[c] <- (2^(r[2c] mul - m), 2^(r[2c+1] mul - m)) in 16 bits; returns the sum of the unrounded values.
+template <typename T>
+__device__ __forceinline__ float probabilities(const uint32_t (&r)[kHalf], float mul, float m, uint32_t* p) {
+  const float m_use = m == -INFINITY ? 0.f : m;
+  const uint64_t neg_m2 = pk2(-m_use, -m_use), mul2 = pk2(mul, mul);
+  uint64_t ls0 = pk2(0.f, 0.f), ls1 = pk2(0.f, 0.f);
+#pragma unroll
+  for (int c = 0; c < kHalf / 2; ++c) {
+    float e0, e1, q0, q1;
+    upk2(ffma2(pk2(u2f(r[2 * c]), u2f(r[2 * c + 1])), mul2, neg_m2), e0, e1);
+    q0 = ex2_approx(e0);
+    q1 = ex2_approx(e1);
+    if (c & 1) ls1 = fadd2(ls1, pk2(q0, q1));
+    else ls0 = fadd2(ls0, pk2(q0, q1));
+    p[c] = pack2<T>(q0, q1);
+  }
+  float a0, a1, b0, b1;
+  upk2(ls0, a0, a1);
+  upk2(ls1, b0, b1);
+  return (a0 + a1) + (b0 + b1);
+}
+
+// kForm: 0 plain scores; 1 with a bias (in the product; a tile with one that does not fit takes the general step);
+// 2 with a cap or a distance too.
+template <typename T, bool kPaged, int kForm>
 __global__ void __launch_bounds__(kThreads, 1)
     masked_attention_tc_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_constant__ CUtensorMap tmap_k,
                                const __grid_constant__ CUtensorMap tmap_v, const __grid_constant__ AttnView a, int blocks, int split) {
@@ -168,45 +344,54 @@ __global__ void __launch_bounds__(kThreads, 1)
   const int row_first = blk * kQT * kBM;
 
   auto bar = [=](int i) -> uint32_t { return sbase + kOffBar + 8 * i; };
-  volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + kOffMisc + 4);
   int* key_lo = reinterpret_cast<int*>(smem + kOffMisc + 8);
   int* key_hi = key_lo + kQT;
-  const bool per_key = a.bias != nullptr || a.slope != nullptr;
+  const bool per_key = kForm > 0 && (a.bias != nullptr || a.slope != nullptr);
+  const bool in_product = kForm > 0 && a.bias != nullptr && a.cap == 0.f;
+  volatile int* bias_flag = reinterpret_cast<volatile int*>(smem + kOffMisc + 24);  // per stage
 
   if (threadIdx.x == 0) {
     mbar_init(bar(kBarQ), 1);
     for (int i = 0; i < kStages; ++i) {
       mbar_init(bar(kBarFull + i), per_key ? 2 : 1);
-      mbar_init(bar(kBarEmpty + i), 1);
+      mbar_init(bar(kBarEmpty + i), kQT);
     }
     for (int t = 0; t < kQT; ++t) {
       mbar_init(bar(kBarS + t), 1);
-      mbar_init(bar(kBarP + t), kBM);
+      mbar_init(bar(kBarSFree + t), 4);
+      mbar_init(bar(kBarP + t), 4);
       mbar_init(bar(kBarO + t), 1);
-      mbar_init(bar(kBarSFree + t), kBM);
       key_lo[t] = 0x7fffffff;
       key_hi[t] = 0;
     }
-    *abort_flag = 0;
     fence_barrier_init();
   }
   if (warp == kWarpMma) {
     tmem_alloc(sbase + kOffMisc, kTmemCols);
     tmem_relinquish();
   }
+  if (in_product) {
+    // the query rows' chunk: 1, 1, 1 in columns 0 to 2; the key rows' chunks: zero beyond column 3
+    const uint32_t one = kBF16 ? 0x3F80u : 0x3C00u;
+    for (int x = threadIdx.x; x < (1 + kStages) * kExtraBytes / 16; x += kThreads) {
+      const bool q = x < kExtraBytes / 16 && ((x >> 3) & 1) == 0;
+      *reinterpret_cast<uint4*>(smem + kOffExtra + 16 * x) = make_uint4(q ? one | one << 16 : 0u, q ? one : 0u, 0u, 0u);
+    }
+    fence_proxy_async_smem();  // generic writes become visible to the tensor core
+  }
   if (warp == kWarpProducer && lane == 0) {
     prefetch_tmap(&tmap_q);
     prefetch_tmap(&tmap_k);
     prefetch_tmap(&tmap_v);
   }
+  int2 be = make_int2(0, 0);  // keys of this thread's row
+  const bool valid = warp < kSoftmaxWarps && row_first + static_cast<int>(threadIdx.x) < s.rows;
+  if (valid) be = row_range<kPaged>(a, s, row_first + threadIdx.x);
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = *reinterpret_cast<volatile uint32_t*>(smem + kOffMisc);
-  int2 be = make_int2(0, 0);
   if (warp < kSoftmaxWarps) {
-    const int i = row_first + static_cast<int>(threadIdx.x);
-    if (i < s.rows) be = row_range<kPaged>(a, s, i);
     const int lo = __reduce_min_sync(0xffffffffu, be.y > be.x ? be.x : 0x7fffffff);
     const int hi = __reduce_max_sync(0xffffffffu, be.y);
     if (lane == 0 && hi > 0) {
@@ -240,13 +425,13 @@ __global__ void __launch_bounds__(kThreads, 1)
   }
   if (j0[0] == j1[0] && j0[1] == j1[1]) p1 = p0;  // the part lies between the two query tiles' keys
 
-  // Each role's code is dominated by its own setmaxnreg, with no merge point in between.
+  // A wait that runs out makes its role go on without waiting (or leave), so that every thread reaches the end and
+  // TMEM is freed.
   if (warp >= kSoftmaxWarps) {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegsLow));
     if (warp == kWarpProducer) {
       // ------------------------------- producer -------------------------------
-      const int npg = kPaged ? kBN >> a.page_shift : 1;
-      const int which = lane / npg, pg = lane - which * npg;  // K (0) or V (1), page of the tile
+      const int npg = kPaged ? kBN >> a.page_shift : 1;       // boxes per tile
+      const int which = lane / npg, pg = lane - which * npg;  // K (0) or V (1), box of the tile
       auto page_at = [&](int j) -> int {
         const int slot = ((j * kBN) >> a.page_shift) + pg;
         return static_cast<long long>(slot) << a.page_shift < s.keys ? page_of(a, s, slot) : a.pages;
@@ -258,91 +443,90 @@ __global__ void __launch_bounds__(kThreads, 1)
         for (int t = 0; t < kQT; ++t)
           tma_load_4d(sbase + kOffQ + t * kTileBytes, &tmap_q, bar(kBarQ), 0, s.row0 + row_first + t * kBM, head, s.batch);
       }
-      for (int j = p0; j < p1; ++j) {
+      int j = p0;
+      bool ok = true;
+      for (; j < p1; ++j) {
         const int n = j - p0, st = n % kStages;
-        bool ok = *abort_flag == 0;
-        if (n >= kStages) ok = mbar_wait(bar(kBarEmpty + st), (n / kStages - 1) & 1, a.err) && ok;
-        if (!__all_sync(0xffffffffu, ok)) {
-          if (lane == 0) *abort_flag = 1;
-          break;
-        }
+        if (n >= kStages) ok = __all_sync(0xffffffffu, mbar_wait(bar(kBarEmpty + st), (n / kStages - 1) & 1, a.err));
+        if (!ok) break;
         // a tile between the two query tiles' keys is not loaded
         const bool used = (j >= j0[0] && j < j1[0]) || (j >= j0[1] && j < j1[1]);
-        if (!used) {
-          if (lane == 0) mbar_arrive(bar(kBarFull + st));
-          if (kPaged && which < 2 && j + 1 < p1) id = page_at(j + 1);
-          continue;
+        if (lane == 0) {
+          if (used) mbar_arrive_expect_tx(bar(kBarFull + st), 2 * kTileBytes);
+          else mbar_arrive(bar(kBarFull + st));
         }
-        if (lane == 0) mbar_arrive_expect_tx(bar(kBarFull + st), 2 * kTileBytes);
         __syncwarp();
         const uint32_t dst = sbase + kOffStage + st * 2 * kTileBytes;
         if constexpr (kPaged) {
           if (which < 2) {
-            tma_load_4d(dst + which * kTileBytes + pg * (kTileBytes / npg), which ? &tmap_v : &tmap_k, bar(kBarFull + st), 0, hk, 0, id);
+            if (used)
+              tma_load_4d(dst + which * kTileBytes + pg * (kTileBytes / npg), which ? &tmap_v : &tmap_k, bar(kBarFull + st), 0, hk, 0, id);
             if (j + 1 < p1) id = page_at(j + 1);
           }
-        } else if (lane < 2) {
+        } else if (lane < 2 && used) {
           tma_load_4d(dst + lane * kTileBytes, lane ? &tmap_v : &tmap_k, bar(kBarFull + st), 0, j * kBN, hk, s.batch);
         }
       }
-    } else if (warp == kWarpMma) {
-      // ------------------------------- MMA issuer -------------------------------
+      if (!ok) {  // the copies in flight land before the CTA leaves
+        mbar_wait(bar(kBarQ), 0, a.err);
+        for (int n = max(j - p0 - kStages, 0); n < j - p0; ++n) mbar_wait(bar(kBarFull + n % kStages), (n / kStages) & 1, a.err);
+      }
+    } else if (warp < kWarpMma + kQT) {
+      // ------------------------------- MMA issuer of query tile t -------------------------------
+      const int t = warp - kWarpMma;
+      const int ja = t == 0 ? j0[0] : j0[1], jb = t == 0 ? j1[0] : j1[1];
       constexpr uint32_t idesc_qk = idesc_f16(kBM, kBN, kBF16 ? 1 : 0, 0, 0);
       constexpr uint32_t idesc_pv = idesc_f16(kBM, kHeadDim, kBF16 ? 1 : 0, 0, 1);
-      const uint64_t q_desc = smem_desc_sw128(sbase + kOffQ, 16, 1024);
+      const uint64_t q_desc = smem_desc_sw128(sbase + kOffQ + t * kTileBytes, 16, 1024);
       const uint64_t k_desc = smem_desc_sw128(sbase + kOffStage, 16, 1024);
       const uint64_t v_desc = smem_desc_sw128(sbase + kOffStage + kTileBytes, 16384, 1024);
       auto stage_off = [=](int j) -> uint64_t { return static_cast<uint64_t>(((j - p0) % kStages) * (2 * kTileBytes >> 4)); };
       auto wait_all = [&](int b, int parity) -> bool {
         return __all_sync(0xffffffffu, mbar_wait(bar(b), static_cast<uint32_t>(parity), a.err));
       };
-      auto qk = [&](int t, int j) {
-        issue_qk(tmem + t * 128, q_desc + t * (kTileBytes >> 4), k_desc + stage_off(j), idesc_qk, bar(kBarS + t));
+      auto full = [&](int j) -> bool { return wait_all(kBarFull + (j - p0) % kStages, ((j - p0) / kStages) & 1); };
+      const uint64_t qx_desc = smem_desc_noswz(sbase + kOffExtra, 128, 256);
+      const uint64_t kx_desc = smem_desc_noswz(sbase + kOffExtra + kExtraBytes, 128, 256);
+      auto qk = [&](int j) {
+        issue_qk(tmem + t * 128, q_desc, k_desc + stage_off(j), qx_desc,
+                 kx_desc + static_cast<uint64_t>(((j - p0) % kStages) * (kExtraBytes >> 4)), in_product ? 1u : 0u, idesc_qk, bar(kBarS + t));
       };
       bool ok = true;
-      if (p0 < p1) {
-        ok = wait_all(kBarQ, 0) && wait_all(kBarFull, 0);
-        if (ok) {
+      // tiles that only the other query tile reads are released as they come
+      for (int j = p0; j < ja && ok; ++j) {
+        ok = full(j);
+        if (ok && lane == 0) mbar_arrive(bar(kBarEmpty + (j - p0) % kStages));
+      }
+      if (ok && ja < jb) {
+        ok = wait_all(kBarQ, 0) && full(ja);
+        tc_fence_after();
+        if (ok) qk(ja);
+      }
+      for (int j = ja; j < jb && ok; ++j) {
+        const int n = j - ja;
+        if (j + 1 < jb) {
+          ok = full(j + 1) && wait_all(kBarSFree + t, n & 1);
+          if (!ok) break;
           tc_fence_after();
-#pragma unroll
-          for (int t = 0; t < kQT; ++t)
-            if (j0[t] == p0 && j1[t] > p0) qk(t, p0);
+          qk(j + 1);
         }
+        ok = wait_all(kBarP + t, n & 1);
+        if (!ok) break;
+        tc_fence_after();
+        issue_pv(tmem + kTmemO + t * kHeadDim, tmem + kTmemP + t * kHeadDim, v_desc + stage_off(j), idesc_pv, n > 0 ? 1u : 0u,
+                 bar(kBarO + t), bar(kBarEmpty + (j - p0) % kStages));
       }
-      for (int j = p0; j < p1 && ok; ++j) {
-        if (__any_sync(0xffffffffu, *abort_flag != 0)) {
-          ok = false;
-          break;
-        }
-        const int st = (j - p0) % kStages;
-        if (j + 1 < p1) ok = wait_all(kBarFull + (j + 1 - p0) % kStages, ((j + 1 - p0) / kStages) & 1);
-        const bool last1 = j >= j0[1] && j < j1[1];
-        bool any = false;
-#pragma unroll
-        for (int t = 0; t < kQT; ++t) {
-          if (ok && j + 1 >= j0[t] && j + 1 < j1[t]) {
-            if (j >= j0[t]) ok = wait_all(kBarSFree + t, (j - j0[t]) & 1);
-            if (ok) {
-              tc_fence_after();
-              qk(t, j + 1);
-            }
-          }
-          if (ok && j >= j0[t] && j < j1[t]) {
-            ok = wait_all(kBarP + t, (j - j0[t]) & 1);
-            if (ok) {
-              tc_fence_after();
-              issue_pv_group(tmem + kTmemO + t * kHeadDim, tmem + kTmemP + t * kHeadDim, v_desc + stage_off(j), idesc_pv,
-                             j > j0[t] ? 1u : 0u, bar(kBarO + t), bar(kBarEmpty + st), (t == kQT - 1 || !last1) ? 1u : 0u);
-              any = true;
-            }
-          }
-        }
-        if (ok && !any && lane == 0) mbar_arrive(bar(kBarEmpty + st));  // a tile between the two query tiles' keys
+      for (int j = jb; j < p1 && ok; ++j) {
+        ok = full(j);
+        if (ok && lane == 0) mbar_arrive(bar(kBarEmpty + (j - p0) % kStages));
       }
-      if (!ok && lane == 0) *abort_flag = 1;
     } else if (warp == kWarpKeys && per_key) {
       // ------------------------------- per-key bias and position -------------------------------
-      for (int j = p0; j < p1; ++j) {
+      const float inv = kLog2E / a.scale;  // bias / scale: a.scale = scale * log2(e) without a cap
+      // what the three 16-bit values can hold (and their product with 1 in fp32)
+      const float most = kBF16 ? 1e30f : 60000.f;
+      bool ok = true;
+      for (int j = p0; j < p1 && ok; ++j) {
         const int n = j - p0, st = n % kStages;
         float b[4], kp[4];
 #pragma unroll
@@ -357,23 +541,34 @@ __global__ void __launch_bounds__(kThreads, 1)
               there = id < a.pages;
               at = (static_cast<long long>(id) << a.page_shift) + (key & ((1 << a.page_shift) - 1));
             }
-            if (a.bias != nullptr && there) b[u] = bias_log2(__ldg(a.bias + at));
+            if (a.bias != nullptr && there) b[u] = __ldg(a.bias + at);
             if (a.slope != nullptr)
               kp[u] = !kPaged && a.kpos != nullptr ? __ldg(a.kpos + s.batch * a.kpos_sb + key) : static_cast<float>(key);
           }
         }
-        bool ok = *abort_flag == 0;
-        if (n >= kStages) ok = mbar_wait(bar(kBarEmpty + st), (n / kStages - 1) & 1, a.err) && ok;
-        if (!__all_sync(0xffffffffu, ok)) {
-          if (lane == 0) *abort_flag = 1;
-          break;
-        }
+        if (n >= kStages) ok = __all_sync(0xffffffffu, mbar_wait(bar(kBarEmpty + st), (n / kStages - 1) & 1, a.err));
+        if (!ok) break;
         float* dst = reinterpret_cast<float*>(smem + kOffKeys) + st * 2 * kBN;
+        bool add = a.cap != 0.f && a.bias != nullptr;
 #pragma unroll
         for (int u = 0; u < 4; ++u) {
-          dst[u * 32 + lane] = b[u];
-          dst[kBN + u * 32 + lane] = kp[u];
+          const int k = u * 32 + lane;
+          float in_softmax = bias_log2(b[u]);
+          if (in_product) {
+            const float x = b[u] * inv;
+            const bool fits = fabsf(x) <= most;  // not for NaN
+            const float hi = to_f32<T>(from_f32<T>(x)), mid = to_f32<T>(from_f32<T>(x - hi));
+            *reinterpret_cast<uint2*>(smem + kOffExtra + (1 + st) * kExtraBytes + (k >> 3) * 256 + (k & 7) * 16) =
+                fits ? make_uint2(pack2<T>(hi, mid), pack2<T>(x - hi - mid, 0.f)) : make_uint2(0u, 0u);
+            add = add || !fits;
+            if (fits) in_softmax = 0.f;
+          }
+          dst[k] = in_softmax;
+          dst[kBN + k] = kp[u];
         }
+        add = __any_sync(0xffffffffu, add);
+        if (in_product) fence_proxy_async_smem();
+        if (lane == 0) bias_flag[st] = add;
         __syncwarp();
         if (lane == 0) mbar_arrive(bar(kBarFull + st));
       }
@@ -386,7 +581,6 @@ __global__ void __launch_bounds__(kThreads, 1)
       cluster_wait();
     }
   } else {
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kRegsHigh));
     // ------------------------------- softmax -------------------------------
     const int t = warp >> 2;
     const int row = (warp & 3) * 32 + lane;
@@ -395,131 +589,74 @@ __global__ void __launch_bounds__(kThreads, 1)
     const uint32_t p_addr = tmem + lane_off + kTmemP + t * kHeadDim;
     const uint32_t o_addr = tmem + lane_off + kTmemO + t * kHeadDim;
     const int i = row_first + t * kBM + row;  // token of the sequence
-    const bool valid = i < s.rows;
-    const bool cap = a.cap != 0.f, has_bias = a.bias != nullptr, dist = a.slope != nullptr;
-    const bool formed = cap || has_bias || dist;  // the scores are brought to the log2 domain before the maximum
-    const float mul = formed ? 1.f : a.scale;
-    const float slope = dist ? __ldg(a.slope + head) * kLog2E : 0.f;
-    const float pos = dist && valid ? row_position<kPaged>(a, s, i) : 0.f;
-    float m_run = -INFINITY, l_run = 0.f;
-    bool ok = true;
+    const float slope = kForm == 2 && a.slope != nullptr ? __ldg(a.slope + head) * kLog2E : 0.f;
+    const float pos = kForm == 2 && a.slope != nullptr && valid ? row_position<kPaged>(a, s, i) : 0.f;
+    // keys that every row of the warp sees
+    const int all_lo = __reduce_max_sync(0xffffffffu, valid ? be.x : 0);
+    const int all_hi = __reduce_min_sync(0xffffffffu, valid ? be.y : 0x7fffffff);
     const int ja = t == 0 ? j0[0] : j0[1], jb = t == 0 ? j1[0] : j1[1];
+    float m_run = -INFINITY, l_run = 0.f;  // the running maximum is a whole number, so that a rescaling is exact
+    bool ok = true;
+    auto wait_for = [&](int b, int parity) {
+      if (ok) ok = mbar_wait(bar(b), static_cast<uint32_t>(parity), a.err);
+    };
 
-    for (int j = ja; j < jb; ++j) {
+    // one key tile: scores, probabilities, P
+    auto step = [&](auto full_form, int j, const float* keys, bool add) {
+      constexpr bool kFull = decltype(full_form)::value;
       const int n = j - ja;
-      ok = ok && !*abort_flag;
-      if (ok) ok = mbar_wait(bar(kBarS + t), n & 1, a.err);
-      if (ok && per_key) ok = mbar_wait(bar(kBarFull + (j - p0) % kStages), ((j - p0) / kStages) & 1, a.err);
-      ok = __all_sync(0xffffffffu, ok);
-      if (!ok) break;
-      uint32_t r[kBN];
-      tc_fence_after();
-#pragma unroll
-      for (int c = 0; c < kBN; c += 32) tmem_ld32x32b_x32_nowait(s_addr + c, *reinterpret_cast<uint32_t(*)[32]>(&r[c]));
-      tmem_wait_ld();
-#pragma unroll
-      for (int c = 0; c < kBN; c += 32) reg_fence32(*reinterpret_cast<uint32_t(*)[32]>(&r[c]));
-      tc_fence_before();
-      mbar_arrive(bar(kBarSFree + t));
-      if (formed) {
-        const float* keys = reinterpret_cast<const float*>(smem + kOffKeys) + ((j - p0) % kStages) * 2 * kBN;
-        if (cap) {
-#pragma unroll
-          for (int c = 0; c < kBN; ++c) r[c] = f2u(a.cap * tanh_fast(u2f(r[c]) * a.scale));
-          if (has_bias) {
-#pragma unroll
-            for (int c = 0; c < kBN; c += 4) {
-              const float4 b = *reinterpret_cast<const float4*>(keys + c);
-              r[c] = f2u(u2f(r[c]) + b.x);
-              r[c + 1] = f2u(u2f(r[c + 1]) + b.y);
-              r[c + 2] = f2u(u2f(r[c + 2]) + b.z);
-              r[c + 3] = f2u(u2f(r[c + 3]) + b.w);
-            }
-          }
-        } else {
-          // without a bias the ring holds zeros
-          const uint64_t sc = pk2(a.scale, a.scale);
-#pragma unroll
-          for (int c = 0; c < kBN; c += 4) {
-            const float4 b = *reinterpret_cast<const float4*>(keys + c);
-            float x0, x1;
-            upk2(ffma2(pk2(u2f(r[c]), u2f(r[c + 1])), sc, pk2(b.x, b.y)), x0, x1);
-            r[c] = f2u(x0);
-            r[c + 1] = f2u(x1);
-            upk2(ffma2(pk2(u2f(r[c + 2]), u2f(r[c + 3])), sc, pk2(b.z, b.w)), x0, x1);
-            r[c + 2] = f2u(x0);
-            r[c + 3] = f2u(x1);
-          }
+      const int key0 = j * kBN;
+      uint32_t p[kBN / 2];
+      float alpha = 1.f;  // what O is to be multiplied by
+      bool need;
+      {
+        uint32_t r[kHalf];
+        tmem_ld32x32b_x32_nowait(s_addr, *reinterpret_cast<uint32_t(*)[32]>(&r[0]));
+        tmem_ld32x32b_x32_nowait(s_addr + 32, *reinterpret_cast<uint32_t(*)[32]>(&r[32]));
+        tmem_wait_ld();
+        reg_fence32(*reinterpret_cast<uint32_t(*)[32]>(&r[0]));
+        reg_fence32(*reinterpret_cast<uint32_t(*)[32]>(&r[32]));
+        const float mul = form_scores<kFull>(r, a, keys, add, slope, pos, be.x - key0, be.y - key0, key0 < all_lo || key0 + kHalf > all_hi);
+        const float m_new = max_of(r) * mul;
+        const bool grow = m_new > m_run + kRescale;
+        need = __any_sync(0xffffffffu, grow);
+        if (need) {
+          const float m_tgt = grow ? ceilf(m_new) : m_run;
+          alpha = grow ? ex2_approx(m_run - m_tgt) : 1.f;
+          l_run *= alpha;
+          m_run = m_tgt;
         }
-        if (dist) {
-#pragma unroll
-          for (int c = 0; c < kBN; c += 4) {
-            const float4 p = *reinterpret_cast<const float4*>(keys + kBN + c);
-            r[c] = f2u(fmaf(-slope, fabsf(pos - p.x), u2f(r[c])));
-            r[c + 1] = f2u(fmaf(-slope, fabsf(pos - p.y), u2f(r[c + 1])));
-            r[c + 2] = f2u(fmaf(-slope, fabsf(pos - p.z), u2f(r[c + 2])));
-            r[c + 3] = f2u(fmaf(-slope, fabsf(pos - p.w), u2f(r[c + 3])));
-          }
-        }
+        l_run += probabilities<T>(r, mul, m_run, p);
       }
       {
-        const int lo = min(max(be.x - j * kBN, 0), kBN), hi = min(max(be.y - j * kBN, 0), kBN);
-        if (__any_sync(0xffffffffu, lo > 0 || hi < kBN)) {
+        uint32_t r[kHalf];
+        tmem_ld32x32b_x32_nowait(s_addr + kHalf, *reinterpret_cast<uint32_t(*)[32]>(&r[0]));
+        tmem_ld32x32b_x32_nowait(s_addr + kHalf + 32, *reinterpret_cast<uint32_t(*)[32]>(&r[32]));
+        tmem_wait_ld();
+        reg_fence32(*reinterpret_cast<uint32_t(*)[32]>(&r[0]));
+        reg_fence32(*reinterpret_cast<uint32_t(*)[32]>(&r[32]));
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(bar(kBarSFree + t));
+        const float mul = form_scores<kFull>(r, a, keys + kHalf, add, slope, pos, be.x - key0 - kHalf, be.y - key0 - kHalf,
+                                             key0 + kHalf < all_lo || key0 + kBN > all_hi);
+        const float m_new = max_of(r) * mul;
+        const bool grow = m_new > m_run + kRescale;
+        if (__any_sync(0xffffffffu, grow)) {  // the first half's probabilities are rescaled too, by a power of two
+          need = true;
+          const float m_tgt = grow ? ceilf(m_new) : m_run;
+          const float f = grow ? ex2_approx(m_run - m_tgt) : 1.f;
+          alpha *= f;
+          l_run *= f;
+          m_run = m_tgt;
 #pragma unroll
-          for (int w = 0; w < kBN / 32; ++w) {
-            // bits [lo, hi) of this word of 32 columns
-            const int l0 = min(max(lo - 32 * w, 0), 32), h0 = min(max(hi - 32 * w, 0), 32);
-            const uint32_t up = h0 >= 32 ? 0xffffffffu : (1u << h0) - 1u;
-            const uint32_t dn = l0 >= 32 ? 0u : 0xffffffffu << l0;
-            const uint32_t see = up & dn;
-#pragma unroll
-            for (int c = 0; c < 32; ++c)
-              if (!((see >> c) & 1u)) r[32 * w + c] = f2u(-INFINITY);
-          }
+          for (int c = 0; c < kHalf / 2; ++c) p[c] = scale2<T>(p[c], f);
         }
+        l_run += probabilities<T>(r, mul, m_run, p + kHalf / 2);
       }
-      float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-#pragma unroll
-      for (int c = 0; c < kBN; c += 8) {
-#pragma unroll
-        for (int u = 0; u < 4; ++u) mx[u] = fmax3(mx[u], u2f(r[c + 2 * u]), u2f(r[c + 2 * u + 1]));
-      }
-      const float m_new = fmaxf(m_run, fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * mul);
-      const bool grow = m_new > m_run + kRescale;
-      const bool need = __any_sync(0xffffffffu, grow);
-      const float m_tgt = grow ? m_new : m_run;
-      const float alpha = grow ? ex2_approx(m_run - m_tgt) : 1.f;
-      const float m_use = m_tgt == -INFINITY ? 0.f : m_tgt;
-      const uint64_t neg_m2 = pk2(-m_use, -m_use), mul2 = pk2(mul, mul);
-      uint64_t ls0 = pk2(0.f, 0.f), ls1 = pk2(0.f, 0.f);
-#pragma unroll
-      for (int c = 0; c < kBN / 2; ++c) {
-        float e0, e1, q0, q1;
-        upk2(ffma2(pk2(u2f(r[2 * c]), u2f(r[2 * c + 1])), mul2, neg_m2), e0, e1);
-        if ((c & 7) < kPolyPairs) {
-          exp2_poly2(e0, e1, q0, q1);
-          // a hidden key's probability is exactly 0 (the polynomial's 2^-125 times a hidden 3e38 would show), and
-          // a score that is NaN stays NaN
-          upk2(ffma2(pk2(e0, e1), pk2(0.f, 0.f), pk2(q0, q1)), q0, q1);
-          q0 = e0 < -125.f ? 0.f : q0;
-          q1 = e1 < -125.f ? 0.f : q1;
-        } else {
-          q0 = ex2_approx(e0);
-          q1 = ex2_approx(e1);
-        }
-        if (c & 1) ls1 = fadd2(ls1, pk2(q0, q1));
-        else ls0 = fadd2(ls0, pk2(q0, q1));
-        r[c] = pack2<T>(q0, q1);
-      }
-      float a0, a1, b0, b1;
-      upk2(ls0, a0, a1);
-      upk2(ls1, b0, b1);
-      l_run = l_run * alpha + ((a0 + a1) + (b0 + b1));
-      m_run = m_tgt;
       if (n > 0) {
-        // PV_t(j-1) is complete before P_t is overwritten or O_t rescaled
-        ok = __all_sync(0xffffffffu, mbar_wait(bar(kBarO + t), (n - 1) & 1, a.err));
-        if (!ok) break;
+        wait_for(kBarO + t, (n - 1) & 1);  // PV(n - 1) has read P, and O is at rest
+        __syncwarp();
         tc_fence_after();
         if (need) {
 #pragma unroll 1
@@ -532,17 +669,38 @@ __global__ void __launch_bounds__(kThreads, 1)
           }
         }
       }
-      tmem_st32x32b_x32(p_addr, *reinterpret_cast<const uint32_t(*)[32]>(&r[0]));
-      tmem_st32x32b_x32(p_addr + 32, *reinterpret_cast<const uint32_t(*)[32]>(&r[32]));
+      tmem_st32x32b_x32(p_addr, *reinterpret_cast<const uint32_t(*)[32]>(&p[0]));
+      tmem_st32x32b_x32(p_addr + 32, *reinterpret_cast<const uint32_t(*)[32]>(&p[32]));
       tmem_wait_st();
       tc_fence_before();
-      mbar_arrive(bar(kBarP + t));
+      __syncwarp();
+      if (lane == 0) mbar_arrive(bar(kBarP + t));
+    };
+#pragma unroll 1
+    for (int j = ja; j < jb; ++j) {
+      const int st = (j - p0) % kStages;
+      {
+        // the scores and the tile's keys, looked at together
+        const uint32_t ps = (j - ja) & 1, pf = ((j - p0) / kStages) & 1;
+        const bool s_there = mbar_try_wait(bar(kBarS + t), ps), keys_there = !per_key || mbar_try_wait(bar(kBarFull + st), pf);
+        if (!s_there) wait_for(kBarS + t, ps);
+        if (!keys_there) wait_for(kBarFull + st, pf);
+      }
+      __syncwarp();
+      tc_fence_after();
+      const float* keys = reinterpret_cast<const float*>(smem + kOffKeys) + st * 2 * kBN;
+      const bool add = per_key && bias_flag[st] != 0;
+      if constexpr (kForm == 0) step(std::false_type{}, j, keys, false);
+      else if constexpr (kForm == 2) step(std::true_type{}, j, keys, add);
+      else if (add) step(std::true_type{}, j, keys, true);
+      else step(std::false_type{}, j, keys, false);
     }
-    if (ok && jb > ja) ok = __all_sync(0xffffffffu, mbar_wait(bar(kBarO + t), (jb - ja - 1) & 1, a.err));
     uint32_t o[kHeadDim];
 #pragma unroll
     for (int c = 0; c < kHeadDim; ++c) o[c] = 0u;
-    if (ok && jb > ja) {
+    if (jb > ja) {
+      wait_for(kBarO + t, (jb - ja - 1) & 1);
+      __syncwarp();
       tc_fence_after();
       tmem_ld32x32b_x32_nowait(o_addr, *reinterpret_cast<uint32_t(*)[32]>(&o[0]));
       tmem_ld32x32b_x32_nowait(o_addr + 32, *reinterpret_cast<uint32_t(*)[32]>(&o[32]));
@@ -550,7 +708,6 @@ __global__ void __launch_bounds__(kThreads, 1)
       reg_fence32(*reinterpret_cast<uint32_t(*)[32]>(&o[0]));
       reg_fence32(*reinterpret_cast<uint32_t(*)[32]>(&o[32]));
     }
-    if (!ok) *abort_flag = 1;
     uint8_t* out_head = static_cast<uint8_t*>(a.out) + 2 * (s.batch * a.o_sb + head * a.o_sh);
     if (split == 1) {
       bool again = false;
@@ -574,9 +731,9 @@ __global__ void __launch_bounds__(kThreads, 1)
       __syncwarp();  // a row's first result is written before its second
       unsigned rows = __ballot_sync(0xffffffffu, again);
       while (rows) {
-        const int b = __ffs(rows) - 1;
+        const int e = __ffs(rows) - 1;
         rows &= rows - 1;
-        exact_row<T, kPaged>(a, s, row_first + t * kBM + (warp & 3) * 32 + b, head);
+        exact_row<T, kPaged>(a, s, row_first + warp * 32 + e, head);
       }
     } else {
       // The parts overlay Q and the ring: every load into them has been consumed, and every tensor-core read of
@@ -589,7 +746,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       *reinterpret_cast<float2*>(smem + kOffPartMl + 8 * (t * kBM + row)) = make_float2(m_run, l_run);
       cluster_arrive();
       cluster_wait();
-      const int per = kQT * kBM / split;  // rows joined by this CTA, 16 lanes per row
+      const int per = kQT * kBM / split;  // rows joined by this CTA, 16 lanes per row; per * 16 is a multiple of 256 threads
       for (int x = threadIdx.x; x < per * 16; x += kSoftmaxWarps * 32) {
         const int rr = piece * per + (x >> 4), c4 = (x & 15) * 4;
         const uint32_t ml = sbase + kOffPartMl + 8 * rr, ov = sbase + 4 * (rr * kPartStride + c4);
@@ -615,10 +772,9 @@ __global__ void __launch_bounds__(kThreads, 1)
           const float inv = sum == 0.f ? 0.f : 1.f / sum;
           *reinterpret_cast<uint2*>(out_head + 2 * ((s.row0 + tok) * a.o_sn + c4)) =
               sum == 0.f ? make_uint2(0u, 0u) : make_uint2(pack2<T>(acc.x * inv, acc.y * inv), pack2<T>(acc.z * inv, acc.w * inv));
-          const float z = fmaf(acc.x, 0.f, fmaf(acc.y, 0.f, fmaf(acc.z, 0.f, acc.w * 0.f)));
+          const float z = fmaf(acc.x, 0.f, fmaf(acc.y, 0.f, fmaf(acc.z, 0.f, acc.w * 0.f)));  // NaN unless all are finite
           again = sum != 0.f && !(z * inv == 0.f);
         }
-        // per * 16 is a multiple of 256, so whole warps run this together
         __syncwarp();  // a row's first result is written before its second
         const unsigned bad = __ballot_sync(0xffffffffu, again);
         const int first_row = row_first + piece * per + ((x - lane) >> 4);
@@ -661,20 +817,15 @@ int pool_map(CUtensorMap* map, const void* base, int dtype, const AttnView& a) {
                           str, b, CU_TENSOR_MAP_SWIZZLE_128B);
 }
 
-template <typename T, bool kPaged>
-int launch(const AttnView& a, const CUtensorMap& tq, const CUtensorMap& tk, const CUtensorMap& tv, long long blocks, int split,
+template <typename T, bool kPaged, int kForm>
+int launch_form(const AttnView& a, const CUtensorMap& tq, const CUtensorMap& tk, const CUtensorMap& tv, long long blocks, int split,
            cudaStream_t st) {
-  auto kernel = masked_attention_tc_kernel<T, kPaged>;
-  // per device: the opt-in to the shared memory, and the register count that the split inside the kernel needs
+  auto kernel = masked_attention_tc_kernel<T, kPaged, kForm>;
+  // per device: the opt-in to the shared memory
   static std::atomic<bool> ready[64];
   int dev = 0;
   VB200_CHECK_CUDA(cudaGetDevice(&dev), "cudaGetDevice");
   if (dev < 0 || dev >= 64 || !ready[dev].load(std::memory_order_acquire)) {
-    cudaFuncAttributes fa{};
-    VB200_CHECK_CUDA(cudaFuncGetAttributes(&fa, kernel), "cudaFuncGetAttributes");
-    if (fa.numRegs != kLaunchRegs)
-      return set_error(VB200_EUNSUPPORTED, "masked_attention_tc_kernel was built with %d registers per thread; its register split needs %d",
-                       fa.numRegs, kLaunchRegs);
     VB200_CHECK_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemBytes), "cudaFuncSetAttribute");
     if (dev >= 0 && dev < 64) ready[dev].store(true, std::memory_order_release);
   }
@@ -694,6 +845,14 @@ int launch(const AttnView& a, const CUtensorMap& tq, const CUtensorMap& tk, cons
   return VB200_OK;
 }
 
+template <typename T, bool kPaged>
+int launch(const AttnView& a, const CUtensorMap& tq, const CUtensorMap& tk, const CUtensorMap& tv, long long blocks, int split,
+           cudaStream_t st) {
+  if (a.cap != 0.f || a.slope != nullptr) return launch_form<T, kPaged, 2>(a, tq, tk, tv, blocks, split, st);
+  return a.bias != nullptr ? launch_form<T, kPaged, 1>(a, tq, tk, tv, blocks, split, st)
+                           : launch_form<T, kPaged, 0>(a, tq, tk, tv, blocks, split, st);
+}
+
 }  // namespace
 
 int tile_attention(int dtype, bool paged, const AttnView& a, long long most_keys, cudaStream_t st) {
@@ -708,7 +867,7 @@ int tile_attention(int dtype, bool paged, const AttnView& a, long long most_keys
   if (sms > 0) {
     double best = 0.0;
     for (int k = 1; k <= 8; k *= 2) {
-      if (k > 1 && k > tiles) break;
+      if (k > 1 && 2 * k > tiles) break;
       const double cost = static_cast<double>((items * k + sms - 1) / sms) * (1.0 / k + 3.0 / tiles);
       if (k == 1 || cost < best - 1e-9) {
         best = cost;

@@ -18,7 +18,7 @@ int error_word_address(unsigned** p) {
 }
 
 int fill_mods(const vb200_score_mods* m, AttnView& a) {
-  VB200_REQUIRE(std::isfinite(m->scale), "attention: scale must be finite");
+  VB200_REQUIRE(std::isfinite(m->scale) && m->scale > 0.f, "attention: scale must be positive and finite");
   VB200_REQUIRE(m->softcap >= 0.f && std::isfinite(m->softcap), "attention: softcap must be 0 (none) or positive and finite");
   a.range = m->key_range;
   a.range_sb = m->key_range_sb;

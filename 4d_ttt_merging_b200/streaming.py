@@ -136,9 +136,7 @@ def masked_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, log_key_
         raise ValueError("q, k and v must have one dtype")
     dt = C.dtype_code(q.dtype)
     softcap = _positive("softcap", softcap)
-    scale = 0.125 if scale is None else float(scale)
-    if not math.isfinite(scale):
-        raise ValueError("scale must be finite")
+    scale = 0.125 if scale is None else _positive("scale", scale)
     if distance_slope is None and (query_position is not None or key_position is not None):
         raise ValueError("positions are used with distance_slope only")
     if distance_slope is not None and distance_slope.shape != (H,):
@@ -335,9 +333,7 @@ def paged_attention(q: torch.Tensor, cache: PagedCache, sequence, offsets, *, ca
     if q.dtype != cache.k.dtype:
         raise ValueError(f"the cache holds {cache.k.dtype}, q is {q.dtype}")
     softcap = _positive("softcap", softcap)
-    scale = 0.125 if scale is None else float(scale)
-    if not math.isfinite(scale):
-        raise ValueError("scale must be finite")
+    scale = 0.125 if scale is None else _positive("scale", scale)
     if distance_slope is not None and distance_slope.shape != (H,):
         raise ValueError(f"distance_slope must be [{H}]")
     if key_range is not None and (key_range.dtype != torch.int32 or key_range.shape != (rows, 2)):

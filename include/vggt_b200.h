@@ -133,7 +133,7 @@ typedef struct {
   int64_t q_position_sb;
   const float* k_position;   /* [B][Nk], NULL: j                                                    */
   int64_t k_position_sb;
-  float scale;               /* usually 1 / 8                                                       */
+  float scale;               /* positive, usually 1 / 8                                             */
   float softcap;             /* 0: none                                                             */
 } vb200_score_mods;
 /* q, k, v, out with strides {batch, head, token}, channel stride 1; rows 16-byte aligned.  mods may be

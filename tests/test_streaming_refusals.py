@@ -28,8 +28,9 @@ def test_masked_attention_refusals(pkg):
     for cap in (0.0, -1.0, float("nan"), float("inf")):
         with pytest.raises(ValueError, match="softcap"):
             f(q, k, k, softcap=cap)
-    with pytest.raises(ValueError, match="scale"):
-        f(q, k, k, scale=float("inf"))
+    for scale in (0.0, -0.1, float("inf")):
+        with pytest.raises(ValueError, match="scale"):
+            f(q, k, k, scale=scale)
     with pytest.raises(ValueError, match="distance_slope"):
         f(q, k, k, distance_slope=torch.zeros(2))
     with pytest.raises(ValueError, match="positions are used"):
