@@ -69,12 +69,14 @@ _SIGNATURES = {
     "vb200_masked_attention": (
         _c_int,
         [_c_int, _c_vp, _c_vp, _c_vp, _c_vp, _c_i64, _c_i64, _c_i64, _c_i64, _c_i64, _c_i64, _p_i64, _p_i64, _p_i64,
-         _p_i64, _p_mods, _c_vp],
+         _p_i64, _p_mods, _c_vp, _c_size, _c_vp],
     ),
+    "vb200_masked_attention_workspace_size": (_c_size, [_c_int, _c_i64, _c_i64, _c_i64, _c_i64, _c_i64]),
+    "vb200_paged_attention_workspace_size": (_c_size, [_c_int, _c_i64, _c_i64, _p_cache, _c_i64]),
     "vb200_paged_attention": (
         _c_int,
         [_c_int, _c_vp, _c_vp, _c_i64, _c_i64, _c_i64, _p_i64, _p_i64, _p_cache, _c_vp, _c_vp, _c_i64, _c_int, _p_mods,
-         _c_vp],
+         _c_vp, _c_size, _c_vp],
     ),
     "vb200_cache_append_workspace_size": (_c_size, [_c_i64, _c_i64, _c_i64]),
     "vb200_cache_append": (

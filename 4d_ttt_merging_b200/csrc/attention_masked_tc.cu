@@ -9,11 +9,10 @@
 //                pages outside the sequence read a coordinate outside the pool and fill with zeros).
 //   warps 9, 10  one MMA stream per query tile: S(j + 1) = Q K_{j+1}^T as soon as S(j) is in registers, then
 //                O += P(j) V_j.
-//   warp 11      per key: bias and position of the tile, into the ring (only when there are any).  Without a cap the
-//                bias rides in the QK product: an extra K=16 chunk holds 1, 1, 1 in columns 0 to 2 of every query
-//                row and bias / scale, split into three 16-bit values that add up to its 24 bits, in those of the
-//                key row.  A tile with a bias that does not fit (infinite, the type's lowest value) gets it in the
-//                softmax instead.
+//   warp 11      per key: bias and position of the tile, into the ring (only when there are any).  A bias alone rides
+//                in the QK product: an extra K=16 chunk holds 1, 1, 1 in columns 0 to 2 of every query row and bias /
+//                scale, split into three 16-bit values that add up to its 24 bits, in those of the key row (adding it
+//                in the softmax measured 20% slower).
 // TMEM: S_t at 128 t, P_t at 256 + 64 t (16-bit, the A operand of PV), O_t at 384 + 64 t.
 //
 // The two warps of an SM sub-partition compute their exponentials at the same time and leave the unit idle at the same time
@@ -31,15 +30,17 @@
 // the PV product, so a row that comes out with a value that is not finite is computed again, key by key, by its
 // warp (exact_row): rows are right whatever the hidden values are, and finite inputs pay one test per row.
 //
-// When the blocks do not fill the GPU, the key tiles of each are split over a cluster of 2, 4 or 8 CTAs;
-// (O, maximum, sum) of the parts meet in distributed shared memory and are joined in rank order (no workspace, no second
-// launch, the same bits at every run).
+// The last, partly filled wave of blocks is split over the keys (up to 8 parts a block).  Every part writes O, maximum
+// and sum to the workspace and counts itself; the part that comes last joins all of them in order, so the result
+// does not depend on which one that is.  (Parts in a cluster, joined in distributed shared memory, need whole clusters of
+// SMs at a time, 128 of 148 for clusters of 8, and one split for all blocks: a frame of 1041 rows over 33,969 keys took 405 us.)
 //
 // The running maximum is lazy: O is rescaled only when a row's maximum grows by more than 2^8.  Probabilities are
 // rounded to the value type for the PV product; sums, maxima and O are fp32.
 #include <cudaTypedefs.h>
 
 #include <atomic>
+#include <cstring>
 
 #include "attention_view.cuh"
 #include "host_common.h"
@@ -65,11 +66,10 @@ constexpr int kOffKeys = kOffExtra + (1 + kStages) * kExtraBytes;  // [stage][2]
 constexpr int kOffBar = kOffKeys + kStages * 2 * kBN * 4;
 constexpr int kBarQ = 0, kBarFull = 1, kBarEmpty = kBarFull + kStages, kBarS = kBarEmpty + kStages, kBarSFree = kBarS + kQT,
               kBarP = kBarSFree + kQT, kBarO = kBarP + kQT, kNumBars = kBarO + kQT;
-constexpr int kOffMisc = kOffBar + kNumBars * 8;  // TMEM base; per query tile: first and last key; per stage: bias in the softmax
-constexpr int kSmemBytes = kOffMisc + 48 + 1024;
-constexpr int kPartStride = kHeadDim + 4;  // floats; parts of a split overlay Q and the ring
-constexpr int kOffPartMl = kQT * kBM * kPartStride * 4;
-static_assert(kOffPartMl + kQT * kBM * 8 <= kOffKeys, "the parts fit");
+constexpr int kOffMisc = kOffBar + kNumBars * 8;  // TMEM base; per query tile: first and last key
+constexpr int kSmemBytes = kOffMisc + 32 + 1024;
+constexpr int kMaxSplit = 8;
+constexpr size_t kPartBytes = static_cast<size_t>(kQT) * kBM * (kHeadDim + 2) * 4;  // O, then (maximum, sum), of a block's rows
 constexpr uint32_t kTmemCols = 512, kTmemP = 256, kTmemO = 384;
 
 // S = Q K^T: four K=16 steps of head_dim 64, the first overwrites, and with use_x the bias chunk (xa, xb).
@@ -127,23 +127,13 @@ __device__ __forceinline__ void issue_pv(uint32_t d, uint32_t a, uint64_t b, uin
 __device__ __forceinline__ float u2f(uint32_t u) { return __uint_as_float(u); }
 __device__ __forceinline__ uint32_t f2u(float f) { return __float_as_uint(f); }
 
-__device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release;" ::: "memory"); }
-__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire;" ::: "memory"); }
-__device__ __forceinline__ uint32_t peer_address(uint32_t addr, uint32_t rank) {
-  uint32_t r;
-  asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(addr), "r"(rank));
-  return r;
-}
-__device__ __forceinline__ float4 peer_load4(uint32_t addr) {
-  float4 v;
-  asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(addr));
-  return v;
-}
-__device__ __forceinline__ float2 peer_load2(uint32_t addr) {
-  float2 v;
-  asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(v.x), "=f"(v.y) : "r"(addr));
-  return v;
-}
+// Blocks below n_full run whole; the rest in `split` parts each.
+struct TileSplit {
+  int blocks;        // row blocks (an upper bound where sequences are ragged)
+  int n_full, split;
+  uint8_t* parts;    // [blocks * H - n_full][split][kPartBytes]
+  unsigned* counters;  // [blocks * H - n_full], zero at the launch
+};
 
 // One output row by one warp, key by key, two channels per lane: for rows whose tile result is not finite.
 template <typename T, bool kPaged>
@@ -155,36 +145,44 @@ __device__ __noinline__ void exact_row(const AttnView& a, AttnSeq s, int i, int 
   const T* q = static_cast<const T*>(a.q) + s.batch * a.q_sb + head * a.q_sh + static_cast<long long>(s.row0 + i) * a.q_sn + 2 * lane;
   const float q0 = to_f32<T>(q[0]) * a.scale, q1 = to_f32<T>(q[1]) * a.scale;
   float m = -INFINITY, l = 0.f, o0 = 0.f, o1 = 0.f;
-  for (int j = be.x; j < be.y; ++j) {
-    long long ko, vo, bo;
-    if constexpr (kPaged) {
-      const int id = page_of(a, s, j >> a.page_shift), at = j & ((1 << a.page_shift) - 1);
-      if (id >= a.pages) continue;
-      ko = id * a.k_sb + at * a.k_sn;
-      vo = id * a.v_sb + at * a.v_sn;
-      bo = (static_cast<long long>(id) << a.page_shift) + at;
-    } else {
-      ko = s.batch * a.k_sb + j * a.k_sn;
-      vo = s.batch * a.v_sb + j * a.v_sn;
-      bo = s.batch * a.bias_sb + j;
+  for (int j0 = be.x; j0 < be.y; j0 += 32) {
+    // each lane looks at one key: where it lies, its bias; keys of mass 0 are left out
+    long long ko = 0, vo = 0;
+    float b = -INFINITY, kp = 0.f;
+    if (j0 + lane < be.y) {
+      const int j = j0 + lane;
+      b = 0.f;
+      if constexpr (kPaged) {
+        const int id = page_of(a, s, j >> a.page_shift), at = j & ((1 << a.page_shift) - 1);
+        ko = id * a.k_sb + at * a.k_sn;
+        vo = id * a.v_sb + at * a.v_sn;
+        if (id >= a.pages) b = -INFINITY;
+        else if (a.bias != nullptr) b = bias_log2(__ldg(a.bias + (static_cast<long long>(id) << a.page_shift) + at));
+      } else {
+        ko = s.batch * a.k_sb + j * a.k_sn;
+        vo = s.batch * a.v_sb + j * a.v_sn;
+        if (a.bias != nullptr) b = bias_log2(__ldg(a.bias + s.batch * a.bias_sb + j));
+      }
+      kp = !kPaged && a.slope != nullptr && a.kpos != nullptr ? __ldg(a.kpos + s.batch * a.kpos_sb + j) : static_cast<float>(j);
     }
-    const float b = a.bias == nullptr ? 0.f : bias_log2(__ldg(a.bias + bo));
-    if (b == -INFINITY) continue;  // mass 0
-    const T* k = static_cast<const T*>(a.k) + ko + hk * a.k_sh + 2 * lane;
-    const T* v = static_cast<const T*>(a.v) + vo + hk * a.v_sh + 2 * lane;
-    float x = q0 * to_f32<T>(k[0]) + q1 * to_f32<T>(k[1]);
+    for (unsigned some = __ballot_sync(0xffffffffu, b != -INFINITY); some != 0; some &= some - 1) {
+      const int from = __ffs(some) - 1;
+      const T* k = static_cast<const T*>(a.k) + __shfl_sync(0xffffffffu, ko, from) + hk * a.k_sh + 2 * lane;
+      const T* v = static_cast<const T*>(a.v) + __shfl_sync(0xffffffffu, vo, from) + hk * a.v_sh + 2 * lane;
+      float x = q0 * to_f32<T>(k[0]) + q1 * to_f32<T>(k[1]);
 #pragma unroll
-    for (int d = 16; d >= 1; d >>= 1) x += __shfl_xor_sync(0xffffffffu, x, d);
-    if (a.cap != 0.f) x = a.cap * tanh_fast(x);
-    x += b;
-    if (a.slope != nullptr)
-      x = fmaf(-slope, fabsf(pos - (!kPaged && a.kpos != nullptr ? __ldg(a.kpos + s.batch * a.kpos_sb + j) : static_cast<float>(j))), x);
-    const float mn = fmaxf(m, x), mu = mn == -INFINITY ? 0.f : mn;
-    const float corr = ex2_approx(m - mu), p = ex2_approx(x - mu);
-    m = mn;
-    l = l * corr + p;
-    o0 = o0 * corr + p * to_f32<T>(v[0]);
-    o1 = o1 * corr + p * to_f32<T>(v[1]);
+      for (int d = 16; d >= 1; d >>= 1) x += __shfl_xor_sync(0xffffffffu, x, d);
+      if (a.cap != 0.f) x = a.cap * tanh_fast(x);
+      x += __shfl_sync(0xffffffffu, b, from);
+      const float at = __shfl_sync(0xffffffffu, kp, from);
+      if (a.slope != nullptr) x = fmaf(-slope, fabsf(pos - at), x);
+      const float mn = fmaxf(m, x), mu = mn == -INFINITY ? 0.f : mn;
+      const float corr = ex2_approx(m - mu), p = ex2_approx(x - mu);
+      m = mn;
+      l = l * corr + p;
+      o0 = o0 * corr + p * to_f32<T>(v[0]);
+      o1 = o1 * corr + p * to_f32<T>(v[1]);
+    }
   }
   T* out = static_cast<T*>(a.out) + s.batch * a.o_sb + head * a.o_sh + static_cast<long long>(s.row0 + i) * a.o_sn + 2 * lane;
   out[0] = from_f32<T>(l == 0.f ? 0.f : o0 / l);
@@ -204,10 +202,18 @@ __device__ __forceinline__ uint32_t pack2(float lo, float hi) {
   return sizeof(T) == 2 && std::is_same<T, __nv_bfloat16>::value ? pack_bf16x2(lo, hi) : pack_f16x2(lo, hi);
 }
 
-// tanh(y) / y for y^2 <= 1 as a polynomial in y^2, fitted here for minimum maximum relative error (least squares
-// reweighted to equal ripples: 6e-7, 7e-7 evaluated in fp32).
-constexpr float kTanh0 = 0.9999994039535522f, kTanh1 = -0.3332904279232025f, kTanh2 = 0.13281433284282684f,
-                kTanh3 = -0.051605671644210815f, kTanh4 = 0.016743112355470657f, kTanh5 = -0.0030670592095702887f;
+// tanh(y) / y as a polynomial in y^2, fitted here for minimum maximum relative error (least squares reweighted to equal
+// ripples): degree 3 for |y| <= 1/2 (5e-7), degree 5 for |y| <= 1 (6e-7); 7e-7 evaluated in fp32.
+constexpr double kTanhNear[4] = {0.999999463558197, -0.33326318860054016, 0.13190296292304993, -0.04440222308039665};
+constexpr double kTanhFar[6] = {0.9999994039535522,    -0.3332904279232025,  0.13281433284282684,
+                                -0.051605671644210815, 0.016743112355470657, -0.0030670592095702887};
+
+// The same for cap * log2(e) * tanh(r s) / r in r^2, each coefficient twice for the packed instructions.
+// A polynomial whose coefficients leave the range of normal numbers (a cap far from the scale) has limit -1 and is not used.
+struct CapPoly {
+  uint64_t near_[4], far_[6];
+  float near_limit, far_limit;  // 1/2 and 1
+};
 
 __device__ __forceinline__ float max_of(const uint32_t (&r)[kHalf]) {
   float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
@@ -219,22 +225,34 @@ __device__ __forceinline__ float max_of(const uint32_t (&r)[kHalf]) {
   return fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
 }
 
-// r <- tanh(r s).  On the FMA pipe while no score of the warp is beyond the cap (eight packed instructions a pair, as long
-// as the exponential unit takes for the probabilities), else two uses of the exponential unit per score.
-__device__ __forceinline__ void cap_scores(uint32_t (&r)[kHalf], float s) {
+// r <- cap * log2(e) * tanh(r s).  On the FMA pipe while no score of the warp is beyond half the cap (five packed
+// instructions a pair) or the cap (seven), else two uses of the exponential unit per score.
+__device__ __forceinline__ void cap_scores(uint32_t (&r)[kHalf], const AttnView& a, const CapPoly& k) {
   float far = 0.f;
 #pragma unroll
   for (int c = 0; c < kHalf; c += 2) far = fmax3(far, fabsf(u2f(r[c])), fabsf(u2f(r[c + 1])));
-  if (__all_sync(0xffffffffu, far * fabsf(s) <= 1.f)) {
-    const uint64_t s2 = pk2(s, s);
+  far *= a.scale;
+  if (__all_sync(0xffffffffu, far <= k.near_limit)) {
 #pragma unroll
     for (int c = 0; c < kHalf; c += 2) {
-      const uint64_t y = fmul2(pk2(u2f(r[c]), u2f(r[c + 1])), s2), z = fmul2(y, y);
-      uint64_t f = ffma2(pk2(kTanh5, kTanh5), z, pk2(kTanh4, kTanh4));
-      f = ffma2(f, z, pk2(kTanh3, kTanh3));
-      f = ffma2(f, z, pk2(kTanh2, kTanh2));
-      f = ffma2(f, z, pk2(kTanh1, kTanh1));
-      f = ffma2(f, z, pk2(kTanh0, kTanh0));
+      const uint64_t y = pk2(u2f(r[c]), u2f(r[c + 1])), z = fmul2(y, y);
+      uint64_t f = ffma2(k.near_[3], z, k.near_[2]);
+      f = ffma2(f, z, k.near_[1]);
+      f = ffma2(f, z, k.near_[0]);
+      float x0, x1;
+      upk2(fmul2(f, y), x0, x1);
+      r[c] = f2u(x0);
+      r[c + 1] = f2u(x1);
+    }
+  } else if (__all_sync(0xffffffffu, far <= k.far_limit)) {
+#pragma unroll
+    for (int c = 0; c < kHalf; c += 2) {
+      const uint64_t y = pk2(u2f(r[c]), u2f(r[c + 1])), z = fmul2(y, y);
+      uint64_t f = ffma2(k.far_[5], z, k.far_[4]);
+      f = ffma2(f, z, k.far_[3]);
+      f = ffma2(f, z, k.far_[2]);
+      f = ffma2(f, z, k.far_[1]);
+      f = ffma2(f, z, k.far_[0]);
       float x0, x1;
       upk2(fmul2(f, y), x0, x1);
       r[c] = f2u(x0);
@@ -242,23 +260,22 @@ __device__ __forceinline__ void cap_scores(uint32_t (&r)[kHalf], float s) {
     }
   } else {
 #pragma unroll
-    for (int c = 0; c < kHalf; ++c) r[c] = f2u(tanh_fast(u2f(r[c]) * s));
+    for (int c = 0; c < kHalf; ++c) r[c] = f2u(a.cap * tanh_fast(u2f(r[c]) * a.scale));
   }
 }
 
 // The scores of 64 keys: products in r -> scores of which mul times is the log2 domain, hidden keys at -inf.  kFull: with
-// the cap, the distance and, with add, biases that are in `keys` and not in the product (always with a cap).
+// the cap, the bias and the distance.
 template <bool kFull>
-__device__ __forceinline__ float form_scores(uint32_t (&r)[kHalf], const AttnView& a, const float* keys, bool add, float slope, float pos,
-                                             int lo, int hi, bool partly) {
+__device__ __forceinline__ float form_scores(uint32_t (&r)[kHalf], const AttnView& a, const CapPoly& k, const float* keys, float slope,
+                                             float pos, int lo, int hi, bool partly) {
   float mul = a.scale;
   if constexpr (kFull) {
     if (a.cap != 0.f) {
-      cap_scores(r, a.scale);
-      mul = a.cap;
+      cap_scores(r, a, k);
+      mul = 1.f;
     }
-    if (add || a.slope != nullptr) {
-      // the ring holds zeros for biases that are in the product
+    if (a.bias != nullptr || a.slope != nullptr) {  // without a bias the ring holds zeros
       const uint64_t sc = pk2(mul, mul);
 #pragma unroll
       for (int c = 0; c < kHalf; c += 4) {
@@ -324,31 +341,44 @@ __device__ __forceinline__ float probabilities(const uint32_t (&r)[kHalf], float
   return (a0 + a1) + (b0 + b1);
 }
 
-// kForm: 0 plain scores; 1 with a bias (in the product; a tile with one that does not fit takes the general step);
-// 2 with a cap or a distance too.
+// What three 16-bit values hold of bias / scale; their product with 1 is exact in fp32.
+template <typename T>
+constexpr float kMostBias = std::is_same<T, __nv_bfloat16>::value ? 1e30f : 60000.f;
+
+// kForm: 0 plain scores; 1 with a bias, in the product; 2 with a cap or a distance, and a bias in the softmax.
+//
+// A bias that does not fit in the product: one below the range (the type's lowest value, say) hides its key there, as -inf
+// does, and a row that ends with no probability, or with a maximum so low that such a key might count, is computed again
+// by exact_row; one above the range, or NaN, makes its scores infinite or NaN, and exact_row computes those rows too.
 template <typename T, bool kPaged, int kForm>
 __global__ void __launch_bounds__(kThreads, 1)
     masked_attention_tc_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_constant__ CUtensorMap tmap_k,
-                               const __grid_constant__ CUtensorMap tmap_v, const __grid_constant__ AttnView a, int blocks, int split) {
+                               const __grid_constant__ CUtensorMap tmap_v, const __grid_constant__ AttnView a, const TileSplit w,
+                               const __grid_constant__ CapPoly poly) {
   constexpr bool kBF16 = std::is_same<T, __nv_bfloat16>::value;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   const uint32_t sbase = smem_u32(smem);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   // blocks in descending order, so that under causal masks the longest start first
-  const int item = static_cast<int>(blockIdx.x) / split, piece = static_cast<int>(blockIdx.x) - item * split;
-  const int vb = blocks - 1 - item / a.H, head = item % a.H, hk = head / a.group;
+  int item = static_cast<int>(blockIdx.x), piece = 0, split = 1;
+  if (item >= w.n_full) {
+    split = w.split;
+    const int x = item - w.n_full;
+    item = w.n_full + x / split;
+    piece = x % split;
+  }
+  const int vb = w.blocks - 1 - item / a.H, head = item % a.H, hk = head / a.group;
   AttnSeq s;
   int blk;
-  if (!locate_block<kPaged>(a, vb, kQT * kBM, 1, s, blk)) return;  // the whole cluster shares the item
+  if (!locate_block<kPaged>(a, vb, kQT * kBM, 1, s, blk)) return;
   const int row_first = blk * kQT * kBM;
 
   auto bar = [=](int i) -> uint32_t { return sbase + kOffBar + 8 * i; };
   int* key_lo = reinterpret_cast<int*>(smem + kOffMisc + 8);
   int* key_hi = key_lo + kQT;
-  const bool per_key = kForm > 0 && (a.bias != nullptr || a.slope != nullptr);
-  const bool in_product = kForm > 0 && a.bias != nullptr && a.cap == 0.f;
-  volatile int* bias_flag = reinterpret_cast<volatile int*>(smem + kOffMisc + 24);  // per stage
+  constexpr bool in_product = kForm == 1;
+  const bool per_key = kForm == 1 || (kForm == 2 && (a.bias != nullptr || a.slope != nullptr));
 
   if (threadIdx.x == 0) {
     mbar_init(bar(kBarQ), 1);
@@ -370,7 +400,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     tmem_alloc(sbase + kOffMisc, kTmemCols);
     tmem_relinquish();
   }
-  if (in_product) {
+  if constexpr (in_product) {
     // the query rows' chunk: 1, 1, 1 in columns 0 to 2; the key rows' chunks: zero beyond column 3
     const uint32_t one = kBF16 ? 0x3F80u : 0x3C00u;
     for (int x = threadIdx.x; x < (1 + kStages) * kExtraBytes / 16; x += kThreads) {
@@ -523,8 +553,6 @@ __global__ void __launch_bounds__(kThreads, 1)
     } else if (warp == kWarpKeys && per_key) {
       // ------------------------------- per-key bias and position -------------------------------
       const float inv = kLog2E / a.scale;  // bias / scale: a.scale = scale * log2(e) without a cap
-      // what the three 16-bit values can hold (and their product with 1 in fp32)
-      const float most = kBF16 ? 1e30f : 60000.f;
       bool ok = true;
       for (int j = p0; j < p1 && ok; ++j) {
         const int n = j - p0, st = n % kStages;
@@ -549,36 +577,30 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (n >= kStages) ok = __all_sync(0xffffffffu, mbar_wait(bar(kBarEmpty + st), (n / kStages - 1) & 1, a.err));
         if (!ok) break;
         float* dst = reinterpret_cast<float*>(smem + kOffKeys) + st * 2 * kBN;
-        bool add = a.cap != 0.f && a.bias != nullptr;
 #pragma unroll
         for (int u = 0; u < 4; ++u) {
           const int k = u * 32 + lane;
-          float in_softmax = bias_log2(b[u]);
-          if (in_product) {
-            const float x = b[u] * inv;
-            const bool fits = fabsf(x) <= most;  // not for NaN
-            const float hi = to_f32<T>(from_f32<T>(x)), mid = to_f32<T>(from_f32<T>(x - hi));
+          if constexpr (in_product) {
+            float x = b[u] * inv, mid = 0.f, lo = 0.f;
+            if (fabsf(x) <= kMostBias<T>) {
+              const float hi = to_f32<T>(from_f32<T>(x));
+              mid = to_f32<T>(from_f32<T>(x - hi));
+              lo = x - hi - mid;
+              x = hi;
+            } else {
+              x = x < 0.f ? -INFINITY : x > 0.f ? INFINITY : x;
+            }
             *reinterpret_cast<uint2*>(smem + kOffExtra + (1 + st) * kExtraBytes + (k >> 3) * 256 + (k & 7) * 16) =
-                fits ? make_uint2(pack2<T>(hi, mid), pack2<T>(x - hi - mid, 0.f)) : make_uint2(0u, 0u);
-            add = add || !fits;
-            if (fits) in_softmax = 0.f;
+                make_uint2(pack2<T>(x, mid), pack2<T>(lo, 0.f));
+          } else {
+            dst[k] = bias_log2(b[u]);
+            dst[kBN + k] = kp[u];
           }
-          dst[k] = in_softmax;
-          dst[kBN + k] = kp[u];
         }
-        add = __any_sync(0xffffffffu, add);
-        if (in_product) fence_proxy_async_smem();
-        if (lane == 0) bias_flag[st] = add;
+        if constexpr (in_product) fence_proxy_async_smem();
         __syncwarp();
         if (lane == 0) mbar_arrive(bar(kBarFull + st));
       }
-    }
-    if (split > 1) {
-      __syncwarp();
-      cluster_arrive();
-      cluster_wait();
-      cluster_arrive();
-      cluster_wait();
     }
   } else {
     // ------------------------------- softmax -------------------------------
@@ -601,10 +623,20 @@ __global__ void __launch_bounds__(kThreads, 1)
       if (ok) ok = mbar_wait(bar(b), static_cast<uint32_t>(parity), a.err);
     };
 
-    // one key tile: scores, probabilities, P
-    auto step = [&](auto full_form, int j, const float* keys, bool add) {
-      constexpr bool kFull = decltype(full_form)::value;
-      const int n = j - ja;
+#pragma unroll 1
+    for (int j = ja; j < jb; ++j) {
+      const int n = j - ja, st = (j - p0) % kStages;
+      {
+        // the scores and, for the softmax, the tile's keys, looked at together
+        const uint32_t ps = n & 1, pf = ((j - p0) / kStages) & 1;
+        const bool wait_keys = kForm == 2 && per_key;
+        const bool s_there = mbar_try_wait(bar(kBarS + t), ps), keys_there = !wait_keys || mbar_try_wait(bar(kBarFull + st), pf);
+        if (!s_there) wait_for(kBarS + t, ps);
+        if (!keys_there) wait_for(kBarFull + st, pf);
+      }
+      __syncwarp();
+      tc_fence_after();
+      const float* keys = reinterpret_cast<const float*>(smem + kOffKeys) + st * 2 * kBN;
       const int key0 = j * kBN;
       uint32_t p[kBN / 2];
       float alpha = 1.f;  // what O is to be multiplied by
@@ -616,7 +648,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         tmem_wait_ld();
         reg_fence32(*reinterpret_cast<uint32_t(*)[32]>(&r[0]));
         reg_fence32(*reinterpret_cast<uint32_t(*)[32]>(&r[32]));
-        const float mul = form_scores<kFull>(r, a, keys, add, slope, pos, be.x - key0, be.y - key0, key0 < all_lo || key0 + kHalf > all_hi);
+        const float mul = form_scores<kForm == 2>(r, a, poly, keys, slope, pos, be.x - key0, be.y - key0, key0 < all_lo || key0 + kHalf > all_hi);
         const float m_new = max_of(r) * mul;
         const bool grow = m_new > m_run + kRescale;
         need = __any_sync(0xffffffffu, grow);
@@ -638,7 +670,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         tc_fence_before();
         __syncwarp();
         if (lane == 0) mbar_arrive(bar(kBarSFree + t));
-        const float mul = form_scores<kFull>(r, a, keys + kHalf, add, slope, pos, be.x - key0 - kHalf, be.y - key0 - kHalf,
+        const float mul = form_scores<kForm == 2>(r, a, poly, keys + kHalf, slope, pos, be.x - key0 - kHalf, be.y - key0 - kHalf,
                                              key0 + kHalf < all_lo || key0 + kBN > all_hi);
         const float m_new = max_of(r) * mul;
         const bool grow = m_new > m_run + kRescale;
@@ -675,25 +707,6 @@ __global__ void __launch_bounds__(kThreads, 1)
       tc_fence_before();
       __syncwarp();
       if (lane == 0) mbar_arrive(bar(kBarP + t));
-    };
-#pragma unroll 1
-    for (int j = ja; j < jb; ++j) {
-      const int st = (j - p0) % kStages;
-      {
-        // the scores and the tile's keys, looked at together
-        const uint32_t ps = (j - ja) & 1, pf = ((j - p0) / kStages) & 1;
-        const bool s_there = mbar_try_wait(bar(kBarS + t), ps), keys_there = !per_key || mbar_try_wait(bar(kBarFull + st), pf);
-        if (!s_there) wait_for(kBarS + t, ps);
-        if (!keys_there) wait_for(kBarFull + st, pf);
-      }
-      __syncwarp();
-      tc_fence_after();
-      const float* keys = reinterpret_cast<const float*>(smem + kOffKeys) + st * 2 * kBN;
-      const bool add = per_key && bias_flag[st] != 0;
-      if constexpr (kForm == 0) step(std::false_type{}, j, keys, false);
-      else if constexpr (kForm == 2) step(std::true_type{}, j, keys, add);
-      else if (add) step(std::true_type{}, j, keys, true);
-      else step(std::false_type{}, j, keys, false);
     }
     uint32_t o[kHeadDim];
 #pragma unroll
@@ -708,81 +721,107 @@ __global__ void __launch_bounds__(kThreads, 1)
       reg_fence32(*reinterpret_cast<uint32_t(*)[32]>(&o[0]));
       reg_fence32(*reinterpret_cast<uint32_t(*)[32]>(&o[32]));
     }
-    uint8_t* out_head = static_cast<uint8_t*>(a.out) + 2 * (s.batch * a.o_sb + head * a.o_sh);
-    if (split == 1) {
-      bool again = false;
-      if (ok && valid) {
-        const float inv = l_run == 0.f ? 0.f : 1.f / l_run;
-        uint4* orow = reinterpret_cast<uint4*>(out_head + 2 * (s.row0 + i) * a.o_sn);
-        float z = 0.f;
+    const bool write = valid && ok;
+    uint4* orow = reinterpret_cast<uint4*>(static_cast<uint8_t*>(a.out) + 2 * (s.batch * a.o_sb + head * a.o_sh + (s.row0 + i) * a.o_sn));
+    float z = 0.f;  // NaN unless every value of the row is finite
+    auto put8 = [&](int c, const float (&x)[8], float inv, bool none) {
+      uint32_t v[4];
 #pragma unroll
-        for (int c = 0; c < kHeadDim / 8; ++c) {
-          uint32_t w[4];
+      for (int e = 0; e < 4; ++e) {
+        z = fmaf(x[2 * e], 0.f, fmaf(x[2 * e + 1], 0.f, z));
+        v[e] = pack2<T>(x[2 * e] * inv, x[2 * e + 1] * inv);
+      }
+      orow[c] = none ? make_uint4(0u, 0u, 0u, 0u) : make_uint4(v[0], v[1], v[2], v[3]);  // no visible key: 0
+    };
+    bool again = false;
+    // rows for exact_row: not finite, or only keys whose bias did not fit
+    auto redo = [&](bool not_finite) {
+      return not_finite || (in_product && be.y > be.x && (l_run == 0.f || m_run < -0.5f * kMostBias<T> * a.scale));
+    };
+    if (split > 1) {
+      // columns of four, rows side by side: [16][256] float4, so that a warp's stores and loads are whole lines
+      const size_t slot0 = static_cast<size_t>(item - w.n_full) * split;
+      auto part_o = [&](int k) { return reinterpret_cast<float4*>(w.parts + (slot0 + k) * kPartBytes) + t * kBM + row; };
+      auto part_ml = [&](int k) {
+        return reinterpret_cast<float2*>(w.parts + (slot0 + k) * kPartBytes + static_cast<size_t>(kQT) * kBM * kHeadDim * 4) + t * kBM + row;
+      };
+      if (jb > ja) {
 #pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const float x = u2f(o[8 * c + 2 * e]), y = u2f(o[8 * c + 2 * e + 1]);
-            z = fmaf(x, 0.f, fmaf(y, 0.f, z));  // NaN unless every value is finite
-            w[e] = pack2<T>(x * inv, y * inv);
-          }
-          orow[c] = l_run == 0.f ? make_uint4(0u, 0u, 0u, 0u) : make_uint4(w[0], w[1], w[2], w[3]);
-        }
-        again = l_run != 0.f && !(z * inv == 0.f);
+        for (int c = 0; c < kHeadDim / 4; ++c)
+          part_o(piece)[c * kQT * kBM] = make_float4(u2f(o[4 * c]), u2f(o[4 * c + 1]), u2f(o[4 * c + 2]), u2f(o[4 * c + 3]));
       }
-      __syncwarp();  // a row's first result is written before its second
-      unsigned rows = __ballot_sync(0xffffffffu, again);
-      while (rows) {
-        const int e = __ffs(rows) - 1;
-        rows &= rows - 1;
-        exact_row<T, kPaged>(a, s, row_first + warp * 32 + e, head);
-      }
-    } else {
-      // The parts overlay Q and the ring: every load into them has been consumed, and every tensor-core read of
-      // them is complete, once both query tiles are.
+      *part_ml(piece) = make_float2(m_run, l_run);
+      __threadfence();
       named_bar_sync(1, kSoftmaxWarps * 32);
-      float* mine = reinterpret_cast<float*>(smem) + (t * kBM + row) * kPartStride;
+      if (threadIdx.x == 0)
+        *reinterpret_cast<volatile int*>(key_lo) = atomicAdd(w.counters + (item - w.n_full), 1u) == static_cast<unsigned>(split - 1);
+      named_bar_sync(1, kSoftmaxWarps * 32);
+      if (write && *reinterpret_cast<volatile int*>(key_lo) != 0) {
+        __threadfence();
+        float f[kMaxSplit];
+        m_run = -INFINITY;
 #pragma unroll
-      for (int c = 0; c < kHeadDim; c += 4)
-        *reinterpret_cast<float4*>(mine + c) = make_float4(u2f(o[c]), u2f(o[c + 1]), u2f(o[c + 2]), u2f(o[c + 3]));
-      *reinterpret_cast<float2*>(smem + kOffPartMl + 8 * (t * kBM + row)) = make_float2(m_run, l_run);
-      cluster_arrive();
-      cluster_wait();
-      const int per = kQT * kBM / split;  // rows joined by this CTA, 16 lanes per row; per * 16 is a multiple of 256 threads
-      for (int x = threadIdx.x; x < per * 16; x += kSoftmaxWarps * 32) {
-        const int rr = piece * per + (x >> 4), c4 = (x & 15) * 4;
-        const uint32_t ml = sbase + kOffPartMl + 8 * rr, ov = sbase + 4 * (rr * kPartStride + c4);
-        float mx = -INFINITY;
-        for (int w = 0; w < split; ++w) mx = fmaxf(mx, peer_load2(peer_address(ml, w)).x);
-        const float mu = mx == -INFINITY ? 0.f : mx;
-        float sum = 0.f;
-        float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-        for (int w = 0; w < split; ++w) {
-          const float2 v = peer_load2(peer_address(ml, w));
-          const float4 y = peer_load4(peer_address(ov, w));
-          const float f = ex2_approx(v.x - mu);
-          if (v.y == 0.f) continue;  // a part without keys of this row: its O may hold 0 * NaN
-          sum = fmaf(v.y, f, sum);
-          acc.x = fmaf(y.x, f, acc.x);
-          acc.y = fmaf(y.y, f, acc.y);
-          acc.z = fmaf(y.z, f, acc.z);
-          acc.w = fmaf(y.w, f, acc.w);
+        for (int k = 0; k < kMaxSplit; ++k)
+          if (k < split) m_run = fmaxf(m_run, __ldcg(part_ml(k)).x);
+        const float mu = m_run == -INFINITY ? 0.f : m_run;
+        l_run = 0.f;
+#pragma unroll
+        for (int k = 0; k < kMaxSplit; ++k) {
+          f[k] = 0.f;
+          if (k < split) {
+            const float2 ml = __ldcg(part_ml(k));
+            if (ml.y != 0.f) {  // a part without keys of this row has no O
+              f[k] = ex2_approx(ml.x - mu);
+              l_run = fmaf(ml.y, f[k], l_run);
+            }
+          }
         }
-        const int tok = row_first + rr;
-        bool again = false;
-        if (tok < s.rows) {
-          const float inv = sum == 0.f ? 0.f : 1.f / sum;
-          *reinterpret_cast<uint2*>(out_head + 2 * ((s.row0 + tok) * a.o_sn + c4)) =
-              sum == 0.f ? make_uint2(0u, 0u) : make_uint2(pack2<T>(acc.x * inv, acc.y * inv), pack2<T>(acc.z * inv, acc.w * inv));
-          const float z = fmaf(acc.x, 0.f, fmaf(acc.y, 0.f, fmaf(acc.z, 0.f, acc.w * 0.f)));  // NaN unless all are finite
-          again = sum != 0.f && !(z * inv == 0.f);
+        const float inv = 1.f / l_run;
+#pragma unroll 1
+        for (int c = 0; c < kHeadDim / 8; ++c) {
+          float4 y[kMaxSplit][2];
+#pragma unroll
+          for (int k = 0; k < kMaxSplit; ++k) {
+            if (k < split && f[k] != 0.f) {
+              y[k][0] = __ldcg(part_o(k) + 2 * c * kQT * kBM);
+              y[k][1] = __ldcg(part_o(k) + (2 * c + 1) * kQT * kBM);
+            } else {
+              y[k][0] = y[k][1] = make_float4(0.f, 0.f, 0.f, 0.f);
+            }
+          }
+          float x[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+          for (int k = 0; k < kMaxSplit; ++k) {
+            x[0] = fmaf(y[k][0].x, f[k], x[0]);
+            x[1] = fmaf(y[k][0].y, f[k], x[1]);
+            x[2] = fmaf(y[k][0].z, f[k], x[2]);
+            x[3] = fmaf(y[k][0].w, f[k], x[3]);
+            x[4] = fmaf(y[k][1].x, f[k], x[4]);
+            x[5] = fmaf(y[k][1].y, f[k], x[5]);
+            x[6] = fmaf(y[k][1].z, f[k], x[6]);
+            x[7] = fmaf(y[k][1].w, f[k], x[7]);
+          }
+          put8(c, x, inv, l_run == 0.f);
         }
-        __syncwarp();  // a row's first result is written before its second
-        const unsigned bad = __ballot_sync(0xffffffffu, again);
-        const int first_row = row_first + piece * per + ((x - lane) >> 4);
-        if (bad & 0xffffu) exact_row<T, kPaged>(a, s, first_row, head);
-        if (bad >> 16) exact_row<T, kPaged>(a, s, first_row + 1, head);
+        again = redo(l_run != 0.f && !(z * inv == 0.f));
       }
-      cluster_arrive();  // the peers read this CTA's part before it leaves
-      cluster_wait();
+    } else if (write) {
+      const float inv = 1.f / l_run;
+#pragma unroll
+      for (int c = 0; c < kHeadDim / 8; ++c) {
+        float x[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) x[e] = u2f(o[8 * c + e]);
+        put8(c, x, inv, l_run == 0.f);
+      }
+      again = redo(l_run != 0.f && !(z * inv == 0.f));
+    }
+    __syncwarp();  // a row's first result is written before its second
+    unsigned rows = __ballot_sync(0xffffffffu, again);
+    while (rows) {
+      const int e = __ffs(rows) - 1;
+      rows &= rows - 1;
+      exact_row<T, kPaged>(a, s, row_first + warp * 32 + e, head);
     }
   }
   tc_fence_before();
@@ -818,8 +857,8 @@ int pool_map(CUtensorMap* map, const void* base, int dtype, const AttnView& a) {
 }
 
 template <typename T, bool kPaged, int kForm>
-int launch_form(const AttnView& a, const CUtensorMap& tq, const CUtensorMap& tk, const CUtensorMap& tv, long long blocks, int split,
-           cudaStream_t st) {
+int launch_form(const AttnView& a, const CUtensorMap& tq, const CUtensorMap& tk, const CUtensorMap& tv, const TileSplit& w, long long grid,
+                cudaStream_t st) {
   auto kernel = masked_attention_tc_kernel<T, kPaged, kForm>;
   // per device: the opt-in to the shared memory
   static std::atomic<bool> ready[64];
@@ -829,66 +868,105 @@ int launch_form(const AttnView& a, const CUtensorMap& tq, const CUtensorMap& tk,
     VB200_CHECK_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemBytes), "cudaFuncSetAttribute");
     if (dev >= 0 && dev < 64) ready[dev].store(true, std::memory_order_release);
   }
-  cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3(static_cast<unsigned>(blocks * a.H * split));
-  cfg.blockDim = dim3(kThreads);
-  cfg.dynamicSmemBytes = kSmemBytes;
-  cfg.stream = st;
-  cudaLaunchAttribute at[1];
-  at[0].id = cudaLaunchAttributeClusterDimension;
-  at[0].val.clusterDim.x = static_cast<unsigned>(split);
-  at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
-  cfg.attrs = at;
-  cfg.numAttrs = split > 1 ? 1 : 0;
-  VB200_CHECK_CUDA(cudaLaunchKernelEx(&cfg, kernel, tq, tk, tv, a, static_cast<int>(blocks), split), "masked_attention_tc_kernel");
+  CapPoly poly{};
+  if (kForm == 2 && a.cap != 0.f) {
+    auto twice = [](double x) {
+      const float f = static_cast<float>(x);
+      uint32_t u;
+      memcpy(&u, &f, 4);
+      return static_cast<uint64_t>(u) << 32 | u;
+    };
+    const double s2 = static_cast<double>(a.scale) * a.scale;
+    double f = static_cast<double>(a.cap) * a.scale;
+    poly.near_limit = 0.5f;
+    poly.far_limit = 1.f;
+    for (int i = 0; i < 6; ++i, f *= s2) {
+      const bool normal = f > 1e-34 && f < 1e34;
+      if (i < 4) poly.near_[i] = twice(kTanhNear[i] * f);
+      poly.far_[i] = twice(kTanhFar[i] * f);
+      if (i < 4 && !normal) poly.near_limit = -1.f;
+      if (!normal) poly.far_limit = -1.f;
+    }
+  }
+  kernel<<<static_cast<unsigned>(grid), kThreads, kSmemBytes, st>>>(tq, tk, tv, a, w, poly);
   VB200_CHECK_LAUNCH("masked_attention_tc_kernel");
   return VB200_OK;
 }
 
 template <typename T, bool kPaged>
-int launch(const AttnView& a, const CUtensorMap& tq, const CUtensorMap& tk, const CUtensorMap& tv, long long blocks, int split,
+int launch(const AttnView& a, const CUtensorMap& tq, const CUtensorMap& tk, const CUtensorMap& tv, const TileSplit& w, long long grid,
            cudaStream_t st) {
-  if (a.cap != 0.f || a.slope != nullptr) return launch_form<T, kPaged, 2>(a, tq, tk, tv, blocks, split, st);
-  return a.bias != nullptr ? launch_form<T, kPaged, 1>(a, tq, tk, tv, blocks, split, st)
-                           : launch_form<T, kPaged, 0>(a, tq, tk, tv, blocks, split, st);
+  if (a.cap != 0.f || a.slope != nullptr) return launch_form<T, kPaged, 2>(a, tq, tk, tv, w, grid, st);
+  return a.bias != nullptr ? launch_form<T, kPaged, 1>(a, tq, tk, tv, w, grid, st) : launch_form<T, kPaged, 0>(a, tq, tk, tv, w, grid, st);
+}
+
+// One CTA per SM: the items (row blocks x heads) run whole while they fill waves of all SMs; those of the last wave in
+// k parts each take ceil(rest * k / SMs) rounds of 1/k of an item plus a ramp of about three key tiles.  The cheapest k.
+struct Plan {
+  long long blocks, items, n_full;
+  int split;
+  size_t counter_bytes, bytes;
+};
+
+Plan plan_of(bool paged, long long rows, long long seqs, long long H, long long most_keys, int sms) {
+  Plan p{};
+  p.blocks = paged ? rows / (kQT * kBM) + seqs : (rows + kQT * kBM - 1) / (kQT * kBM) * seqs;
+  p.items = p.n_full = p.blocks * H;
+  p.split = 1;
+  const double tiles = static_cast<double>((most_keys + kBN - 1) / kBN), ramp = 3.0 / tiles;
+  const long long rest = sms > 0 ? p.items % sms : 0;
+  if (rest == 0) return p;
+  double best = 1.0 + ramp;
+  for (int k = 2; k <= kMaxSplit && 2 * k <= tiles; ++k) {
+    const double cost = static_cast<double>((rest * k + sms - 1) / sms) * (1.0 / k + ramp);
+    if (cost < best - 1e-9) {
+      best = cost;
+      p.split = k;
+    }
+  }
+  if (p.split > 1) {
+    p.n_full = p.items - rest;
+    p.counter_bytes = align_up(static_cast<size_t>(rest) * sizeof(unsigned), 256);
+    p.bytes = p.counter_bytes + static_cast<size_t>(rest) * p.split * kPartBytes;
+  }
+  return p;
 }
 
 }  // namespace
 
-int tile_attention(int dtype, bool paged, const AttnView& a, long long most_keys, cudaStream_t st) {
-  const long long blocks = paged ? static_cast<long long>(a.Nq) / (kQT * kBM) + a.n_seq
-                                 : (static_cast<long long>(a.Nq) + kQT * kBM - 1) / (kQT * kBM) * a.B;
-  // One CTA per SM: `blocks * H` items take ceil(items / SMs) rounds.  Splitting the keys s ways makes the rounds 1/s
-  // as long plus a ramp of about three key tiles each; the cheapest s is taken.
-  const int sms = sm_count_of_device();
-  const long long items = blocks * a.H;
-  const double tiles = static_cast<double>((most_keys + kBN - 1) / kBN);
-  int split = 1;
-  if (sms > 0) {
-    double best = 0.0;
-    for (int k = 1; k <= 8; k *= 2) {
-      if (k > 1 && 2 * k > tiles) break;
-      const double cost = static_cast<double>((items * k + sms - 1) / sms) * (1.0 / k + 3.0 / tiles);
-      if (k == 1 || cost < best - 1e-9) {
-        best = cost;
-        split = k;
-      }
-    }
+size_t tile_attention_workspace(bool paged, long long rows, long long seqs, long long H, long long most_keys) {
+  return plan_of(paged, rows, seqs, H, most_keys, sm_count_of_device()).bytes;
+}
+
+int tile_attention(int dtype, bool paged, const AttnView& a, long long most_keys, void* workspace, size_t workspace_bytes, cudaStream_t st) {
+  Plan p = plan_of(paged, a.Nq, paged ? a.n_seq : a.B, a.H, most_keys, sm_count_of_device());
+  if (p.split > 1 && (workspace == nullptr || workspace_bytes < p.bytes)) {  // no room for parts: whole blocks
+    p.split = 1;
+    p.n_full = p.items;
   }
-  VB200_REQUIRE(items * split < (1ll << 31), "attention: too many work items");
+  const long long grid = p.n_full + (p.items - p.n_full) * p.split;
+  VB200_REQUIRE(grid < (1ll << 31), "attention: too many work items");
+  TileSplit w{};
+  w.blocks = static_cast<int>(p.blocks);
+  w.n_full = static_cast<int>(p.n_full);
+  w.split = p.split;
+  if (p.split > 1) {
+    VB200_REQUIRE((reinterpret_cast<uintptr_t>(workspace) & 255u) == 0, "attention: workspace must be 256-byte aligned");
+    w.counters = static_cast<unsigned*>(workspace);
+    w.parts = static_cast<uint8_t*>(workspace) + p.counter_bytes;
+    VB200_CHECK_CUDA(cudaMemsetAsync(w.counters, 0, p.counter_bytes, st), "zeroing the counters");
+  }
   CUtensorMap tq, tk, tv;
   int rc = rows_map(&tq, a.q, dtype, a.Nq, a.H, paged ? 1 : a.B, a.q_sn, a.q_sh, a.q_sb, kBM);
   if (rc != VB200_OK) return rc;
   if (paged) {
     if ((rc = pool_map(&tk, a.k, dtype, a)) != VB200_OK || (rc = pool_map(&tv, a.v, dtype, a)) != VB200_OK) return rc;
-    return dtype == VB200_BF16 ? launch<__nv_bfloat16, true>(a, tq, tk, tv, blocks, split, st)
-                               : launch<__half, true>(a, tq, tk, tv, blocks, split, st);
+    return dtype == VB200_BF16 ? launch<__nv_bfloat16, true>(a, tq, tk, tv, w, grid, st) : launch<__half, true>(a, tq, tk, tv, w, grid, st);
   }
   if ((rc = rows_map(&tk, a.k, dtype, a.Nk, a.Hkv, a.B, a.k_sn, a.k_sh, a.k_sb, kBN)) != VB200_OK ||
       (rc = rows_map(&tv, a.v, dtype, a.Nk, a.Hkv, a.B, a.v_sn, a.v_sh, a.v_sb, kBN)) != VB200_OK)
     return rc;
-  return dtype == VB200_BF16 ? launch<__nv_bfloat16, false>(a, tq, tk, tv, blocks, split, st)
-                             : launch<__half, false>(a, tq, tk, tv, blocks, split, st);
+  return dtype == VB200_BF16 ? launch<__nv_bfloat16, false>(a, tq, tk, tv, w, grid, st) : launch<__half, false>(a, tq, tk, tv, w, grid, st);
 }
 
 }  // namespace vb200

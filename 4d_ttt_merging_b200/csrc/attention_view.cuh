@@ -126,10 +126,11 @@ __device__ __forceinline__ int page_of(const AttnView& a, const AttnSeq& s, int 
   return id;
 }
 
-// Log2-domain bias of a key.  A finite bias stays finite (the type's lowest value times log2(e) would
-// overflow, and a row whose every key has it would come out empty instead of uniform).
+// Log2-domain bias of a key.  A finite bias stays finite: the type's lowest value times log2(e) would overflow, and a row
+// whose every key has it would come out empty instead of uniform.
 __device__ __forceinline__ float bias_log2(float b) {
-  return b < kLowest / kLog2E && b >= kLowest ? kLowest : b * kLog2E;
+  const float x = b * kLog2E;
+  return fabsf(b) == INFINITY ? b : x > -kLowest ? -kLowest : x < kLowest ? kLowest : x;
 }
 
 // tanh for scores held in fp32 and probabilities rounded to 16 bits: 1 - 2 / (e^{2y} + 1).  Absolute

@@ -72,9 +72,22 @@ unsigned masked_error_word(int clear) {
 
 using namespace vb200;
 
+extern "C" size_t vb200_masked_attention_workspace_size(int dtype, int64_t B, int64_t H, int64_t Hkv, int64_t Nq, int64_t Nk) {
+  if (B < 1 || H < 1 || Hkv < 1 || Nq < 1 || Nk < 1 || few_rows(dtype, Nq, static_cast<int>(H / Hkv))) return 0;
+  return tile_attention_workspace(false, Nq, B, H, Nk);
+}
+
+extern "C" size_t vb200_paged_attention_workspace_size(int dtype, int64_t rows, int64_t H, const vb200_paged_cache* cache, int64_t n) {
+  if (cache == nullptr || rows < 1 || H < 1 || n < 1 || cache->kv_heads < 1 || cache->max_pages < 1 || cache->page_size < 1 ||
+      few_rows(dtype, (rows + n - 1) / n, static_cast<int>(H / cache->kv_heads)))
+    return 0;
+  return tile_attention_workspace(true, rows, n, H, cache->max_pages * cache->page_size);
+}
+
 extern "C" int vb200_masked_attention(int dtype, const void* q, const void* k, const void* v, void* out, int64_t B, int64_t H,
                                       int64_t Hkv, int64_t Nq, int64_t Nk, int64_t D, const int64_t* qs, const int64_t* ks,
-                                      const int64_t* vs, const int64_t* os, const vb200_score_mods* mods, void* stream) {
+                                      const int64_t* vs, const int64_t* os, const vb200_score_mods* mods, void* workspace,
+                                      size_t workspace_bytes, void* stream) {
   VB200_REQUIRE(dtype == VB200_BF16 || dtype == VB200_F16 || dtype == VB200_F32, "masked_attention: unsupported dtype code %d", dtype);
   VB200_REQUIRE(D == kHeadDim, "masked_attention supports head_dim=64 only (got %lld)", (long long)D);
   VB200_REQUIRE(B >= 1 && H >= 1 && Hkv >= 1 && H % Hkv == 0 && Nq >= 0 && Nk >= 1,
@@ -104,12 +117,13 @@ extern "C" int vb200_masked_attention(int dtype, const void* q, const void* k, c
   a.qpos = mods->q_position, a.qpos_sb = mods->q_position_sb;
   a.kpos = mods->k_position, a.kpos_sb = mods->k_position_sb;
   if (few_rows(dtype, Nq, a.group)) return rows_attention(dtype, false, a, Nk, static_cast<cudaStream_t>(stream));
-  return tile_attention(dtype, false, a, Nk, static_cast<cudaStream_t>(stream));
+  return tile_attention(dtype, false, a, Nk, workspace, workspace_bytes, static_cast<cudaStream_t>(stream));
 }
 
 extern "C" int vb200_paged_attention(int dtype, const void* q, void* out, int64_t rows, int64_t H, int64_t D, const int64_t* qs,
                                      const int64_t* os, const vb200_paged_cache* cache, const int32_t* sequence, const int32_t* offsets,
-                                     int64_t n, int causal, const vb200_score_mods* mods, void* stream) {
+                                     int64_t n, int causal, const vb200_score_mods* mods, void* workspace, size_t workspace_bytes,
+                                     void* stream) {
   VB200_REQUIRE(dtype == VB200_BF16 || dtype == VB200_F16 || dtype == VB200_F32, "paged_attention: unsupported dtype code %d", dtype);
   VB200_REQUIRE(D == kHeadDim, "paged_attention supports head_dim=64 only (got %lld)", (long long)D);
   VB200_REQUIRE(cache != nullptr && mods != nullptr, "paged_attention: null handle or mods");
@@ -148,5 +162,5 @@ extern "C" int vb200_paged_attention(int dtype, const void* q, void* out, int64_
   a.max_pages = static_cast<int>(cache->max_pages), a.causal = causal;
   const int64_t most = cache->max_pages * cache->page_size;
   if (few_rows(dtype, (rows + n - 1) / n, a.group)) return rows_attention(dtype, true, a, most, static_cast<cudaStream_t>(stream));
-  return tile_attention(dtype, true, a, most, static_cast<cudaStream_t>(stream));
+  return tile_attention(dtype, true, a, most, workspace, workspace_bytes, static_cast<cudaStream_t>(stream));
 }

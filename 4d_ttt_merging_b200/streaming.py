@@ -48,6 +48,10 @@ def _rows(t: torch.Tensor) -> torch.Tensor:
     return t.clone(memory_format=torch.contiguous_format)
 
 
+def _scratch(size: int, device: torch.device) -> torch.Tensor | None:
+    return torch.empty(size, dtype=torch.uint8, device=device) if size else None
+
+
 def _float_row(what: str, t: torch.Tensor, batch: int, n: int) -> tuple[torch.Tensor, int]:
     """A [n] or [batch, n] tensor as fp32 with its batch stride."""
     if t.shape != (n,) and t.shape != (batch, n):
@@ -172,9 +176,12 @@ def masked_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, log_key_
             if key_position is not None:
                 key_position, mods.k_position_sb = _float_row("key_position", key_position, B, Nk)
                 mods.k_position = key_position.data_ptr()
-        rc = C.lib().vb200_masked_attention(dt, q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), B, H, Hkv, Nq, Nk, D,
-                                            C.strides3(q), C.strides3(k), C.strides3(v), C.strides3(out), mods,
-                                            C.stream_of(q.device))
+        lib = C.lib()
+        size = lib.vb200_masked_attention_workspace_size(dt, B, H, Hkv, Nq, Nk)
+        ws = _scratch(size, q.device)
+        rc = lib.vb200_masked_attention(dt, q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), B, H, Hkv, Nq, Nk, D,
+                                        C.strides3(q), C.strides3(k), C.strides3(v), C.strides3(out), mods, C.ptr(ws), size,
+                                        C.stream_of(q.device))
         C.check(rc, "masked_attention")
     return out
 
@@ -244,9 +251,6 @@ class PagedCache:
     def device(self) -> torch.device:
         return self.k.device
 
-    def _scratch(self, size: int) -> torch.Tensor:
-        return torch.empty(size, dtype=torch.uint8, device=self.k.device)
-
     def append(self, sequence, offsets, k: torch.Tensor, v: torch.Tensor, log_mass: torch.Tensor | None = None) -> None:
         """Rows offsets[i] .. offsets[i + 1] of k, v [tokens, kv heads, 64] and log_mass [tokens] go behind the tokens of slot
         sequence[i].  Pages are taken lowest number first; a shared, partly filled last page is copied before it is written.
@@ -272,11 +276,11 @@ class PagedCache:
                 log_mass = log_mass.to(torch.float32).contiguous()
             lib = C.lib()
             size = lib.vb200_cache_append_workspace_size(n, self.table.shape[0], self.k.shape[0])
-            ws = self._scratch(size)
+            ws = _scratch(size, dev)
             two = ctypes.c_int64 * 2
             rc = lib.vb200_cache_append(self._handle, self._dtype, sequence.data_ptr(), offsets.data_ptr(), n, k.data_ptr(),
                                         v.data_ptr(), C.ptr(log_mass), k.shape[0], two(*k.stride()[:2]), two(*v.stride()[:2]),
-                                        ws.data_ptr(), size, C.stream_of(dev))
+                                        C.ptr(ws), size, C.stream_of(dev))
             C.check(rc, "PagedCache.append")
 
     def fork(self, source, target) -> None:
@@ -288,8 +292,8 @@ class PagedCache:
             target = _int_vector("target", target, dev, source.numel())
             lib = C.lib()
             size = lib.vb200_cache_fork_workspace_size(source.numel(), *self.table.shape)
-            ws = self._scratch(size)
-            rc = lib.vb200_cache_fork(self._handle, self._dtype, source.data_ptr(), target.data_ptr(), source.numel(), ws.data_ptr(),
+            ws = _scratch(size, dev)
+            rc = lib.vb200_cache_fork(self._handle, self._dtype, source.data_ptr(), target.data_ptr(), source.numel(), C.ptr(ws),
                                       size, C.stream_of(dev))
             C.check(rc, "PagedCache.fork")
 
@@ -307,9 +311,9 @@ class PagedCache:
         with torch.cuda.device(dev):
             lib = C.lib()
             size = lib.vb200_cache_compact_workspace_size(self.k.shape[0])
-            ws = self._scratch(size)
+            ws = _scratch(size, dev)
             used = torch.empty(1, dtype=torch.int32, device=dev)
-            rc = lib.vb200_cache_compact(self._handle, self._dtype, used.data_ptr(), ws.data_ptr(), size, C.stream_of(dev))
+            rc = lib.vb200_cache_compact(self._handle, self._dtype, used.data_ptr(), C.ptr(ws), size, C.stream_of(dev))
             C.check(rc, "PagedCache.compact")
         return used
 
@@ -358,9 +362,12 @@ def paged_attention(q: torch.Tensor, cache: PagedCache, sequence, offsets, *, ca
         if distance_slope is not None:
             distance_slope = distance_slope.to(torch.float32).contiguous()
             mods.slope = distance_slope.data_ptr()
+        lib = C.lib()
+        size = lib.vb200_paged_attention_workspace_size(cache._dtype, rows, H, cache._handle, n)
+        ws = _scratch(size, dev)
         two = ctypes.c_int64 * 2
-        rc = C.lib().vb200_paged_attention(cache._dtype, q.data_ptr(), out.data_ptr(), rows, H, D, two(q.stride(1), q.stride(0)),
-                                           two(out.stride(1), out.stride(0)), cache._handle, sequence.data_ptr(), offsets.data_ptr(),
-                                           n, int(causal), mods, C.stream_of(dev))
+        rc = lib.vb200_paged_attention(cache._dtype, q.data_ptr(), out.data_ptr(), rows, H, D, two(q.stride(1), q.stride(0)),
+                                       two(out.stride(1), out.stride(0)), cache._handle, sequence.data_ptr(), offsets.data_ptr(),
+                                       n, int(causal), mods, C.ptr(ws), size, C.stream_of(dev))
         C.check(rc, "paged_attention")
     return out

@@ -136,12 +136,15 @@ typedef struct {
   float scale;               /* positive, usually 1 / 8                                             */
   float softcap;             /* 0: none                                                             */
 } vb200_score_mods;
-/* q, k, v, out with strides {batch, head, token}, channel stride 1; rows 16-byte aligned.  mods may be
- * NULL only through its fields: pass a struct with scale set. */
+/* q, k, v, out with strides {batch, head, token}, channel stride 1; rows 16-byte aligned.
+ * workspace: scratch that lets the tensor-core launch split its last wave of row blocks over the keys (0 bytes where
+ * it does not); with less, or NULL, that wave runs whole.  Calls that may overlap need separate workspaces; nothing
+ * carries over between calls. */
+VB200_API size_t vb200_masked_attention_workspace_size(int dtype, int64_t B, int64_t H, int64_t Hkv, int64_t Nq, int64_t Nk);
 VB200_API int vb200_masked_attention(int dtype, const void* q, const void* k, const void* v, void* out, int64_t B, int64_t H,
                                      int64_t Hkv, int64_t Nq, int64_t Nk, int64_t D, const int64_t* q_strides,
                                      const int64_t* k_strides, const int64_t* v_strides, const int64_t* o_strides,
-                                     const vb200_score_mods* mods, void* stream);
+                                     const vb200_score_mods* mods, void* workspace, size_t workspace_bytes, void* stream);
 
 /* ---- paged cache of streamed keys and values ---------------------------------------------------
  * The handle: contiguous pools k, v [pages][page_size][kv_heads][64] and log_mass [pages][page_size] (or NULL),
@@ -159,11 +162,13 @@ typedef struct {
 /* Attention of ragged chunks over the cache: rows offsets[i] .. offsets[i+1] of q (strides {head, row}) are the
  * last tokens of slot sequence[i] (NULL: slot i), already appended.  Without mods->key_range a row sees all
  * keys of its slot, or with causal != 0 those up to its own.  Positions are token indices (q_position, k_position
- * and key_bias of mods are not used: the bias is the cache's log_mass).  Rows outside every chunk are not written. */
+ * and key_bias of mods are not used: the bias is the cache's log_mass).  Rows outside every chunk are not written.
+ * workspace as for vb200_masked_attention. */
+VB200_API size_t vb200_paged_attention_workspace_size(int dtype, int64_t rows, int64_t H, const vb200_paged_cache* cache, int64_t n);
 VB200_API int vb200_paged_attention(int dtype, const void* q, void* out, int64_t rows, int64_t H, int64_t D,
                                     const int64_t* q_strides, const int64_t* o_strides, const vb200_paged_cache* cache,
                                     const int32_t* sequence, const int32_t* offsets, int64_t n, int causal,
-                                    const vb200_score_mods* mods, void* stream);
+                                    const vb200_score_mods* mods, void* workspace, size_t workspace_bytes, void* stream);
 /* Appends rows offsets[i] .. offsets[i+1] of k, v (strides {token, head}) and log_mass [tokens] (NULL: 0) behind
  * the tokens of slot sequence[i].  New pages are the lowest free ones in the order of the call; a shared, partly
  * filled last page is copied first.  All or nothing: with too few pages (error bit 2) or offsets that

@@ -135,6 +135,31 @@ def test_extreme_biases(pkg, oracle, cuda_device, dtype, queries):
 
 
 @pytest.mark.parametrize("dtype", ["bf16", "f16", "f32"])
+@pytest.mark.parametrize("queries", [150, 2])
+@pytest.mark.parametrize("softcap", [None, 30.0])
+def test_mask_constants(pkg, oracle, cuda_device, dtype, queries, softcap):
+    """Large biases that programs use as masks, alone in a row and beside others, and rows that only see such keys."""
+    rng, q, k, v = make(14, 1, 2, 2, queries, 260, dtype, oracle)
+    bias = rng.choice([0.0, -1e4, -1e9, -7600.0, -3e38, -np.inf, 2.0], 260).astype(np.float32)
+    bias[:130] = -1e4 - np.arange(130) / 8
+    bias[20:40] = -1e9
+    bias[40:60] = -2e30
+    r = np.stack([rng.integers(0, 60, queries), rng.integers(60, 261, queries)], 1).astype(np.int32)
+    r[::3] = [20, 40]
+    r[1::5] = [30, 60]
+    run(pkg, oracle, cuda_device, dtype, q, k, v, bias, r, softcap=softcap)
+    bias[200], bias[7] = 3e38, 1e33
+    run(pkg, oracle, cuda_device, dtype, q, k, v, bias, r, softcap=softcap)
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f16", "f32"])
+@pytest.mark.parametrize("softcap", [0.01, 1.0, 4.0, 9.0, 400.0, 1e5, 1e12])
+def test_caps_of_any_size(pkg, oracle, cuda_device, dtype, softcap):
+    _, q, k, v = make(15, 1, 2, 2, 140, 200, dtype, oracle, q_scale=8.0)
+    run(pkg, oracle, cuda_device, dtype, q, k, v, softcap=softcap)
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f16", "f32"])
 @pytest.mark.parametrize("queries", [333, 4])
 def test_hidden_values_do_not_reach_a_row(pkg, oracle, cuda_device, dtype, queries):
     """NaN and infinities in keys and values that a row does not see, in the tiles that it reads."""

@@ -74,7 +74,7 @@ def test_c_entry_points_refuse_bad_arguments(pkg):
     s = (ctypes.c_int64 * 3)(64, 64, 64)
     mods = C.ScoreMods(scale=0.125)
     dense = lambda dt=1, q=16, B=1, H=4, Hkv=2, Nq=3, Nk=5, D=64, st=s, m=mods: lib.vb200_masked_attention(  # noqa: E731
-        dt, q, 16, 16, 16, B, H, Hkv, Nq, Nk, D, st, s, s, s, m, None)
+        dt, q, 16, 16, 16, B, H, Hkv, Nq, Nk, D, st, s, s, s, m, None, 0, None)
     for kw, word in ((dict(dt=7), b"dtype"), (dict(D=32), b"head_dim"), (dict(Hkv=3), b"sizes"), (dict(Nk=0), b"sizes"),
                      (dict(Nk=1 << 31), b"range"), (dict(q=None), b"null"), (dict(q=8), b"aligned"),
                      (dict(st=(ctypes.c_int64 * 3)(64, 64, 60)), b"aligned"), (dict(m=C.ScoreMods(scale=float("nan"))), b"scale"),
@@ -85,7 +85,7 @@ def test_c_entry_points_refuse_bad_arguments(pkg):
                                                   kv_heads=2, slots=2, max_pages=4), **k))
     two = (ctypes.c_int64 * 2)(64, 64)
     paged = lambda c, H=4, rows=2, n=1, q=16, seq=16: lib.vb200_paged_attention(1, q, 16, rows, H, 64, two, two, c, seq, 16, n, 1,  # noqa: E731
-                                                                               mods, None)
+                                                                               mods, None, 0, None)
     for c, kw, word in ((cache(page_size=24), {}, b"pages of"), (cache(), dict(H=3), b"multiple"), (cache(pages=0), {}, b"range"),
                         (cache(k=None), {}, b"null"), (cache(), dict(q=None), b"null"), (cache(), dict(n=3, seq=None), b"slots"),
                         (cache(k=24), {}, b"aligned")):
