@@ -65,7 +65,7 @@ constexpr int kOffExtra = kOffStage + kStages * 2 * kTileBytes;   // the query r
 constexpr int kOffKeys = kOffExtra + (1 + kStages) * kExtraBytes;  // [stage][2][128] fp32: bias, position
 constexpr int kOffBar = kOffKeys + kStages * 2 * kBN * 4;
 constexpr int kBarQ = 0, kBarFull = 1, kBarEmpty = kBarFull + kStages, kBarS = kBarEmpty + kStages, kBarSFree = kBarS + kQT,
-              kBarP = kBarSFree + kQT, kBarO = kBarP + kQT, kNumBars = kBarO + kQT;
+              kBarP = kBarSFree + kQT, kBarO = kBarP + kQT, kBarTail = kBarO + kQT, kNumBars = kBarTail + 1;
 constexpr int kOffMisc = kOffBar + kNumBars * 8;  // TMEM base; per query tile: first and last key
 constexpr int kSmemBytes = kOffMisc + 32 + 1024;
 constexpr int kMaxSplit = 8;
@@ -134,60 +134,6 @@ struct TileSplit {
   uint8_t* parts;    // [blocks * H - n_full][split][kPartBytes]
   unsigned* counters;  // [blocks * H - n_full], zero at the launch
 };
-
-// One output row by one warp, key by key, two channels per lane: for rows whose tile result is not finite.
-template <typename T, bool kPaged>
-__device__ __noinline__ void exact_row(const AttnView& a, AttnSeq s, int i, int head) {
-  const int lane = threadIdx.x & 31, hk = head / a.group;
-  const int2 be = row_range<kPaged>(a, s, i);
-  const float slope = a.slope == nullptr ? 0.f : __ldg(a.slope + head) * kLog2E;
-  const float pos = row_position<kPaged>(a, s, i);
-  const T* q = static_cast<const T*>(a.q) + s.batch * a.q_sb + head * a.q_sh + static_cast<long long>(s.row0 + i) * a.q_sn + 2 * lane;
-  const float q0 = to_f32<T>(q[0]) * a.scale, q1 = to_f32<T>(q[1]) * a.scale;
-  float m = -INFINITY, l = 0.f, o0 = 0.f, o1 = 0.f;
-  for (int j0 = be.x; j0 < be.y; j0 += 32) {
-    // each lane looks at one key: where it lies, its bias; keys of mass 0 are left out
-    long long ko = 0, vo = 0;
-    float b = -INFINITY, kp = 0.f;
-    if (j0 + lane < be.y) {
-      const int j = j0 + lane;
-      b = 0.f;
-      if constexpr (kPaged) {
-        const int id = page_of(a, s, j >> a.page_shift), at = j & ((1 << a.page_shift) - 1);
-        ko = id * a.k_sb + at * a.k_sn;
-        vo = id * a.v_sb + at * a.v_sn;
-        if (id >= a.pages) b = -INFINITY;
-        else if (a.bias != nullptr) b = bias_log2(__ldg(a.bias + (static_cast<long long>(id) << a.page_shift) + at));
-      } else {
-        ko = s.batch * a.k_sb + j * a.k_sn;
-        vo = s.batch * a.v_sb + j * a.v_sn;
-        if (a.bias != nullptr) b = bias_log2(__ldg(a.bias + s.batch * a.bias_sb + j));
-      }
-      kp = !kPaged && a.slope != nullptr && a.kpos != nullptr ? __ldg(a.kpos + s.batch * a.kpos_sb + j) : static_cast<float>(j);
-    }
-    for (unsigned some = __ballot_sync(0xffffffffu, b != -INFINITY); some != 0; some &= some - 1) {
-      const int from = __ffs(some) - 1;
-      const T* k = static_cast<const T*>(a.k) + __shfl_sync(0xffffffffu, ko, from) + hk * a.k_sh + 2 * lane;
-      const T* v = static_cast<const T*>(a.v) + __shfl_sync(0xffffffffu, vo, from) + hk * a.v_sh + 2 * lane;
-      float x = q0 * to_f32<T>(k[0]) + q1 * to_f32<T>(k[1]);
-#pragma unroll
-      for (int d = 16; d >= 1; d >>= 1) x += __shfl_xor_sync(0xffffffffu, x, d);
-      if (a.cap != 0.f) x = a.cap * tanh_fast(x);
-      x += __shfl_sync(0xffffffffu, b, from);
-      const float at = __shfl_sync(0xffffffffu, kp, from);
-      if (a.slope != nullptr) x = fmaf(-slope, fabsf(pos - at), x);
-      const float mn = fmaxf(m, x), mu = mn == -INFINITY ? 0.f : mn;
-      const float corr = ex2_approx(m - mu), p = ex2_approx(x - mu);
-      m = mn;
-      l = l * corr + p;
-      o0 = o0 * corr + p * to_f32<T>(v[0]);
-      o1 = o1 * corr + p * to_f32<T>(v[1]);
-    }
-  }
-  T* out = static_cast<T*>(a.out) + s.batch * a.o_sb + head * a.o_sh + static_cast<long long>(s.row0 + i) * a.o_sn + 2 * lane;
-  out[0] = from_f32<T>(l == 0.f ? 0.f : o0 / l);
-  out[1] = from_f32<T>(l == 0.f ? 0.f : o1 / l);
-}
 
 // Both 16-bit halves of x times f.
 template <typename T>
@@ -382,6 +328,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 
   if (threadIdx.x == 0) {
     mbar_init(bar(kBarQ), 1);
+    mbar_init(bar(kBarTail), 1);
     for (int i = 0; i < kStages; ++i) {
       mbar_init(bar(kBarFull + i), per_key ? 2 : 1);
       mbar_init(bar(kBarEmpty + i), kQT);
@@ -454,6 +401,14 @@ __global__ void __launch_bounds__(kThreads, 1)
     j1[t] = max(min(j1[t], p1), j0[t]);
   }
   if (j0[0] == j1[0] && j0[1] == j1[1]) p1 = p0;  // the part lies between the two query tiles' keys
+
+  // Paged: the tile whose last page the sequence fills in part.  The slots behind the last key hold anything, NaN perhaps, so
+  // warp 11 overwrites their values with zeros before the PV product reads them.  -1: none in this part.
+  int tail = -1;
+  if (kPaged && (s.keys & (kBN - 1)) != 0) {
+    const int j = s.keys / kBN;
+    if ((j >= j0[0] && j < j1[0]) || (j >= j0[1] && j < j1[1])) tail = j;
+  }
 
   // A wait that runs out makes its role go on without waiting (or leave), so that every thread reaches the end and
   // TMEM is freed.
@@ -540,7 +495,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           tc_fence_after();
           qk(j + 1);
         }
-        ok = wait_all(kBarP + t, n & 1);
+        ok = wait_all(kBarP + t, n & 1) && (!kPaged || j != tail || wait_all(kBarTail, 0));
         if (!ok) break;
         tc_fence_after();
         issue_pv(tmem + kTmemO + t * kHeadDim, tmem + kTmemP + t * kHeadDim, v_desc + stage_off(j), idesc_pv, n > 0 ? 1u : 0u,
@@ -550,11 +505,11 @@ __global__ void __launch_bounds__(kThreads, 1)
         ok = full(j);
         if (ok && lane == 0) mbar_arrive(bar(kBarEmpty + (j - p0) % kStages));
       }
-    } else if (warp == kWarpKeys && per_key) {
+    } else if (warp == kWarpKeys) {
       // ------------------------------- per-key bias and position -------------------------------
       const float inv = kLog2E / a.scale;  // bias / scale: a.scale = scale * log2(e) without a cap
       bool ok = true;
-      for (int j = p0; j < p1 && ok; ++j) {
+      for (int j = p0; per_key && j < p1 && ok; ++j) {
         const int n = j - p0, st = n % kStages;
         float b[4], kp[4];
 #pragma unroll
@@ -600,6 +555,16 @@ __global__ void __launch_bounds__(kThreads, 1)
         if constexpr (in_product) fence_proxy_async_smem();
         __syncwarp();
         if (lane == 0) mbar_arrive(bar(kBarFull + st));
+      }
+      if (kPaged && tail >= 0 && ok) {
+        const int n = tail - p0, st = n % kStages;
+        ok = __all_sync(0xffffffffu, mbar_wait(bar(kBarFull + st), (n / kStages) & 1, a.err));
+        // whole rows, so the swizzle inside a row does not matter
+        uint4* v = reinterpret_cast<uint4*>(smem + kOffStage + (2 * st + 1) * kTileBytes);
+        for (int x = (s.keys & (kBN - 1)) * 8 + lane; ok && x < kBN * 8; x += 32) v[x] = make_uint4(0u, 0u, 0u, 0u);
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0 && ok) mbar_arrive(bar(kBarTail));
       }
     }
   } else {
@@ -832,30 +797,6 @@ __global__ void __launch_bounds__(kThreads, 1)
   }
 }
 
-int rows_map(CUtensorMap* map, const void* base, int dtype, long long n, long long heads, long long batch, long long sn, long long sh,
-             long long sb, int box) {
-  // (channel, row, head, batch); dimensions of size one get a harmless stride
-  if (n == 1) sn = kHeadDim;
-  if (heads == 1) sh = sn * n;
-  if (batch == 1) sb = sh * heads;
-  const uint64_t dims[4] = {kHeadDim, static_cast<uint64_t>(n), static_cast<uint64_t>(heads), static_cast<uint64_t>(batch)};
-  const uint64_t str[3] = {static_cast<uint64_t>(sn) * 2, static_cast<uint64_t>(sh) * 2, static_cast<uint64_t>(sb) * 2};
-  const uint32_t b[4] = {kHeadDim, static_cast<uint32_t>(box), 1, 1};
-  return encode_tiled_map(map, dtype == VB200_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 4, base, dims,
-                          str, b, CU_TENSOR_MAP_SWIZZLE_128B);
-}
-
-int pool_map(CUtensorMap* map, const void* base, int dtype, const AttnView& a) {
-  // (channel, head, slot, page): contiguous pools
-  const int page = 1 << a.page_shift;
-  const uint64_t dims[4] = {kHeadDim, static_cast<uint64_t>(a.Hkv), static_cast<uint64_t>(page), static_cast<uint64_t>(a.pages)};
-  const uint64_t row = static_cast<uint64_t>(a.Hkv) * kHeadDim * 2;
-  const uint64_t str[3] = {kHeadDim * 2, row, row * page};
-  const uint32_t b[4] = {kHeadDim, 1, static_cast<uint32_t>(page), 1};
-  return encode_tiled_map(map, dtype == VB200_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 4, base, dims,
-                          str, b, CU_TENSOR_MAP_SWIZZLE_128B);
-}
-
 template <typename T, bool kPaged, int kForm>
 int launch_form(const AttnView& a, const CUtensorMap& tq, const CUtensorMap& tk, const CUtensorMap& tv, const TileSplit& w, long long grid,
                 cudaStream_t st) {
@@ -960,7 +901,7 @@ int tile_attention(int dtype, bool paged, const AttnView& a, long long most_keys
   int rc = rows_map(&tq, a.q, dtype, a.Nq, a.H, paged ? 1 : a.B, a.q_sn, a.q_sh, a.q_sb, kBM);
   if (rc != VB200_OK) return rc;
   if (paged) {
-    if ((rc = pool_map(&tk, a.k, dtype, a)) != VB200_OK || (rc = pool_map(&tv, a.v, dtype, a)) != VB200_OK) return rc;
+    if ((rc = pool_map(&tk, a.k, dtype, a, kBN)) != VB200_OK || (rc = pool_map(&tv, a.v, dtype, a, kBN)) != VB200_OK) return rc;
     return dtype == VB200_BF16 ? launch<__nv_bfloat16, true>(a, tq, tk, tv, w, grid, st) : launch<__half, true>(a, tq, tk, tv, w, grid, st);
   }
   if ((rc = rows_map(&tk, a.k, dtype, a.Nk, a.Hkv, a.B, a.k_sn, a.k_sh, a.k_sb, kBN)) != VB200_OK ||

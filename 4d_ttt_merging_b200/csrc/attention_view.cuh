@@ -52,7 +52,8 @@ struct AttnSeq {
 // without a host that knows their lengths: sequence i's blocks start at index offsets[i] * mult / per
 // + i.  The starts of two neighbours differ by at least ceil(rows * mult / per), so blocks never
 // overlap; indices between a sequence's last block and the next start are empty.  Returns false for
-// an empty index.  Offsets that do not ascend or leave [0, Nq], and slots out of range, set the error
+// an empty index.  Called by the whole block (it has a barrier): the threads look at the starts side by side, one load deep,
+// where a search would make log2(sequences) dependent ones (0.6 us each).  Offsets that do not ascend or leave [0, Nq], and slots out of range, set the error
 // word and leave the sequence out.
 template <bool kPaged>
 __device__ __forceinline__ bool locate_block(const AttnView& a, int index, int per, int mult, AttnSeq& s, int& block) {
@@ -70,12 +71,14 @@ __device__ __forceinline__ bool locate_block(const AttnView& a, int index, int p
       const int o = min(max(__ldg(a.offsets + i), 0), a.Nq);
       return static_cast<long long>(o) * mult / per + i;
     };
-    int lo = 0, hi = a.n_seq;  // the last i with start(i) <= index
-    while (hi - lo > 1) {
-      const int mid = (lo + hi) >> 1;
-      if (start(mid) <= index) lo = mid;
-      else hi = mid;
+    int upto = 0;  // sequences that start at or before the index
+    for (int base = 0; base < a.n_seq; base += blockDim.x) {
+      const int i = base + static_cast<int>(threadIdx.x);
+      const int here = __syncthreads_count(i < a.n_seq && start(i) <= index);
+      upto += here;
+      if (here < static_cast<int>(blockDim.x)) break;  // the same in every thread
     }
+    const int lo = max(upto - 1, 0);
     const int o0 = __ldg(a.offsets + lo), o1 = __ldg(a.offsets + lo + 1);
     const int slot = a.sequence == nullptr ? lo : __ldg(a.sequence + lo);
     if (o0 < 0 || o1 < o0 || o1 > a.Nq || slot < 0 || slot >= a.slots) {
@@ -140,6 +143,61 @@ __device__ __forceinline__ float bias_log2(float b) {
 __device__ __forceinline__ float tanh_fast(float y) {
   const float e = ex2_approx(y * (2.f * kLog2E));
   return 1.f - __fdividef(2.f, e + 1.f);
+}
+
+// One output row by one warp, key by key, two channels per lane: for rows that a tensor-core kernel finds not finite.  There a
+// hidden key's probability 0 meets its value, whatever that is, in the product; here hidden keys are not read.
+template <typename T, bool kPaged>
+__device__ __noinline__ void exact_row(const AttnView& a, AttnSeq s, int i, int head) {
+  const int lane = threadIdx.x & 31, hk = head / a.group;
+  const int2 be = row_range<kPaged>(a, s, i);
+  const float slope = a.slope == nullptr ? 0.f : __ldg(a.slope + head) * kLog2E;
+  const float pos = row_position<kPaged>(a, s, i);
+  const T* q = static_cast<const T*>(a.q) + s.batch * a.q_sb + head * a.q_sh + static_cast<long long>(s.row0 + i) * a.q_sn + 2 * lane;
+  const float q0 = to_f32<T>(q[0]) * a.scale, q1 = to_f32<T>(q[1]) * a.scale;
+  float m = -INFINITY, l = 0.f, o0 = 0.f, o1 = 0.f;
+  for (int j0 = be.x; j0 < be.y; j0 += 32) {
+    // each lane looks at one key: where it lies, its bias; keys of mass 0 are left out
+    long long ko = 0, vo = 0;
+    float b = -INFINITY, kp = 0.f;
+    if (j0 + lane < be.y) {
+      const int j = j0 + lane;
+      b = 0.f;
+      if constexpr (kPaged) {
+        const int id = page_of(a, s, j >> a.page_shift), at = j & ((1 << a.page_shift) - 1);
+        ko = id * a.k_sb + at * a.k_sn;
+        vo = id * a.v_sb + at * a.v_sn;
+        if (id >= a.pages) b = -INFINITY;
+        else if (a.bias != nullptr) b = bias_log2(__ldg(a.bias + (static_cast<long long>(id) << a.page_shift) + at));
+      } else {
+        ko = s.batch * a.k_sb + j * a.k_sn;
+        vo = s.batch * a.v_sb + j * a.v_sn;
+        if (a.bias != nullptr) b = bias_log2(__ldg(a.bias + s.batch * a.bias_sb + j));
+      }
+      kp = !kPaged && a.slope != nullptr && a.kpos != nullptr ? __ldg(a.kpos + s.batch * a.kpos_sb + j) : static_cast<float>(j);
+    }
+    for (unsigned some = __ballot_sync(0xffffffffu, b != -INFINITY); some != 0; some &= some - 1) {
+      const int from = __ffs(some) - 1;
+      const T* k = static_cast<const T*>(a.k) + __shfl_sync(0xffffffffu, ko, from) + hk * a.k_sh + 2 * lane;
+      const T* v = static_cast<const T*>(a.v) + __shfl_sync(0xffffffffu, vo, from) + hk * a.v_sh + 2 * lane;
+      float x = q0 * to_f32<T>(k[0]) + q1 * to_f32<T>(k[1]);
+#pragma unroll
+      for (int d = 16; d >= 1; d >>= 1) x += __shfl_xor_sync(0xffffffffu, x, d);
+      if (a.cap != 0.f) x = a.cap * tanh_fast(x);
+      x += __shfl_sync(0xffffffffu, b, from);
+      const float at = __shfl_sync(0xffffffffu, kp, from);
+      if (a.slope != nullptr) x = fmaf(-slope, fabsf(pos - at), x);
+      const float mn = fmaxf(m, x), mu = mn == -INFINITY ? 0.f : mn;
+      const float corr = ex2_approx(m - mu), p = ex2_approx(x - mu);
+      m = mn;
+      l = l * corr + p;
+      o0 = o0 * corr + p * to_f32<T>(v[0]);
+      o1 = o1 * corr + p * to_f32<T>(v[1]);
+    }
+  }
+  T* out = static_cast<T*>(a.out) + s.batch * a.o_sb + head * a.o_sh + static_cast<long long>(s.row0 + i) * a.o_sn + 2 * lane;
+  out[0] = from_f32<T>(l == 0.f ? 0.f : o0 / l);
+  out[1] = from_f32<T>(l == 0.f ? 0.f : o1 / l);
 }
 
 }  // namespace vb200

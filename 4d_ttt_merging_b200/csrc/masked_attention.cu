@@ -1,4 +1,6 @@
 // Entry points of the masked and the paged attention: argument checks and the choice of kernel.
+#include <cudaTypedefs.h>
+
 #include <cmath>
 #include <initializer_list>
 
@@ -45,11 +47,35 @@ bool aligned(const void* p, const int64_t* s, std::initializer_list<int64_t> siz
   return ok;
 }
 
-// fp32, or at most 8 (row, head) pairs per key head: the FMA kernel.  A tile of the tensor-core kernel has 128 rows
-// of one head, so below that its tiles are nearly empty and the heads of a group read their keys one by one.
-bool few_rows(int dtype, int64_t rows, int group) { return dtype == VB200_F32 || rows * group <= 8; }
+// fp32, or at most 16 (row, head) pairs per key head.  A tile of the other kernel has 128 rows of one head, so below that its
+// tiles are nearly empty and the heads of a group read their keys one by one.
+bool few_rows(int dtype, int64_t rows, int group) { return dtype == VB200_F32 || rows * group <= 16; }
 
 }  // namespace
+
+int rows_map(CUtensorMap* map, const void* base, int dtype, long long n, long long heads, long long batch, long long sn, long long sh,
+             long long sb, int box) {
+  // (channel, row, head, batch); dimensions of size one get a harmless stride
+  if (n == 1) sn = kHeadDim;
+  if (heads == 1) sh = sn * n;
+  if (batch == 1) sb = sh * heads;
+  const uint64_t dims[4] = {kHeadDim, static_cast<uint64_t>(n), static_cast<uint64_t>(heads), static_cast<uint64_t>(batch)};
+  const uint64_t str[3] = {static_cast<uint64_t>(sn) * 2, static_cast<uint64_t>(sh) * 2, static_cast<uint64_t>(sb) * 2};
+  const uint32_t b[4] = {kHeadDim, static_cast<uint32_t>(box), 1, 1};
+  return encode_tiled_map(map, dtype == VB200_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 4, base, dims,
+                          str, b, CU_TENSOR_MAP_SWIZZLE_128B);
+}
+
+int pool_map(CUtensorMap* map, const void* base, int dtype, const AttnView& a, int box) {
+  // (channel, head, slot, page): contiguous pools
+  const int page = 1 << a.page_shift;
+  const uint64_t dims[4] = {kHeadDim, static_cast<uint64_t>(a.Hkv), static_cast<uint64_t>(page), static_cast<uint64_t>(a.pages)};
+  const uint64_t row = static_cast<uint64_t>(a.Hkv) * kHeadDim * 2;
+  const uint64_t str[3] = {kHeadDim * 2, row, row * page};
+  const uint32_t b[4] = {kHeadDim, 1, static_cast<uint32_t>(page < box ? page : box), 1};
+  return encode_tiled_map(map, dtype == VB200_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 4, base, dims,
+                          str, b, CU_TENSOR_MAP_SWIZZLE_128B);
+}
 
 int sm_count_of_device() {
   int dev = 0, n = 0;
