@@ -15,7 +15,7 @@
 //     16-byte asynchronous copies spent a third of its time issuing them and reached 4.6 TB/s, loads into registers spilled
 //     and reached 3.7, the FMA pipe 2.2 with one row per key head and 0.7 with eight.)  A tcgen05 tile has 128 rows of
 //     which these would use 1 to 16.
-//   rows_attention_kernel (fp32): up to 8 pairs, on the FMA pipe: eight lanes hold one key, 8 channels each.
+//   rows_attention_kernel (fp32): up to 4 pairs, on the FMA pipe: eight lanes hold one key, 8 channels each.
 #include <cooperative_groups.h>
 
 #include <algorithm>
@@ -67,7 +67,7 @@ __device__ __forceinline__ void join(int parts, F part, int ch, float& mx, float
 
 // resident CTAs: as many as the registers of R rows (their queries and sums) allow
 template <int R, bool kPaged>
-__global__ void __launch_bounds__(kRowWarps * 32, R <= 2 ? 3 : R <= 4 ? 2 : 1) rows_attention_kernel(const AttnView a, int split) {
+__global__ void __launch_bounds__(kRowWarps * 32, R <= 2 ? 3 : 2) rows_attention_kernel(const AttnView a, int split) {
   using T = float;
   constexpr int U = 2;  // loads in flight per lane: 4 x (K, V) vectors of 16 bytes
   constexpr int kStep = 4 * U;               // keys per warp and step; divides every page size
@@ -691,8 +691,7 @@ int launch_cluster(void (*kernel)(P...), long long items, int split, int smem, c
 
 template <bool kPaged>
 int launch_f32(const AttnView& a, int R, long long items, int split, cudaStream_t st) {
-  auto kernel = R == 1 ? rows_attention_kernel<1, kPaged> : R == 2 ? rows_attention_kernel<2, kPaged>
-                : R == 4 ? rows_attention_kernel<4, kPaged> : rows_attention_kernel<8, kPaged>;
+  auto kernel = R == 1 ? rows_attention_kernel<1, kPaged> : R == 2 ? rows_attention_kernel<2, kPaged> : rows_attention_kernel<4, kPaged>;
   return launch_cluster(kernel, items, split, 0, "rows_attention_kernel", st, a, split);
 }
 
@@ -728,16 +727,18 @@ int launch_16(const AttnView& a, bool paged, bool wide, long long items, int spl
 
 int rows_attention(int dtype, bool paged, const AttnView& a, long long most_keys, cudaStream_t st) {
   // Pairs per CTA.  16 bits: 8, or 16 where a sequence has more on average.  fp32: as many as a sequence has on average, at
-  // most 8 (registers).  Longer sequences take several blocks, shorter ones leave rows idle; both are right.
+  // most 4 (17 rows of 16 heads over 1041 keys of 4 key heads: 15.9 us, with up to 8 pairs 28.7; 1041 rows over 1041 keys of
+  // 16: 368 and 394).  Longer sequences take several blocks, shorter ones leave rows idle; both are right.
   const long long seqs = paged ? a.n_seq : a.B;
   const long long total = static_cast<long long>(a.Nq) * a.group;  // of all sequences (paged), or of one
   const long long mean = paged ? (total + seqs - 1) / seqs : total;
-  const int R = dtype != VB200_F32 ? (mean <= 8 ? 8 : 16) : mean <= 1 ? 1 : mean <= 2 ? 2 : mean <= 4 ? 4 : 8;
+  const int R = dtype != VB200_F32 ? (mean <= 8 ? 8 : 16) : mean <= 1 ? 1 : mean <= 2 ? 2 : 4;
   const long long blocks = paged ? total / R + a.n_seq : (total + R - 1) / R * a.B;
   const long long items = blocks * a.Hkv;
-  // Split the keys while two CTAs per SM are not filled and a piece keeps at least 256 keys; once more, for even ends of
-  // ragged sequences, while four are not and it keeps 1024 (32 sequences of 500 to 9000 keys: 175 -> 157 us; 8 of 4000, where
-  // it would not: 43 -> 57 us).  Up to 8 parts, the portable size of a cluster (16 gained 5% for one sequence of 32,928 keys).
+  // Split the keys while two CTAs per SM are not filled and a piece keeps at least 256 keys; once more, for even ends
+  // of ragged sequences, while four are not and it keeps 1024 (32 sequences of 500 to 9000 keys: 175 -> 157 us; 8 of 4000,
+  // where it would not: 43 -> 57 us).  Up to 8 parts, the portable size of a cluster (16 gained 5% for one sequence of 32,928
+  // keys).
   int split = 1;
   const long long sms = sm_count_of_device();
   const long long busy = (paged ? std::max((total + R - 1) / R, seqs) : blocks) * a.Hkv;

@@ -1,8 +1,10 @@
 // Entry points of the masked and the paged attention: argument checks and the choice of kernel.
 #include <cudaTypedefs.h>
 
+#include <atomic>
 #include <cmath>
 #include <initializer_list>
+#include <mutex>
 
 #include "attention_view.cuh"
 #include "host_common.h"
@@ -13,9 +15,31 @@ namespace {
 
 static __device__ unsigned g_masked_err;
 
-int error_word_address(unsigned** p) {
-  // resolved for the current device at every call: the address differs per device
-  VB200_CHECK_CUDA(cudaGetSymbolAddress(reinterpret_cast<void**>(p), g_masked_err), "cudaGetSymbolAddress(g_masked_err)");
+// What does not change about a device: that it is an sm_100 one, its SMs, the address of its error word.
+struct DeviceFacts {
+  int sms;
+  unsigned* err;
+};
+
+int device_facts(DeviceFacts& f) {
+  static DeviceFacts known[64];
+  static std::atomic<bool> ready[64];
+  int dev = 0;
+  VB200_CHECK_CUDA(cudaGetDevice(&dev), "cudaGetDevice");
+  if (dev >= 0 && dev < 64 && ready[dev].load(std::memory_order_acquire)) {
+    f = known[dev];
+    return VB200_OK;
+  }
+  const int rc = check_sm100();
+  if (rc != VB200_OK) return rc;
+  VB200_CHECK_CUDA(cudaDeviceGetAttribute(&f.sms, cudaDevAttrMultiProcessorCount, dev), "cudaDeviceGetAttribute");
+  VB200_CHECK_CUDA(cudaGetSymbolAddress(reinterpret_cast<void**>(&f.err), g_masked_err), "cudaGetSymbolAddress(g_masked_err)");
+  if (dev >= 0 && dev < 64) {
+    static std::mutex write;
+    std::lock_guard<std::mutex> lock(write);
+    known[dev] = f;
+    ready[dev].store(true, std::memory_order_release);
+  }
   return VB200_OK;
 }
 
@@ -47,9 +71,13 @@ bool aligned(const void* p, const int64_t* s, std::initializer_list<int64_t> siz
   return ok;
 }
 
-// fp32, or at most 16 (row, head) pairs per key head.  A tile of the other kernel has 128 rows of one head, so below that its
-// tiles are nearly empty and the heads of a group read their keys one by one.
-bool few_rows(int dtype, int64_t rows, int group) { return dtype == VB200_F32 || rows * group <= 16; }
+// fp32; at most 16 (row, head) pairs per key head, since a tile of the other kernel has 128 rows of one head, so below that
+// its tiles are nearly empty and the heads of a group read their keys one by one; or at most 32 blocks of 16 pairs in
+// all, where either kernel leaves SMs idle and the lighter one ends sooner (17 rows, 16 heads, 1041 keys: 12 against 18 us,
+// 16,464 keys: 29 against 35; 33 rows and 4116 keys, beyond the rule: 27 against 20).
+bool few_rows(int dtype, int64_t rows, int64_t group, int64_t heads_and_sequences) {
+  return dtype == VB200_F32 || rows * group <= 16 || (rows * group + 15) / 16 * heads_and_sequences <= 32;
+}
 
 }  // namespace
 
@@ -78,10 +106,8 @@ int pool_map(CUtensorMap* map, const void* base, int dtype, const AttnView& a, i
 }
 
 int sm_count_of_device() {
-  int dev = 0, n = 0;
-  if (cudaGetDevice(&dev) != cudaSuccess) return 0;
-  if (cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess) return 0;
-  return n;
+  DeviceFacts f;
+  return device_facts(f) == VB200_OK ? f.sms : 0;
 }
 
 unsigned masked_error_word(int clear) {
@@ -99,13 +125,13 @@ unsigned masked_error_word(int clear) {
 using namespace vb200;
 
 extern "C" size_t vb200_masked_attention_workspace_size(int dtype, int64_t B, int64_t H, int64_t Hkv, int64_t Nq, int64_t Nk) {
-  if (B < 1 || H < 1 || Hkv < 1 || Nq < 1 || Nk < 1 || few_rows(dtype, Nq, static_cast<int>(H / Hkv))) return 0;
+  if (B < 1 || H < 1 || Hkv < 1 || Nq < 1 || Nk < 1 || few_rows(dtype, Nq, H / Hkv, Hkv * B)) return 0;
   return tile_attention_workspace(false, Nq, B, H, Nk);
 }
 
 extern "C" size_t vb200_paged_attention_workspace_size(int dtype, int64_t rows, int64_t H, const vb200_paged_cache* cache, int64_t n) {
   if (cache == nullptr || rows < 1 || H < 1 || n < 1 || cache->kv_heads < 1 || cache->max_pages < 1 || cache->page_size < 1 ||
-      few_rows(dtype, (rows + n - 1) / n, static_cast<int>(H / cache->kv_heads)))
+      few_rows(dtype, (rows + n - 1) / n, H / cache->kv_heads, cache->kv_heads * n))
     return 0;
   return tile_attention_workspace(true, rows, n, H, cache->max_pages * cache->page_size);
 }
@@ -131,7 +157,9 @@ extern "C" int vb200_masked_attention(int dtype, const void* q, const void* k, c
   AttnView a{};
   int rc = fill_mods(mods, a);
   if (rc != VB200_OK) return rc;
-  if ((rc = check_sm100()) != VB200_OK || (rc = error_word_address(&a.err)) != VB200_OK) return rc;
+  DeviceFacts facts;
+  if ((rc = device_facts(facts)) != VB200_OK) return rc;
+  a.err = facts.err;
   a.q = q, a.k = k, a.v = v, a.out = out;
   a.q_sb = qs[0], a.q_sh = qs[1], a.q_sn = qs[2];
   a.k_sb = ks[0], a.k_sh = ks[1], a.k_sn = ks[2];
@@ -142,7 +170,7 @@ extern "C" int vb200_masked_attention(int dtype, const void* q, const void* k, c
   a.bias = mods->key_bias, a.bias_sb = mods->key_bias_sb;
   a.qpos = mods->q_position, a.qpos_sb = mods->q_position_sb;
   a.kpos = mods->k_position, a.kpos_sb = mods->k_position_sb;
-  if (few_rows(dtype, Nq, a.group)) return rows_attention(dtype, false, a, Nk, static_cast<cudaStream_t>(stream));
+  if (few_rows(dtype, Nq, a.group, Hkv * B)) return rows_attention(dtype, false, a, Nk, static_cast<cudaStream_t>(stream));
   return tile_attention(dtype, false, a, Nk, workspace, workspace_bytes, static_cast<cudaStream_t>(stream));
 }
 
@@ -171,7 +199,9 @@ extern "C" int vb200_paged_attention(int dtype, const void* q, void* out, int64_
   AttnView a{};
   int rc = fill_mods(mods, a);
   if (rc != VB200_OK) return rc;
-  if ((rc = check_sm100()) != VB200_OK || (rc = error_word_address(&a.err)) != VB200_OK) return rc;
+  DeviceFacts facts;
+  if ((rc = device_facts(facts)) != VB200_OK) return rc;
+  a.err = facts.err;
   a.q = q, a.k = cache->k, a.v = cache->v, a.out = out;
   a.q_sh = qs[0], a.q_sn = qs[1], a.o_sh = os[0], a.o_sn = os[1];
   a.Hkv = static_cast<int>(cache->kv_heads);
@@ -187,6 +217,6 @@ extern "C" int vb200_paged_attention(int dtype, const void* q, void* out, int64_
   a.page_shift = cache->page_size == 16 ? 4 : cache->page_size == 32 ? 5 : cache->page_size == 64 ? 6 : 7;
   a.max_pages = static_cast<int>(cache->max_pages), a.causal = causal;
   const int64_t most = cache->max_pages * cache->page_size;
-  if (few_rows(dtype, (rows + n - 1) / n, a.group)) return rows_attention(dtype, true, a, most, static_cast<cudaStream_t>(stream));
+  if (few_rows(dtype, (rows + n - 1) / n, a.group, cache->kv_heads * n)) return rows_attention(dtype, true, a, most, static_cast<cudaStream_t>(stream));
   return tile_attention(dtype, true, a, most, workspace, workspace_bytes, static_cast<cudaStream_t>(stream));
 }

@@ -32,6 +32,7 @@ static __device__ unsigned g_cache_err;
 
 constexpr int kBook = 1024;  // threads of the bookkeeping CTAs
 constexpr int kForkCtas = 8;
+constexpr int kFewSlots = 128;
 
 struct CacheView {
   uint8_t *k, *v;
@@ -84,18 +85,32 @@ __global__ void __launch_bounds__(kBook, 1)
                        AppendWork w) {
   __shared__ int red[33];
   __shared__ int fail;
+  __shared__ int slots[kFewSlots];
   const int tid = threadIdx.x;
   if (tid == 0) fail = 0;
-  for (int i = tid; i < n; i += kBook) {
-    const int slot = sequence[i];
-    if (slot >= 0 && slot < c.slots) w.claim[slot] = 0x7fffffff;
+  // The first of a slot's mentions counts.  Few sequences compare their slots in shared memory; many claim them in the
+  // workspace, two more round trips to memory.
+  if (n <= kFewSlots) {
+    if (tid < n) slots[tid] = sequence[tid];
+    __syncthreads();
+  } else {
+    for (int i = tid; i < n; i += kBook) {
+      const int slot = sequence[i];
+      if (slot >= 0 && slot < c.slots) w.claim[slot] = 0x7fffffff;
+    }
+    __syncthreads();
+    for (int i = tid; i < n; i += kBook) {
+      const int slot = sequence[i];
+      if (slot >= 0 && slot < c.slots) atomicMin(&w.claim[slot], i);
+    }
+    __syncthreads();
   }
-  __syncthreads();
-  for (int i = tid; i < n; i += kBook) {
-    const int slot = sequence[i];
-    if (slot >= 0 && slot < c.slots) atomicMin(&w.claim[slot], i);
-  }
-  __syncthreads();
+  auto first_mention = [&](int i, int slot) {
+    if (n > kFewSlots) return w.claim[slot] == i;
+    for (int k = 0; k < i; ++k)
+      if (slots[k] == slot) return false;
+    return true;
+  };
   long long needs = 0;
   for (int base = 0; base < n; base += kBook) {
     const int i = base + tid;
@@ -104,7 +119,7 @@ __global__ void __launch_bounds__(kBook, 1)
       const int slot = sequence[i], o0 = offsets[i], o1 = offsets[i + 1];
       if (o0 < 0 || o1 < o0 || o1 > tokens) {  // with ascending offsets the sums below fit in 32 bits
         atomicOr(&fail, 2);
-      } else if (slot < 0 || slot >= c.slots || w.claim[slot] != i) {
+      } else if (slot < 0 || slot >= c.slots || !first_mention(i, slot)) {
         atomicOr(&g_cache_err, kErrBadArgument);  // a slot out of range or named before: left out
       } else {
         const int count = o1 - o0;
@@ -195,6 +210,7 @@ __global__ void __launch_bounds__(256)
                         long long v_sh, int head_vecs, const float* __restrict__ mass, AppendWork w) {
   const int lane = threadIdx.x & 31;
   const long long row = static_cast<long long>(blockIdx.x) * 8 + (threadIdx.x >> 5);
+  cudaGridDependencySynchronize();  // launched while the plan still runs
   if (w.status[0] == 0) return;
   const uint8_t *ks, *vs;
   const float* ms = nullptr;
@@ -372,6 +388,7 @@ __global__ void __launch_bounds__(kBook, 1) compact_plan_kernel(const CacheView 
 
 // 16 KB pieces of the moving pages, and the tables' new page numbers.
 __global__ void __launch_bounds__(256) compact_move_kernel(const CacheView c, const int* __restrict__ used, CompactWork w) {
+  cudaGridDependencySynchronize();  // launched while the plan still runs
   const int moves = w.moves[0], L = used[0];
   if (moves == 0) return;
   constexpr int U = 4;
@@ -404,6 +421,21 @@ __global__ void __launch_bounds__(256) compact_move_kernel(const CacheView c, co
 }
 
 // ---------------------------------------------------------------- host
+
+// Launches a kernel that may start before the one in front of it on the stream has ended (it waits itself).
+template <typename... P, typename... A>
+cudaError_t launch_behind(void (*kernel)(P...), unsigned grid, cudaStream_t st, const A&... args) {
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(grid);
+  cfg.blockDim = dim3(256);
+  cfg.stream = st;
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = at;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, kernel, args...);
+}
 
 int element_size(int dtype) { return dtype == VB200_F32 ? 4 : 2; }
 
@@ -488,9 +520,11 @@ extern "C" int vb200_cache_append(const vb200_paged_cache* cache, int dtype, con
   VB200_REQUIRE((rows + 7) / 8 < (1ll << 31), "cache_append: too many rows");
   const int64_t zero[2] = {0, 0};
   const int64_t *ks = tokens > 0 ? k_strides : zero, *vs = tokens > 0 ? v_strides : zero;
-  append_write_kernel<<<static_cast<unsigned>((rows + 7) / 8), 256, 0, st>>>(
-      c, sequence, offsets, static_cast<int>(n), static_cast<int>(tokens), static_cast<const uint8_t*>(k), static_cast<const uint8_t*>(v),
-      ks[0] * es, ks[1] * es, vs[0] * es, vs[1] * es, 64 * es / 16, log_mass, w);
+  VB200_CHECK_CUDA(launch_behind(append_write_kernel, static_cast<unsigned>((rows + 7) / 8), st, c, sequence, offsets, static_cast<int>(n),
+                                 static_cast<int>(tokens), static_cast<const uint8_t*>(k), static_cast<const uint8_t*>(v),
+                                 static_cast<long long>(ks[0] * es), static_cast<long long>(ks[1] * es), static_cast<long long>(vs[0] * es),
+                                 static_cast<long long>(vs[1] * es), 64 * es / 16, log_mass, w),
+                   "append_write_kernel");
   VB200_CHECK_LAUNCH("append_write_kernel");
   return VB200_OK;
 }
@@ -565,7 +599,7 @@ extern "C" int vb200_cache_compact(const vb200_paged_cache* cache, int dtype, in
   // eight CTAs of 256 threads fill an SM; no more than there can be pieces
   const long long most = static_cast<long long>(c.pages) * 2 * ((static_cast<long long>(c.page) * c.row_vecs + 1023) / 1024);
   const unsigned grid = static_cast<unsigned>(most < 148 * 8 ? most : 148 * 8);
-  compact_move_kernel<<<grid, 256, 0, st>>>(c, used, w);
+  VB200_CHECK_CUDA(launch_behind(compact_move_kernel, grid, st, c, static_cast<const int*>(used), w), "compact_move_kernel");
   VB200_CHECK_LAUNCH("compact_move_kernel");
   return VB200_OK;
 }

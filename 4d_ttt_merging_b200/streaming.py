@@ -15,6 +15,7 @@ has no counterpart (its inference is one clip, batch one).
 """
 from __future__ import annotations
 
+import contextlib
 import ctypes
 import math
 from dataclasses import dataclass
@@ -27,11 +28,20 @@ from .ops import _tma_ready
 __all__ = ["PagedCache", "attention_ranges", "masked_attention", "paged_attention"]
 
 _PAGES = (16, 32, 64, 128)
+_Two = ctypes.c_int64 * 2
+_HERE = contextlib.nullcontext()
+
+
+def _on(device: torch.device):
+    """The device made current for a call, where it is not already."""
+    return _HERE if torch.cuda.current_device() == device.index else torch.cuda.device(device)
 
 
 def _refuse_gradients(what: str, *tensors) -> None:
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
-        raise RuntimeError(f"{what} has no backward pass: call it under torch.no_grad() or detach its inputs")
+    if torch.is_grad_enabled():
+        for t in tensors:
+            if t is not None and t.requires_grad:
+                raise RuntimeError(f"{what} has no backward pass: call it under torch.no_grad() or detach its inputs")
 
 
 def _same_device(what: str, device: torch.device, *tensors) -> None:
@@ -43,7 +53,10 @@ def _same_device(what: str, device: torch.device, *tensors) -> None:
 def _rows(t: torch.Tensor) -> torch.Tensor:
     """``t``, or a packed copy where the kernels cannot read it: a channel stride, rows that are not 16-byte aligned (a
     packed tensor at an odd offset too), broadcast dimensions."""
-    if _tma_ready(t) and 0 not in t.stride():
+    if t.is_contiguous():
+        if t.data_ptr() % 16 == 0:
+            return t
+    elif _tma_ready(t) and 0 not in t.stride():
         return t
     return t.clone(memory_format=torch.contiguous_format)
 
@@ -71,6 +84,9 @@ def _positive(what: str, value: float | None) -> float:
 
 def _int_vector(what: str, t, device: torch.device, n: int | None = None) -> torch.Tensor:
     """A 1-D int32 device tensor; lists and other integer tensors are converted."""
+    if isinstance(t, torch.Tensor) and t.dtype is torch.int32 and t.device == device and t.ndim == 1 and t.is_contiguous() and (
+            n is None or t.numel() == n):
+        return t
     if not isinstance(t, torch.Tensor):
         t = torch.tensor(t, dtype=None if len(t) else torch.int32)
     if t.ndim != 1 or t.dtype.is_floating_point or t.dtype == torch.bool or (n is not None and t.numel() != n):
@@ -152,7 +168,7 @@ def masked_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, log_key_
     C.require_cuda(q, "masked_attention")
     _same_device("masked_attention", q.device, k, v, log_key_mass, key_range, distance_slope, query_position, key_position, out)
     _refuse_gradients("masked_attention", q, k, v, log_key_mass, distance_slope, query_position, key_position)
-    with torch.cuda.device(q.device):
+    with _on(q.device):
         if out is None:
             out = torch.empty((B, Nq, H, D), device=q.device, dtype=q.dtype).transpose(1, 2)
         if out.numel() == 0:
@@ -225,6 +241,7 @@ class PagedCache:
             raise ValueError("cache tensors must be contiguous, the pools 16-byte aligned")
         C.require_cuda(k, "PagedCache")
         _same_device("PagedCache", k.device, *every)
+        self._device, self._heads = k.device, heads
         self._handle = C.CacheHandle(*(C.ptr(t) for t in (k, self.v, self.log_mass, *ints)), pages, page, heads, *self.table.shape)
 
     @classmethod
@@ -245,18 +262,18 @@ class PagedCache:
 
     @property
     def heads(self) -> int:
-        return self.k.shape[2]
+        return self._heads
 
     @property
     def device(self) -> torch.device:
-        return self.k.device
+        return self._device
 
     def append(self, sequence, offsets, k: torch.Tensor, v: torch.Tensor, log_mass: torch.Tensor | None = None) -> None:
         """Rows offsets[i] .. offsets[i + 1] of k, v [tokens, kv heads, 64] and log_mass [tokens] go behind the tokens of slot
         sequence[i].  Pages are taken lowest number first; a shared, partly filled last page is copied before it is written.
         All or nothing: a pool or a table row that is too short leaves the cache as it was (error bit 2).  A slot named
         twice in one call takes its first chunk only (error bit 1).  Without log_mass the tokens have mass 1."""
-        dev = self.k.device
+        dev = self._device
         if k.ndim != 3 or k.shape[1:] != self.k.shape[2:] or v.shape != k.shape:
             raise ValueError(f"append: k and v must be [tokens, {self.heads}, 64]")
         if k.dtype != self.k.dtype or v.dtype != self.k.dtype:
@@ -267,7 +284,7 @@ class PagedCache:
             raise ValueError(f"append: log_mass must be [{k.shape[0]}]")
         _same_device("append", dev, k, v, log_mass)
         _refuse_gradients("append", k, v, log_mass)
-        with torch.cuda.device(dev):
+        with _on(dev):
             sequence = _int_vector("sequence", sequence, dev)
             n = sequence.numel()
             offsets = _int_vector("offsets", offsets, dev, n + 1)
@@ -277,17 +294,16 @@ class PagedCache:
             lib = C.lib()
             size = lib.vb200_cache_append_workspace_size(n, self.table.shape[0], self.k.shape[0])
             ws = _scratch(size, dev)
-            two = ctypes.c_int64 * 2
             rc = lib.vb200_cache_append(self._handle, self._dtype, sequence.data_ptr(), offsets.data_ptr(), n, k.data_ptr(),
-                                        v.data_ptr(), C.ptr(log_mass), k.shape[0], two(*k.stride()[:2]), two(*v.stride()[:2]),
+                                        v.data_ptr(), C.ptr(log_mass), k.shape[0], _Two(*k.stride()[:2]), _Two(*v.stride()[:2]),
                                         C.ptr(ws), size, C.stream_of(dev))
             C.check(rc, "PagedCache.append")
 
     def fork(self, source, target) -> None:
         """Slot target[i] gets the tokens of slot source[i] by sharing its pages, and gives back what it held.  All
         sources are read before any target is written; of several pairs with one target the last counts."""
-        dev = self.k.device
-        with torch.cuda.device(dev):
+        dev = self._device
+        with _on(dev):
             source = _int_vector("source", source, dev)
             target = _int_vector("target", target, dev, source.numel())
             lib = C.lib()
@@ -299,16 +315,16 @@ class PagedCache:
 
     def free(self, sequence) -> None:
         """Empties slots; pages that no other slot shares become free."""
-        dev = self.k.device
-        with torch.cuda.device(dev):
+        dev = self._device
+        with _on(dev):
             sequence = _int_vector("sequence", sequence, dev)
             rc = C.lib().vb200_cache_free(self._handle, self._dtype, sequence.data_ptr(), sequence.numel(), C.stream_of(dev))
             C.check(rc, "PagedCache.free")
 
     def compact(self) -> torch.Tensor:
         """Moves the pages in use to the front of the pool and returns their number (int32 [1], on the device)."""
-        dev = self.k.device
-        with torch.cuda.device(dev):
+        dev = self._device
+        with _on(dev):
             lib = C.lib()
             size = lib.vb200_cache_compact_workspace_size(self.k.shape[0])
             ws = _scratch(size, dev)
@@ -332,8 +348,8 @@ def paged_attention(q: torch.Tensor, cache: PagedCache, sequence, offsets, *, ca
     if q.ndim != 3 or q.shape[-1] != 64:
         raise ValueError("q must be [rows, heads, 64]")
     rows, H, D = q.shape
-    if H == 0 or H % cache.heads:
-        raise ValueError(f"{H} query heads are no multiple of the cache's {cache.heads}")
+    if H == 0 or H % cache._heads:
+        raise ValueError(f"{H} query heads are no multiple of the cache's {cache._heads}")
     if q.dtype != cache.k.dtype:
         raise ValueError(f"the cache holds {cache.k.dtype}, q is {q.dtype}")
     softcap = _positive("softcap", softcap)
@@ -345,15 +361,15 @@ def paged_attention(q: torch.Tensor, cache: PagedCache, sequence, offsets, *, ca
     if out is not None and (out.shape != q.shape or out.dtype != q.dtype or not _tma_ready(out)):
         raise ValueError("out must have q's shape and dtype, a unit channel stride and 16-byte aligned rows")
     C.require_cuda(q, "paged_attention")
-    dev = cache.device
+    dev = cache._device
     _same_device("paged_attention", dev, q, key_range, distance_slope, out)
     _refuse_gradients("paged_attention", q, distance_slope)
-    with torch.cuda.device(dev):
+    with _on(dev):
         sequence = _int_vector("sequence", sequence, dev)
         n = sequence.numel()
         offsets = _int_vector("offsets", offsets, dev, n + 1)
         if out is None:
-            out = torch.empty((rows, H, D), device=dev, dtype=q.dtype)
+            out = q.new_empty(rows, H, D)
         q = _rows(q)
         mods = C.ScoreMods(scale=scale, softcap=softcap)
         if key_range is not None:
@@ -365,9 +381,8 @@ def paged_attention(q: torch.Tensor, cache: PagedCache, sequence, offsets, *, ca
         lib = C.lib()
         size = lib.vb200_paged_attention_workspace_size(cache._dtype, rows, H, cache._handle, n)
         ws = _scratch(size, dev)
-        two = ctypes.c_int64 * 2
-        rc = lib.vb200_paged_attention(cache._dtype, q.data_ptr(), out.data_ptr(), rows, H, D, two(q.stride(1), q.stride(0)),
-                                       two(out.stride(1), out.stride(0)), cache._handle, sequence.data_ptr(), offsets.data_ptr(),
+        rc = lib.vb200_paged_attention(cache._dtype, q.data_ptr(), out.data_ptr(), rows, H, D, _Two(q.stride(1), q.stride(0)),
+                                       _Two(out.stride(1), out.stride(0)), cache._handle, sequence.data_ptr(), offsets.data_ptr(),
                                        n, int(causal), mods, C.ptr(ws), size, C.stream_of(dev))
         C.check(rc, "paged_attention")
     return out
