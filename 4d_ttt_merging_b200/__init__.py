@@ -31,11 +31,12 @@ from .ops import (
 from .streaming import PagedCache, attention_ranges, masked_attention, paged_attention
 from .token_plan import TokenPlan, WeightedBilinearTokenPlan
 from .planners import build_fastvggt_plan, build_ttt_protected_uniform_convex_plan, build_uniform_convex_plan
-from .attention_block import GlobalAttention, compute_attention
+from .attention_block import AttentionMask, GlobalAttention, compute_attention
 from .install import install, uninstall
 from . import parallel, ttt_kernels
 
 __all__ = [
+    "AttentionMask",
     "GlobalAttention",
     "PagedCache",
     "PlanCSR",

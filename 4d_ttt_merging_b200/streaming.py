@@ -61,6 +61,13 @@ def _rows(t: torch.Tensor) -> torch.Tensor:
     return t.clone(memory_format=torch.contiguous_format)
 
 
+def _check_out(q: torch.Tensor, out: torch.Tensor) -> None:
+    if out.shape != q.shape or out.dtype != q.dtype or not _tma_ready(out):
+        raise ValueError("out must have q's shape and dtype, a unit channel stride and 16-byte aligned rows")
+    if any(s == 0 and n > 1 for s, n in zip(out.stride(), out.shape)):
+        raise ValueError("out must not be a broadcast tensor")
+
+
 def _scratch(size: int, device: torch.device) -> torch.Tensor | None:
     return torch.empty(size, dtype=torch.uint8, device=device) if size else None
 
@@ -102,7 +109,7 @@ def attention_ranges(queries: int, keys: int | None = None, *, documents: torch.
     ``step``       causal order in blocks of this many tokens from the document's start: 1 is token by token, the tokens
                    of a frame make frames that see themselves and earlier ones.  None: the whole document.
     ``prefix``     the first tokens of a document that every row of it sees (camera and register tokens), besides the above.
-    ``window``     no more than this many tokens back (the row's own counts).
+    ``window``     no more than this many tokens back (the row's own counts), prefix tokens too: a row's keys are one interval.
 
     Everything is computed on the device of ``documents`` (else ``device``), without host synchronisation."""
     keys = queries if keys is None else keys
@@ -163,11 +170,11 @@ def masked_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, log_key_
         raise ValueError(f"distance_slope must be [{H}]")
     if key_range is not None and (key_range.dtype != torch.int32 or key_range.shape not in ((Nq, 2), (B, Nq, 2))):
         raise ValueError(f"key_range must be int32 [{Nq}, 2] or [{B}, {Nq}, 2]")
-    if out is not None and (out.shape != q.shape or out.dtype != q.dtype or not _tma_ready(out)):
-        raise ValueError("out must have q's shape and dtype, a unit channel stride and 16-byte aligned rows")
+    if out is not None:
+        _check_out(q, out)
     C.require_cuda(q, "masked_attention")
     _same_device("masked_attention", q.device, k, v, log_key_mass, key_range, distance_slope, query_position, key_position, out)
-    _refuse_gradients("masked_attention", q, k, v, log_key_mass, distance_slope, query_position, key_position)
+    _refuse_gradients("masked_attention", q, k, v, log_key_mass, distance_slope, query_position, key_position, out)
     with _on(q.device):
         if out is None:
             out = torch.empty((B, Nq, H, D), device=q.device, dtype=q.dtype).transpose(1, 2)
@@ -202,7 +209,7 @@ def masked_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, log_key_
     return out
 
 
-@dataclass
+@dataclass(frozen=True, eq=False)
 class PagedCache:
     """Keys, values and log-masses of streams, in pages of 16, 32, 64 or 128 tokens; all state is on the device.
 
@@ -225,7 +232,7 @@ class PagedCache:
             raise ValueError("cache pools are [pages, 16 | 32 | 64 | 128, kv heads, 64]")
         if self.v.shape != k.shape or self.v.dtype != k.dtype:
             raise ValueError("k and v pools must have one shape and dtype")
-        self._dtype = C.dtype_code(k.dtype)
+        dtype = C.dtype_code(k.dtype)
         pages, page, heads, _ = k.shape
         if pages == 0 or heads == 0:
             raise ValueError("a cache has at least one page and one head")
@@ -241,8 +248,9 @@ class PagedCache:
             raise ValueError("cache tensors must be contiguous, the pools 16-byte aligned")
         C.require_cuda(k, "PagedCache")
         _same_device("PagedCache", k.device, *every)
-        self._device, self._heads = k.device, heads
-        self._handle = C.CacheHandle(*(C.ptr(t) for t in (k, self.v, self.log_mass, *ints)), pages, page, heads, *self.table.shape)
+        # the fields stay what they are, so what every call needs of them is worked out once
+        self.__dict__.update(_device=k.device, _heads=heads, _dtype=dtype, _handle=C.CacheHandle(
+            *(C.ptr(t) for t in (k, self.v, self.log_mass, *ints)), pages, page, heads, *self.table.shape))
 
     @classmethod
     def empty(cls, slots: int, pages: int, max_pages: int, *, page_size: int = 64, heads: int = 16, dtype=torch.bfloat16,
@@ -358,12 +366,12 @@ def paged_attention(q: torch.Tensor, cache: PagedCache, sequence, offsets, *, ca
         raise ValueError(f"distance_slope must be [{H}]")
     if key_range is not None and (key_range.dtype != torch.int32 or key_range.shape != (rows, 2)):
         raise ValueError(f"key_range must be int32 [{rows}, 2]")
-    if out is not None and (out.shape != q.shape or out.dtype != q.dtype or not _tma_ready(out)):
-        raise ValueError("out must have q's shape and dtype, a unit channel stride and 16-byte aligned rows")
+    if out is not None:
+        _check_out(q, out)
     C.require_cuda(q, "paged_attention")
     dev = cache._device
     _same_device("paged_attention", dev, q, key_range, distance_slope, out)
-    _refuse_gradients("paged_attention", q, distance_slope)
+    _refuse_gradients("paged_attention", q, distance_slope, out)
     with _on(dev):
         sequence = _int_vector("sequence", sequence, dev)
         n = sequence.numel()
