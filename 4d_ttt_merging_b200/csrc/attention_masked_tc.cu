@@ -4,16 +4,22 @@
 // CTA per SM, 12 warps:
 //   warps 0-7    two softmax warpgroups, one per query tile, one thread per row (its TMEM lane).  A row's scores sit
 //                in one thread's registers, so the cap, the bias, the distance and the mask are applied once, and
-//                the row's maximum needs no exchange.  A tile of 128 keys is taken in two halves of 64.
+//                the row's maximum needs no exchange.  A tile of 128 keys is taken in parts of 64, or 32 with a cap.
 //   warp 8       TMA producer: Q once; K and V tiles of 128 keys into a ring (dense: one box; paged: a box per page,
 //                pages outside the sequence read a coordinate outside the pool and fill with zeros).
 //   warps 9, 10  one MMA stream per query tile: S(j + 1) = Q K_{j+1}^T as soon as S(j) is in registers, then
 //                O += P(j) V_j.
-//   warp 11      per key: bias and position of the tile, into the ring (only when there are any).  A bias alone rides
+//   warp 11      per key: bias and position of the tile, into the ring (only when there are any).  Without a cap the bias rides
 //                in the QK product: an extra K=16 chunk holds 1, 1, 1 in columns 0 to 2 of every query row and bias /
 //                scale, split into three 16-bit values that add up to its 24 bits, in those of the key row (adding it
 //                in the softmax measured 20% slower).
 // TMEM: S_t at 128 t, P_t at 256 + 64 t (16-bit, the A operand of PV), O_t at 384 + 64 t.
+//
+// Most tiles are seen whole by all rows of a warp and move no row's maximum by 2^8: their probabilities are formed straight from
+// the products, with the maximum as it is, and the tile's maximum is looked at afterwards; the first tile, tiles that the
+// mask cuts and tiles after a miss take their maximum first.  With a cap this lets its polynomial (FMA pipe) run beside the
+// exponentials: 213 -> 154 us (1024 rows, 8192 keys, 37 heads; parts of 64 keys
+// instead of 32 leave the compiler too few registers to interleave them: 186); without a cap 127 -> 117.
 //
 // The two warps of an SM sub-partition compute their exponentials at the same time and leave the unit idle at the same time
 // (3200 clocks per 256 x 128 scores, 2100 of them in exponentials); making them take turns measured 8% slower, starting one
@@ -35,7 +41,8 @@
 // does not depend on which one that is.  (Parts in a cluster, joined in distributed shared memory, need whole clusters of
 // SMs at a time, 128 of 148 for clusters of 8, and one split for all blocks: a frame of 1041 rows over 33,969 keys took 405 us.)
 //
-// The running maximum is lazy: O is rescaled only when a row's maximum grows by more than 2^8.  Probabilities are
+// The running maximum is lazy: O is rescaled only when a row's maximum grows by more than 2^8; the new one is set 2^4 above it,
+// so that the next tiles seldom exceed it again (143 -> 137 us, four clips of 2058 keys).  Probabilities are
 // rounded to the value type for the PV product; sums, maxima and O are fp32.
 #include <cudaTypedefs.h>
 
@@ -49,13 +56,14 @@
 namespace vb200 {
 namespace {
 
-constexpr int kBM = 128, kQT = 2, kBN = 128, kHalf = 64;
+constexpr int kBM = 128, kQT = 2, kBN = 128;
 constexpr int kStages = 4;
 constexpr int kTileBytes = kBN * kHeadDim * 2;  // 16 KB: a Q, K or V tile
 constexpr int kSoftmaxWarps = 8;
 constexpr int kWarpProducer = 8, kWarpMma = 9, kWarpKeys = 11;
 constexpr int kThreads = 12 * 32;
 constexpr float kRescale = 8.f;  // P stays <= 2^8
+constexpr float kMargin = 4.f;   // a new maximum leaves this much room; the largest P stays >= 2^-5
 
 constexpr int kOffQ = 0;
 constexpr int kOffStage = kQT * kTileBytes;
@@ -161,10 +169,11 @@ struct CapPoly {
   float near_limit, far_limit;  // 1/2 and 1
 };
 
-__device__ __forceinline__ float max_of(const uint32_t (&r)[kHalf]) {
+template <int N>
+__device__ __forceinline__ float max_of(const uint32_t (&r)[N]) {
   float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-  for (int c = 0; c < kHalf; c += 8) {
+  for (int c = 0; c < N; c += 8) {
 #pragma unroll
     for (int u = 0; u < 4; ++u) mx[u] = fmax3(mx[u], u2f(r[c + 2 * u]), u2f(r[c + 2 * u + 1]));
   }
@@ -173,14 +182,15 @@ __device__ __forceinline__ float max_of(const uint32_t (&r)[kHalf]) {
 
 // r <- cap * log2(e) * tanh(r s).  On the FMA pipe while no score of the warp is beyond half the cap (five packed
 // instructions a pair) or the cap (seven), else two uses of the exponential unit per score.
-__device__ __forceinline__ void cap_scores(uint32_t (&r)[kHalf], const AttnView& a, const CapPoly& k) {
+template <int N>
+__device__ __forceinline__ void cap_scores(uint32_t (&r)[N], const AttnView& a, const CapPoly& k) {
   float far = 0.f;
 #pragma unroll
-  for (int c = 0; c < kHalf; c += 2) far = fmax3(far, fabsf(u2f(r[c])), fabsf(u2f(r[c + 1])));
+  for (int c = 0; c < N; c += 2) far = fmax3(far, fabsf(u2f(r[c])), fabsf(u2f(r[c + 1])));
   far *= a.scale;
   if (__all_sync(0xffffffffu, far <= k.near_limit)) {
 #pragma unroll
-    for (int c = 0; c < kHalf; c += 2) {
+    for (int c = 0; c < N; c += 2) {
       const uint64_t y = pk2(u2f(r[c]), u2f(r[c + 1])), z = fmul2(y, y);
       uint64_t f = ffma2(k.near_[3], z, k.near_[2]);
       f = ffma2(f, z, k.near_[1]);
@@ -192,7 +202,7 @@ __device__ __forceinline__ void cap_scores(uint32_t (&r)[kHalf], const AttnView&
     }
   } else if (__all_sync(0xffffffffu, far <= k.far_limit)) {
 #pragma unroll
-    for (int c = 0; c < kHalf; c += 2) {
+    for (int c = 0; c < N; c += 2) {
       const uint64_t y = pk2(u2f(r[c]), u2f(r[c + 1])), z = fmul2(y, y);
       uint64_t f = ffma2(k.far_[5], z, k.far_[4]);
       f = ffma2(f, z, k.far_[3]);
@@ -206,52 +216,44 @@ __device__ __forceinline__ void cap_scores(uint32_t (&r)[kHalf], const AttnView&
     }
   } else {
 #pragma unroll
-    for (int c = 0; c < kHalf; ++c) r[c] = f2u(a.cap * tanh_fast(u2f(r[c]) * a.scale));
+    for (int c = 0; c < N; ++c) r[c] = f2u(a.cap * tanh_fast(u2f(r[c]) * a.scale));
   }
 }
 
-// The scores of 64 keys: products in r -> scores of which mul times is the log2 domain, hidden keys at -inf.  kFull: with
-// the cap, the bias and the distance.
-template <bool kFull>
-__device__ __forceinline__ float form_scores(uint32_t (&r)[kHalf], const AttnView& a, const CapPoly& k, const float* keys, float slope,
-                                             float pos, int lo, int hi, bool partly) {
+// The scores of N keys: products in r -> scores of which mul times is the log2 domain, hidden keys at -inf.  kCap: the cap and
+// the tile's values per key are applied here.  apart: the distance too, key by key.
+template <bool kCap, int N>
+__device__ __forceinline__ float form_scores(uint32_t (&r)[N], const AttnView& a, const CapPoly& k, const float* keys, bool apart,
+                                             float slope, float pos, int lo, int hi, bool partly) {
   float mul = a.scale;
-  if constexpr (kFull) {
-    if (a.cap != 0.f) {
-      cap_scores(r, a, k);
-      mul = 1.f;
-    }
-    if (a.bias != nullptr || a.slope != nullptr) {  // without a bias the ring holds zeros
-      const uint64_t sc = pk2(mul, mul);
+  if constexpr (kCap) {
+    cap_scores(r, a, k);
 #pragma unroll
-      for (int c = 0; c < kHalf; c += 4) {
-        const float4 y = *reinterpret_cast<const float4*>(keys + c);
-        float x0, x1;
-        upk2(ffma2(pk2(u2f(r[c]), u2f(r[c + 1])), sc, pk2(y.x, y.y)), x0, x1);
-        r[c] = f2u(x0);
-        r[c + 1] = f2u(x1);
-        upk2(ffma2(pk2(u2f(r[c + 2]), u2f(r[c + 3])), sc, pk2(y.z, y.w)), x0, x1);
-        r[c + 2] = f2u(x0);
-        r[c + 3] = f2u(x1);
-      }
-      mul = 1.f;
+    for (int c = 0; c < N; c += 4) {
+      const float4 y = *reinterpret_cast<const float4*>(keys + c);
+      r[c] = f2u(u2f(r[c]) + y.x);
+      r[c + 1] = f2u(u2f(r[c + 1]) + y.y);
+      r[c + 2] = f2u(u2f(r[c + 2]) + y.z);
+      r[c + 3] = f2u(u2f(r[c + 3]) + y.w);
     }
-    if (a.slope != nullptr) {
+    mul = 1.f;
+  }
+  if (apart) {
 #pragma unroll
-      for (int c = 0; c < kHalf; c += 4) {
-        const float4 y = *reinterpret_cast<const float4*>(keys + kBN + c);
-        r[c] = f2u(fmaf(-slope, fabsf(pos - y.x), u2f(r[c])));
-        r[c + 1] = f2u(fmaf(-slope, fabsf(pos - y.y), u2f(r[c + 1])));
-        r[c + 2] = f2u(fmaf(-slope, fabsf(pos - y.z), u2f(r[c + 2])));
-        r[c + 3] = f2u(fmaf(-slope, fabsf(pos - y.w), u2f(r[c + 3])));
-      }
+    for (int c = 0; c < N; c += 4) {
+      const float4 y = *reinterpret_cast<const float4*>(keys + kBN + c);
+      r[c] = f2u(fmaf(-slope, fabsf(pos - y.x), u2f(r[c]) * mul));
+      r[c + 1] = f2u(fmaf(-slope, fabsf(pos - y.y), u2f(r[c + 1]) * mul));
+      r[c + 2] = f2u(fmaf(-slope, fabsf(pos - y.z), u2f(r[c + 2]) * mul));
+      r[c + 3] = f2u(fmaf(-slope, fabsf(pos - y.w), u2f(r[c + 3]) * mul));
     }
+    mul = 1.f;
   }
   if (partly) {
-    lo = min(max(lo, 0), kHalf);
-    hi = min(max(hi, 0), kHalf);
+    lo = min(max(lo, 0), N);
+    hi = min(max(hi, 0), N);
 #pragma unroll
-    for (int w = 0; w < kHalf / 32; ++w) {
+    for (int w = 0; w < N / 32; ++w) {
       // bits [lo, hi) of this word of 32 columns
       const int l0 = min(max(lo - 32 * w, 0), 32), h0 = min(max(hi - 32 * w, 0), 32);
       const uint32_t up = h0 >= 32 ? 0xffffffffu : (1u << h0) - 1u;
@@ -265,14 +267,13 @@ __device__ __forceinline__ float form_scores(uint32_t (&r)[kHalf], const AttnVie
   return mul;
 }
 
-// p[c] <- (2^(r[2c] mul - m), 2^(r[2c+1] mul - m)) in 16 bits; returns the sum of the unrounded values.
-template <typename T>
-__device__ __forceinline__ float probabilities(const uint32_t (&r)[kHalf], float mul, float m, uint32_t* p) {
-  const float m_use = m == -INFINITY ? 0.f : m;
-  const uint64_t neg_m2 = pk2(-m_use, -m_use), mul2 = pk2(mul, mul);
+// p[c] <- (2^(r[2c] mul + off), 2^(r[2c+1] mul + off)) in 16 bits; returns the sum of the unrounded values.
+template <typename T, int N>
+__device__ __forceinline__ float probabilities(const uint32_t (&r)[N], float mul, float off, uint32_t* p) {
+  const uint64_t neg_m2 = pk2(off, off), mul2 = pk2(mul, mul);
   uint64_t ls0 = pk2(0.f, 0.f), ls1 = pk2(0.f, 0.f);
 #pragma unroll
-  for (int c = 0; c < kHalf / 2; ++c) {
+  for (int c = 0; c < N / 2; ++c) {
     float e0, e1, q0, q1;
     upk2(ffma2(pk2(u2f(r[2 * c]), u2f(r[2 * c + 1])), mul2, neg_m2), e0, e1);
     q0 = ex2_approx(e0);
@@ -287,11 +288,64 @@ __device__ __forceinline__ float probabilities(const uint32_t (&r)[kHalf], float
   return (a0 + a1) + (b0 + b1);
 }
 
+// The same for keys that every row of the warp sees, straight from the products and with the maximum that the row has so far,
+// so that the exponential unit, the FMA pipe (cap, exponents, sums) and the ALU (maxima) work side by side instead of one
+// after the other.  False for a row whose maximum grows by more than 2^8 or, with a cap, whose scores leave the polynomial's
+// range: then nothing of it holds, and r is as it was.  off: what is added to a score, less the maximum; most: by how much a
+// score may exceed it.
+template <typename T, bool kCap, int N>
+__device__ __forceinline__ bool probabilities_at_once(const uint32_t (&r)[N], const AttnView& a, const CapPoly& k, const float* keys,
+                                                      float off, float most, uint32_t* p, float& sum) {
+  const uint64_t off2 = pk2(off, off), mul2 = pk2(a.scale, a.scale);
+  uint64_t ls[2] = {pk2(0.f, 0.f), pk2(0.f, 0.f)};
+  float top[2] = {-INFINITY, -INFINITY}, far[2] = {0.f, 0.f};
+#pragma unroll
+  for (int c = 0; c < N; c += 4) {
+    float4 key = make_float4(0.f, 0.f, 0.f, 0.f);
+    if constexpr (kCap) key = *reinterpret_cast<const float4*>(keys + c);
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      const float x0 = u2f(r[c + 2 * u]), x1 = u2f(r[c + 2 * u + 1]);
+      const uint64_t x = pk2(x0, x1);
+      uint64_t e;
+      if constexpr (kCap) {
+        far[u] = fmax3(far[u], fabsf(x0), fabsf(x1));
+        const uint64_t z = fmul2(x, x);
+        uint64_t f = ffma2(k.near_[3], z, k.near_[2]);
+        f = ffma2(f, z, k.near_[1]);
+        f = ffma2(f, z, k.near_[0]);
+        e = fadd2(ffma2(f, x, u ? pk2(key.z, key.w) : pk2(key.x, key.y)), off2);
+      } else {
+        e = ffma2(x, mul2, off2);
+      }
+      float e0, e1;
+      upk2(e, e0, e1);
+      top[u] = fmax3(top[u], e0, e1);
+      const float q0 = ex2_approx(e0), q1 = ex2_approx(e1);
+      ls[u] = fadd2(ls[u], pk2(q0, q1));
+      p[c / 2 + u] = pack2<T>(q0, q1);
+    }
+  }
+  float a0, a1, b0, b1;
+  upk2(ls[0], a0, a1);
+  upk2(ls[1], b0, b1);
+  sum = (a0 + a1) + (b0 + b1);
+  return fmaxf(top[0], top[1]) <= most && (!kCap || fmaxf(far[0], far[1]) * a.scale <= k.near_limit);
+}
+
 // What three 16-bit values hold of bias / scale; their product with 1 is exact in fp32.
 template <typename T>
 constexpr float kMostBias = std::is_same<T, __nv_bfloat16>::value ? 1e30f : 60000.f;
 
-// kForm: 0 plain scores; 1 with a bias, in the product; 2 with a cap or a distance, and a bias in the softmax.
+// kForm: 0 plain scores; 1 with a bias, in the product; 2 with a cap, bias and distance in the softmax; 3 with a distance and no
+// cap, in the product like a bias.
+//
+// Distance.  Where positions are token indices and all keys of a tile lie on one side of all rows, slope |pos - key| is
+// slope |pos - ref|, one number per row, plus slope |ref - key|, one per key, with ref the tile's key nearest to the rows:
+// the second is a bias like any other, and the first goes where the maximum is subtracted.  The few tiles among the rows'
+// own positions, tiles of explicit positions and negative slopes take the distance key by key in the softmax.  (All tiles key
+// by key: 195 us instead of 112 without a distance, six streams of 42 to 542 new tokens over 1900 to 9600.)  With a distance the
+// tiles are taken last to first: a causal row then meets its largest scores first, and its maximum hardly ever grows.
 //
 // A bias that does not fit in the product: one below the range (the type's lowest value, say) hides its key there, as -inf
 // does, and a row that ends with no probability, or with a maximum so low that such a key might count, is computed again
@@ -323,8 +377,10 @@ __global__ void __launch_bounds__(kThreads, 1)
   auto bar = [=](int i) -> uint32_t { return sbase + kOffBar + 8 * i; };
   int* key_lo = reinterpret_cast<int*>(smem + kOffMisc + 8);
   int* key_hi = key_lo + kQT;
-  constexpr bool in_product = kForm == 1;
-  const bool per_key = kForm == 1 || (kForm == 2 && (a.bias != nullptr || a.slope != nullptr));
+  // keys of a tile that are in registers at a time
+  constexpr int kPart = kForm == 2 ? 32 : 64, kParts = kBN / kPart;
+  constexpr bool in_product = kForm == 1 || kForm == 3;
+  constexpr bool per_key = kForm != 0;  // without a bias and a distance form 2's ring holds zeros
 
   if (threadIdx.x == 0) {
     mbar_init(bar(kBarQ), 1);
@@ -402,12 +458,31 @@ __global__ void __launch_bounds__(kThreads, 1)
   }
   if (j0[0] == j1[0] && j0[1] == j1[1]) p1 = p0;  // the part lies between the two query tiles' keys
 
+  // Tiles are counted by u from 0 to n_tiles; first to last, or last to first with a distance.  Query tile t takes [ua, ub).
+  const int n_tiles = p1 - p0;
+  const bool down = kForm == 3 || (kForm == 2 && a.slope != nullptr);
+  auto tile_of = [=](int u) -> int { return down ? p1 - 1 - u : p0 + u; };
+  int ua[kQT], ub[kQT];
+#pragma unroll
+  for (int t = 0; t < kQT; ++t) {
+    ua[t] = down ? p1 - j1[t] : j0[t] - p0;
+    ub[t] = down ? p1 - j0[t] : j1[t] - p0;
+    if (n_tiles == 0) ua[t] = ub[t] = 0;
+  }
+  const float slope = down ? __ldg(a.slope + head) * kLog2E : 0.f;
+  const bool by_side = down && a.qpos == nullptr && a.kpos == nullptr && slope >= 0.f;
+  const int pos_first = s.keys - s.rows + row_first;
+  // 1: all keys of the tile at or before all rows; -1: at or behind; 0: neither, or not asked
+  auto side_of = [=](int j) -> int {
+    return !by_side ? 0 : j * kBN + kBN - 1 <= pos_first ? 1 : j * kBN >= pos_first + kQT * kBM - 1 ? -1 : 0;
+  };
+
   // Paged: the tile whose last page the sequence fills in part.  The slots behind the last key hold anything, NaN perhaps, so
   // warp 11 overwrites their values with zeros before the PV product reads them.  -1: none in this part.
   int tail = -1;
   if (kPaged && (s.keys & (kBN - 1)) != 0) {
     const int j = s.keys / kBN;
-    if ((j >= j0[0] && j < j1[0]) || (j >= j0[1] && j < j1[1])) tail = j;
+    if ((j >= j0[0] && j < j1[0]) || (j >= j0[1] && j < j1[1])) tail = down ? p1 - 1 - j : j - p0;
   }
 
   // A wait that runs out makes its role go on without waiting (or leave), so that every thread reaches the end and
@@ -422,20 +497,20 @@ __global__ void __launch_bounds__(kThreads, 1)
         return static_cast<long long>(slot) << a.page_shift < s.keys ? page_of(a, s, slot) : a.pages;
       };
       int id = 0;
-      if (kPaged && which < 2 && p0 < p1) id = page_at(p0);
-      if (lane == 0 && p0 < p1) {
+      if (kPaged && which < 2 && n_tiles > 0) id = page_at(tile_of(0));
+      if (lane == 0 && n_tiles > 0) {
         mbar_arrive_expect_tx(bar(kBarQ), kQT * kTileBytes);
         for (int t = 0; t < kQT; ++t)
           tma_load_4d(sbase + kOffQ + t * kTileBytes, &tmap_q, bar(kBarQ), 0, s.row0 + row_first + t * kBM, head, s.batch);
       }
-      int j = p0;
+      int n = 0;
       bool ok = true;
-      for (; j < p1; ++j) {
-        const int n = j - p0, st = n % kStages;
+      for (; n < n_tiles; ++n) {
+        const int st = n % kStages;
         if (n >= kStages) ok = __all_sync(0xffffffffu, mbar_wait(bar(kBarEmpty + st), (n / kStages - 1) & 1, a.err));
         if (!ok) break;
         // a tile between the two query tiles' keys is not loaded
-        const bool used = (j >= j0[0] && j < j1[0]) || (j >= j0[1] && j < j1[1]);
+        const bool used = (n >= ua[0] && n < ub[0]) || (n >= ua[1] && n < ub[1]);
         if (lane == 0) {
           if (used) mbar_arrive_expect_tx(bar(kBarFull + st), 2 * kTileBytes);
           else mbar_arrive(bar(kBarFull + st));
@@ -446,41 +521,41 @@ __global__ void __launch_bounds__(kThreads, 1)
           if (which < 2) {
             if (used)
               tma_load_4d(dst + which * kTileBytes + pg * (kTileBytes / npg), which ? &tmap_v : &tmap_k, bar(kBarFull + st), 0, hk, 0, id);
-            if (j + 1 < p1) id = page_at(j + 1);
+            if (n + 1 < n_tiles) id = page_at(tile_of(n + 1));
           }
         } else if (lane < 2 && used) {
-          tma_load_4d(dst + lane * kTileBytes, lane ? &tmap_v : &tmap_k, bar(kBarFull + st), 0, j * kBN, hk, s.batch);
+          tma_load_4d(dst + lane * kTileBytes, lane ? &tmap_v : &tmap_k, bar(kBarFull + st), 0, tile_of(n) * kBN, hk, s.batch);
         }
       }
       if (!ok) {  // the copies in flight land before the CTA leaves
         mbar_wait(bar(kBarQ), 0, a.err);
-        for (int n = max(j - p0 - kStages, 0); n < j - p0; ++n) mbar_wait(bar(kBarFull + n % kStages), (n / kStages) & 1, a.err);
+        for (int u = max(n - kStages, 0); u < n; ++u) mbar_wait(bar(kBarFull + u % kStages), (u / kStages) & 1, a.err);
       }
     } else if (warp < kWarpMma + kQT) {
       // ------------------------------- MMA issuer of query tile t -------------------------------
       const int t = warp - kWarpMma;
-      const int ja = t == 0 ? j0[0] : j0[1], jb = t == 0 ? j1[0] : j1[1];
+      const int ja = t == 0 ? ua[0] : ua[1], jb = t == 0 ? ub[0] : ub[1];
       constexpr uint32_t idesc_qk = idesc_f16(kBM, kBN, kBF16 ? 1 : 0, 0, 0);
       constexpr uint32_t idesc_pv = idesc_f16(kBM, kHeadDim, kBF16 ? 1 : 0, 0, 1);
       const uint64_t q_desc = smem_desc_sw128(sbase + kOffQ + t * kTileBytes, 16, 1024);
       const uint64_t k_desc = smem_desc_sw128(sbase + kOffStage, 16, 1024);
       const uint64_t v_desc = smem_desc_sw128(sbase + kOffStage + kTileBytes, 16384, 1024);
-      auto stage_off = [=](int j) -> uint64_t { return static_cast<uint64_t>(((j - p0) % kStages) * (2 * kTileBytes >> 4)); };
+      auto stage_off = [=](int j) -> uint64_t { return static_cast<uint64_t>((j % kStages) * (2 * kTileBytes >> 4)); };
       auto wait_all = [&](int b, int parity) -> bool {
         return __all_sync(0xffffffffu, mbar_wait(bar(b), static_cast<uint32_t>(parity), a.err));
       };
-      auto full = [&](int j) -> bool { return wait_all(kBarFull + (j - p0) % kStages, ((j - p0) / kStages) & 1); };
+      auto full = [&](int j) -> bool { return wait_all(kBarFull + j % kStages, (j / kStages) & 1); };
       const uint64_t qx_desc = smem_desc_noswz(sbase + kOffExtra, 128, 256);
       const uint64_t kx_desc = smem_desc_noswz(sbase + kOffExtra + kExtraBytes, 128, 256);
       auto qk = [&](int j) {
         issue_qk(tmem + t * 128, q_desc, k_desc + stage_off(j), qx_desc,
-                 kx_desc + static_cast<uint64_t>(((j - p0) % kStages) * (kExtraBytes >> 4)), in_product ? 1u : 0u, idesc_qk, bar(kBarS + t));
+                 kx_desc + static_cast<uint64_t>((j % kStages) * (kExtraBytes >> 4)), in_product ? 1u : 0u, idesc_qk, bar(kBarS + t));
       };
       bool ok = true;
       // tiles that only the other query tile reads are released as they come
-      for (int j = p0; j < ja && ok; ++j) {
+      for (int j = 0; j < ja && ok; ++j) {
         ok = full(j);
-        if (ok && lane == 0) mbar_arrive(bar(kBarEmpty + (j - p0) % kStages));
+        if (ok && lane == 0) mbar_arrive(bar(kBarEmpty + j % kStages));
       }
       if (ok && ja < jb) {
         ok = wait_all(kBarQ, 0) && full(ja);
@@ -499,18 +574,27 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (!ok) break;
         tc_fence_after();
         issue_pv(tmem + kTmemO + t * kHeadDim, tmem + kTmemP + t * kHeadDim, v_desc + stage_off(j), idesc_pv, n > 0 ? 1u : 0u,
-                 bar(kBarO + t), bar(kBarEmpty + (j - p0) % kStages));
+                 bar(kBarO + t), bar(kBarEmpty + j % kStages));
       }
-      for (int j = jb; j < p1 && ok; ++j) {
+      for (int j = jb; j < n_tiles && ok; ++j) {
         ok = full(j);
-        if (ok && lane == 0) mbar_arrive(bar(kBarEmpty + (j - p0) % kStages));
+        if (ok && lane == 0) mbar_arrive(bar(kBarEmpty + j % kStages));
       }
     } else if (warp == kWarpKeys) {
       // ------------------------------- per-key bias and position -------------------------------
-      const float inv = kLog2E / a.scale;  // bias / scale: a.scale = scale * log2(e) without a cap
+      const float inv = 1.f / a.scale;  // a.scale = scale * log2(e) without a cap
       bool ok = true;
-      for (int j = p0; per_key && j < p1 && ok; ++j) {
-        const int n = j - p0, st = n % kStages;
+      auto clear_tail = [&] {  // whole rows, so the swizzle inside a row does not matter
+        const int st = tail % kStages;
+        ok = __all_sync(0xffffffffu, mbar_wait(bar(kBarFull + st), (tail / kStages) & 1, a.err));
+        uint4* v = reinterpret_cast<uint4*>(smem + kOffStage + (2 * st + 1) * kTileBytes);
+        for (int x = (s.keys & (kBN - 1)) * 8 + lane; ok && x < kBN * 8; x += 32) v[x] = make_uint4(0u, 0u, 0u, 0u);
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0 && ok) mbar_arrive(bar(kBarTail));
+      };
+      for (int n = 0; per_key && n < n_tiles && ok; ++n) {
+        const int j = tile_of(n), st = n % kStages, side = side_of(j);
         float b[4], kp[4];
 #pragma unroll
         for (int u = 0; u < 4; ++u) {
@@ -525,7 +609,7 @@ __global__ void __launch_bounds__(kThreads, 1)
               at = (static_cast<long long>(id) << a.page_shift) + (key & ((1 << a.page_shift) - 1));
             }
             if (a.bias != nullptr && there) b[u] = __ldg(a.bias + at);
-            if (a.slope != nullptr)
+            if (down)
               kp[u] = !kPaged && a.kpos != nullptr ? __ldg(a.kpos + s.batch * a.kpos_sb + key) : static_cast<float>(key);
           }
         }
@@ -535,8 +619,10 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
         for (int u = 0; u < 4; ++u) {
           const int k = u * 32 + lane;
+          const float away = side > 0 ? slope * static_cast<float>(k - (kBN - 1)) : side < 0 ? -slope * static_cast<float>(k) : 0.f;
+          if (down) dst[kBN + k] = kp[u];
           if constexpr (in_product) {
-            float x = b[u] * inv, mid = 0.f, lo = 0.f;
+            float x = fmaf(b[u], kLog2E, away) * inv, mid = 0.f, lo = 0.f;
             if (fabsf(x) <= kMostBias<T>) {
               const float hi = to_f32<T>(from_f32<T>(x));
               mid = to_f32<T>(from_f32<T>(x - hi));
@@ -548,24 +634,15 @@ __global__ void __launch_bounds__(kThreads, 1)
             *reinterpret_cast<uint2*>(smem + kOffExtra + (1 + st) * kExtraBytes + (k >> 3) * 256 + (k & 7) * 16) =
                 make_uint2(pack2<T>(x, mid), pack2<T>(lo, 0.f));
           } else {
-            dst[k] = bias_log2(b[u]);
-            dst[kBN + k] = kp[u];
+            dst[k] = bias_log2(b[u]) + away;
           }
         }
         if constexpr (in_product) fence_proxy_async_smem();
         __syncwarp();
         if (lane == 0) mbar_arrive(bar(kBarFull + st));
+        if (kPaged && n == tail) clear_tail();
       }
-      if (kPaged && tail >= 0 && ok) {
-        const int n = tail - p0, st = n % kStages;
-        ok = __all_sync(0xffffffffu, mbar_wait(bar(kBarFull + st), (n / kStages) & 1, a.err));
-        // whole rows, so the swizzle inside a row does not matter
-        uint4* v = reinterpret_cast<uint4*>(smem + kOffStage + (2 * st + 1) * kTileBytes);
-        for (int x = (s.keys & (kBN - 1)) * 8 + lane; ok && x < kBN * 8; x += 32) v[x] = make_uint4(0u, 0u, 0u, 0u);
-        fence_proxy_async_smem();
-        __syncwarp();
-        if (lane == 0 && ok) mbar_arrive(bar(kBarTail));
-      }
+      if (kPaged && !per_key && tail >= 0) clear_tail();
     }
   } else {
     // ------------------------------- softmax -------------------------------
@@ -576,25 +653,27 @@ __global__ void __launch_bounds__(kThreads, 1)
     const uint32_t p_addr = tmem + lane_off + kTmemP + t * kHeadDim;
     const uint32_t o_addr = tmem + lane_off + kTmemO + t * kHeadDim;
     const int i = row_first + t * kBM + row;  // token of the sequence
-    const float slope = kForm == 2 && a.slope != nullptr ? __ldg(a.slope + head) * kLog2E : 0.f;
-    const float pos = kForm == 2 && a.slope != nullptr && valid ? row_position<kPaged>(a, s, i) : 0.f;
+    const float pos = by_side ? static_cast<float>(pos_first + t * kBM + row) : down && valid ? row_position<kPaged>(a, s, i) : 0.f;
     // keys that every row of the warp sees
     const int all_lo = __reduce_max_sync(0xffffffffu, valid ? be.x : 0);
     const int all_hi = __reduce_min_sync(0xffffffffu, valid ? be.y : 0x7fffffff);
-    const int ja = t == 0 ? j0[0] : j0[1], jb = t == 0 ? j1[0] : j1[1];
+    const int ja = t == 0 ? ua[0] : ua[1], jb = t == 0 ? ub[0] : ub[1];
     float m_run = -INFINITY, l_run = 0.f;  // the running maximum is a whole number, so that a rescaling is exact
+    int rest = 1, back = 0;  // tiles until the next try at once: not the first, whose maximum is unknown, and more after each miss
     bool ok = true;
     auto wait_for = [&](int b, int parity) {
       if (ok) ok = mbar_wait(bar(b), static_cast<uint32_t>(parity), a.err);
     };
 
 #pragma unroll 1
-    for (int j = ja; j < jb; ++j) {
-      const int n = j - ja, st = (j - p0) % kStages;
+    for (int u = ja; u < jb; ++u) {
+      const int n = u - ja, st = u % kStages, j = tile_of(u);
+      const int side = side_of(j);
+      const bool apart = down && side == 0;
       {
         // the scores and, for the softmax, the tile's keys, looked at together
-        const uint32_t ps = n & 1, pf = ((j - p0) / kStages) & 1;
-        const bool wait_keys = kForm == 2 && per_key;
+        const uint32_t ps = n & 1, pf = (u / kStages) & 1;
+        const bool wait_keys = kForm == 2 || apart;
         const bool s_there = mbar_try_wait(bar(kBarS + t), ps), keys_there = !wait_keys || mbar_try_wait(bar(kBarFull + st), pf);
         if (!s_there) wait_for(kBarS + t, ps);
         if (!keys_there) wait_for(kBarFull + st, pf);
@@ -603,71 +682,100 @@ __global__ void __launch_bounds__(kThreads, 1)
       tc_fence_after();
       const float* keys = reinterpret_cast<const float*>(smem + kOffKeys) + st * 2 * kBN;
       const int key0 = j * kBN;
-      uint32_t p[kBN / 2];
-      float alpha = 1.f;  // what O is to be multiplied by
-      bool need;
-      {
-        uint32_t r[kHalf];
-        tmem_ld32x32b_x32_nowait(s_addr, *reinterpret_cast<uint32_t(*)[32]>(&r[0]));
-        tmem_ld32x32b_x32_nowait(s_addr + 32, *reinterpret_cast<uint32_t(*)[32]>(&r[32]));
-        tmem_wait_ld();
-        reg_fence32(*reinterpret_cast<uint32_t(*)[32]>(&r[0]));
-        reg_fence32(*reinterpret_cast<uint32_t(*)[32]>(&r[32]));
-        const float mul = form_scores<kForm == 2>(r, a, poly, keys, slope, pos, be.x - key0, be.y - key0, key0 < all_lo || key0 + kHalf > all_hi);
-        const float m_new = max_of(r) * mul;
-        const bool grow = m_new > m_run + kRescale;
-        need = __any_sync(0xffffffffu, grow);
-        if (need) {
-          const float m_tgt = grow ? ceilf(m_new) : m_run;
-          alpha = grow ? ex2_approx(m_run - m_tgt) : 1.f;
-          l_run *= alpha;
-          m_run = m_tgt;
-        }
-        l_run += probabilities<T>(r, mul, m_run, p);
-      }
-      {
-        uint32_t r[kHalf];
-        tmem_ld32x32b_x32_nowait(s_addr + kHalf, *reinterpret_cast<uint32_t(*)[32]>(&r[0]));
-        tmem_ld32x32b_x32_nowait(s_addr + kHalf + 32, *reinterpret_cast<uint32_t(*)[32]>(&r[32]));
-        tmem_wait_ld();
-        reg_fence32(*reinterpret_cast<uint32_t(*)[32]>(&r[0]));
-        reg_fence32(*reinterpret_cast<uint32_t(*)[32]>(&r[32]));
-        tc_fence_before();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(bar(kBarSFree + t));
-        const float mul = form_scores<kForm == 2>(r, a, poly, keys + kHalf, slope, pos, be.x - key0 - kHalf, be.y - key0 - kHalf,
-                                             key0 + kHalf < all_lo || key0 + kBN > all_hi);
-        const float m_new = max_of(r) * mul;
-        const bool grow = m_new > m_run + kRescale;
-        if (__any_sync(0xffffffffu, grow)) {  // the first half's probabilities are rescaled too, by a power of two
-          need = true;
-          const float m_tgt = grow ? ceilf(m_new) : m_run;
-          const float f = grow ? ex2_approx(m_run - m_tgt) : 1.f;
-          alpha *= f;
-          l_run *= f;
-          m_run = m_tgt;
+      // what the row's own distance adds to every score of the tile
+      const float add = side == 0 ? 0.f : -slope * fabsf(pos - static_cast<float>(side > 0 ? key0 + kBN - 1 : key0));
+      uint32_t r[kPart];
+      auto load = [&](int h) {
 #pragma unroll
-          for (int c = 0; c < kHalf / 2; ++c) p[c] = scale2<T>(p[c], f);
+        for (int c = 0; c < kPart; c += 32)
+          tmem_ld32x32b_x32_nowait(s_addr + h * kPart + c, *reinterpret_cast<uint32_t(*)[32]>(&r[c]));
+        tmem_wait_ld();
+#pragma unroll
+        for (int c = 0; c < kPart; c += 32) reg_fence32(*reinterpret_cast<uint32_t(*)[32]>(&r[c]));
+        if (h == kParts - 1) {
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(bar(kBarSFree + t));
         }
-        l_run += probabilities<T>(r, mul, m_run, p + kHalf / 2);
-      }
-      if (n > 0) {
-        wait_for(kBarO + t, (n - 1) & 1);  // PV(n - 1) has read P, and O is at rest
+      };
+      auto o_at_rest = [&] {  // PV(n - 1) has read P, and O is at rest
+        if (n == 0) return;
+        wait_for(kBarO + t, (n - 1) & 1);
         __syncwarp();
         tc_fence_after();
-        if (need) {
-#pragma unroll 1
-          for (int c = 0; c < kHeadDim; c += 16) {
-            uint32_t o[16];
-            tmem_ld32x32b_x16(o_addr + c, o);
+      };
+      auto store = [&](int h, const uint32_t (&p)[kPart / 2]) {
+        if constexpr (kPart == 64) tmem_st32x32b_x32(p_addr + h * 32, *reinterpret_cast<const uint32_t(*)[32]>(&p[0]));
+        else tmem_st32x32b_x16(p_addr + h * 16, *reinterpret_cast<const uint32_t(*)[16]>(&p[0]));
+      };
+      int h = 0;           // parts of the tile that are done
+      bool loaded = false;  // part h is in r
+      if (!apart && key0 >= all_lo && key0 + kBN <= all_hi && --rest < 0) {
 #pragma unroll
-            for (int e = 0; e < 16; ++e) o[e] = f2u(u2f(o[e]) * alpha);
-            tmem_st32x32b_x16(o_addr + c, o);
+        for (int g = 0; g < kParts; ++g) {
+          if (g != h) continue;  // an earlier part missed
+          load(g);
+          uint32_t p[kPart / 2];
+          float sum;
+          const bool none = m_run == -INFINITY;
+          if (__all_sync(0xffffffffu, probabilities_at_once<T, kForm == 2>(r, a, poly, keys + g * kPart, none ? add : add - m_run,
+                                                                           none ? -INFINITY : kRescale, p, sum))) {
+            l_run += sum;
+            if (g == 0) o_at_rest();
+            store(g, p);
+            h = g + 1;
+          } else {
+            loaded = true;
+            break;
           }
         }
+        back = h == kParts ? 0 : min(2 * back + 1, 15);
+        rest = h == kParts ? 0 : back >> 1;
       }
-      tmem_st32x32b_x32(p_addr, *reinterpret_cast<const uint32_t(*)[32]>(&p[0]));
-      tmem_st32x32b_x32(p_addr + 32, *reinterpret_cast<const uint32_t(*)[32]>(&p[32]));
+#pragma unroll 1
+      for (; h < kParts; ++h) {
+        if (!loaded) load(h);
+        loaded = false;
+        const int first = key0 + h * kPart;
+        const float mul = form_scores<kForm == 2>(r, a, poly, keys + h * kPart, apart, slope, pos, be.x - first, be.y - first,
+                                                  first < all_lo || first + kPart > all_hi);
+        const float m_new = fmaf(max_of(r), mul, add);
+        const bool grow = m_new > m_run + kRescale;
+        const bool need = __any_sync(0xffffffffu, grow);
+        float f = 1.f;  // what O, and the probabilities of the parts before, are to be multiplied by
+        if (need) {
+          const float m_tgt = grow ? ceilf(m_new) + kMargin : m_run;
+          f = grow ? ex2_approx(m_run - m_tgt) : 1.f;
+          l_run *= f;
+          m_run = m_tgt;
+        }
+        uint32_t p[kPart / 2];
+        l_run += probabilities<T>(r, mul, add - (m_run == -INFINITY ? 0.f : m_run), p);
+        if (h == 0) o_at_rest();
+        if (need) {
+          if (n > 0) {
+#pragma unroll 1
+            for (int c = 0; c < kHeadDim; c += 16) {
+              uint32_t o[16];
+              tmem_ld32x32b_x16(o_addr + c, o);
+#pragma unroll
+              for (int e = 0; e < 16; ++e) o[e] = f2u(u2f(o[e]) * f);
+              tmem_st32x32b_x16(o_addr + c, o);
+            }
+          }
+          // by a power of two, so exactly
+#pragma unroll 1
+          for (int c = 0; c < h * (kPart / 2); c += 16) {
+            uint32_t o[16];
+            tmem_wait_st();
+            tmem_ld32x32b_x16(p_addr + c, o);
+#pragma unroll
+            for (int e = 0; e < 16; ++e) o[e] = scale2<T>(o[e], f);
+            tmem_st32x32b_x16(p_addr + c, o);
+          }
+        }
+        store(h, p);
+      }
       tmem_wait_st();
       tc_fence_before();
       __syncwarp();
@@ -701,7 +809,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     bool again = false;
     // rows for exact_row: not finite, or only keys whose bias did not fit
     auto redo = [&](bool not_finite) {
-      return not_finite || (in_product && be.y > be.x && (l_run == 0.f || m_run < -0.5f * kMostBias<T> * a.scale));
+      return not_finite || (in_product && (kForm == 1 || a.bias != nullptr || slope * (kBN - 1) > kMostBias<T> * a.scale) && be.y > be.x && (l_run == 0.f || m_run < -0.5f * kMostBias<T> * a.scale));
     };
     if (split > 1) {
       // columns of four, rows side by side: [16][256] float4, so that a warp's stores and loads are whole lines
@@ -810,7 +918,7 @@ int launch_form(const AttnView& a, const CUtensorMap& tq, const CUtensorMap& tk,
     if (dev >= 0 && dev < 64) ready[dev].store(true, std::memory_order_release);
   }
   CapPoly poly{};
-  if (kForm == 2 && a.cap != 0.f) {
+  if (kForm == 2) {
     auto twice = [](double x) {
       const float f = static_cast<float>(x);
       uint32_t u;
@@ -837,7 +945,8 @@ int launch_form(const AttnView& a, const CUtensorMap& tq, const CUtensorMap& tk,
 template <typename T, bool kPaged>
 int launch(const AttnView& a, const CUtensorMap& tq, const CUtensorMap& tk, const CUtensorMap& tv, const TileSplit& w, long long grid,
            cudaStream_t st) {
-  if (a.cap != 0.f || a.slope != nullptr) return launch_form<T, kPaged, 2>(a, tq, tk, tv, w, grid, st);
+  if (a.cap != 0.f) return launch_form<T, kPaged, 2>(a, tq, tk, tv, w, grid, st);
+  if (a.slope != nullptr) return launch_form<T, kPaged, 3>(a, tq, tk, tv, w, grid, st);
   return a.bias != nullptr ? launch_form<T, kPaged, 1>(a, tq, tk, tv, w, grid, st) : launch_form<T, kPaged, 0>(a, tq, tk, tv, w, grid, st);
 }
 

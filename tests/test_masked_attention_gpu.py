@@ -297,3 +297,34 @@ def test_refusals_on_the_gpu(pkg, cuda_device):
         pkg.masked_attention(q, q, q, torch.zeros(4))
     with pytest.raises(ValueError, match="out must"):
         pkg.masked_attention(q, q, q, out=torch.empty(1, 2, 4, 65, device=cuda_device, dtype=torch.bfloat16)[..., :64])
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+@pytest.mark.parametrize("softcap", [None, 4.0])
+@pytest.mark.parametrize("mask", [None, dict(step=1), dict(step=200, window=500)])
+def test_distance_over_whole_tiles(pkg, oracle, cuda_device, dtype, softcap, mask):
+    """Tiles whose keys all lie before, behind or among the rows' positions, flat to steep slopes and one that grows with
+    the distance, with a bias that hides keys and one that nearly does."""
+    slope = np.array([0.0, 1e-4, 0.02, 0.7, 3.0, 40.0, -0.01, 0.2], np.float32)
+    rng, q, k, v = make(31, 1, 8, 4, 700, 1100, dtype, oracle, q_scale=1.0)
+    bias = np.log(rng.integers(1, 9, 1100)).astype(np.float32)
+    bias[[3, 500, 1099]] = -np.inf
+    bias[[4, 501, 1098]] = np.finfo(np.float32).min
+    ranges = None if mask is None else to_np(pkg.attention_ranges(700, 1100, **mask)).astype(np.int32)
+    for b in (bias, None):
+        run(pkg, oracle, cuda_device, dtype, q, k, v, b, ranges, slope=slope, softcap=softcap)
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+@pytest.mark.parametrize("softcap", [None, 3.0, 60.0])
+@pytest.mark.parametrize("growth", [0.02, -0.02, 0.3])
+def test_maxima_that_keep_growing(pkg, oracle, cuda_device, dtype, softcap, growth):
+    """Scores that rise (or fall) along the keys by far more than the running maximum leaves room for, in steps of one row or
+    of all, so that parts of a tile, the first or the last, have to be taken again."""
+    rng, q, k, v = make(32, 1, 2, 2, 256, 1000, dtype, oracle, q_scale=1.0)
+    lift = np.arange(1000, dtype=np.float32) * growth
+    q[..., 0], k[..., 0] = 8.0, oracle.round_to(lift % 50 if growth == 0.3 else lift, dtype)
+    q[:, :, 5::7, 0] = 0.0  # rows whose scores do not rise
+    run(pkg, oracle, cuda_device, dtype, q, k, v, softcap=softcap)
+    bias = oracle.round_to(rng.standard_normal(1000).astype(np.float32) * 9, "f32")
+    run(pkg, oracle, cuda_device, dtype, q, k, v, bias, softcap=softcap)

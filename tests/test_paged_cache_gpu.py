@@ -383,3 +383,27 @@ def test_refusals_on_the_gpu(pkg, cuda_device):
         f(z(1, 2, 64), cache, [0], [0, 1], distance_slope=z(3))
     with pytest.raises(RuntimeError, match="no backward"):
         f(z(1, 2, 64).requires_grad_(), cache, [0], [0, 1])
+
+
+@pytest.mark.parametrize("causal", [True, False])
+@pytest.mark.parametrize("softcap", [None, 5.0])
+def test_paged_distance_over_whole_tiles(pkg, oracle, cuda_device, causal, softcap):
+    """Chunks longer than a query tile over a past whose tiles are taken last to first, the last of them filled in part."""
+    rng = np.random.default_rng(33)
+    cache, ref = pair(pkg, oracle, cuda_device, slots=2, pages=120, max_pages=60, page=32, heads=2)
+    append(cache, ref, cuda_device, "bf16", rng, oracle, [0, 1], [1203, 650])
+    append(cache, ref, cuda_device, "bf16", rng, oracle, [0, 1], [290, 150])
+    q = oracle.round_to(rng.standard_normal((440, 4, 64)).astype(np.float32), "bf16")
+    slope = np.array([0.003, 0.5, 2.0, 0.0], np.float32)
+    out = pkg.paged_attention(torch.from_numpy(q).to(cuda_device, torch.bfloat16), cache, [0, 1], [0, 290, 440], causal=causal,
+                              softcap=softcap, distance_slope=torch.from_numpy(slope).to(cuda_device))
+    for s, (a, b) in enumerate(((0, 290), (290, 440))):
+        L, n = ref.length[s], b - a
+        rows = [ref.held[s][j // 32] * 32 + j % 32 for j in range(L)]
+        k, v, m = (t.reshape(-1, *t.shape[2:])[rows] for t in (ref.k, ref.v, ref.mass))
+        seen = np.array([[0, L - n + i + 1 if causal else L] for i in range(n)])
+        want, bound = oracle.streaming.masked_attention(q[a:b].transpose(1, 0, 2)[None], k.transpose(1, 0, 2)[None], v.transpose(1, 0, 2)[None],
+                                                        m, seen, softcap=softcap, slope=slope, dtype="bf16")
+        off = np.abs(to_np(out[a:b]).transpose(1, 0, 2) - want[0]) - bound[0]
+        assert off.max() <= 0, off.max()
+    assert pkg.device_error_flags() == 0
