@@ -107,9 +107,12 @@ __global__ void __launch_bounds__(kBook, 1)
   }
   auto first_mention = [&](int i, int slot) {
     if (n > kFewSlots) return w.claim[slot] == i;
-    for (int k = 0; k < i; ++k)
-      if (slots[k] == slot) return false;
-    return true;
+    // as many steps for every lane: lanes that left the loop one by one would make the loads below one by one (36 -> 9 us for
+    // 64 sequences)
+    bool before = false;
+#pragma unroll 8
+    for (int k = 0; k < n; ++k) before |= k < i && slots[k] == slot;
+    return !before;
   };
   long long needs = 0;
   for (int base = 0; base < n; base += kBook) {
