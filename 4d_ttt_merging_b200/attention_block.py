@@ -44,7 +44,8 @@ class AttentionMask:
     """What a block's rows see and how their scores change, over the tokens of the clip (``attention_ranges`` makes the
     intervals, ``masked_attention`` says what the fields do).  With a token plan a merged token stands at the place of the
     token that it keeps: it is seen where that one is, and distances are those of the kept tokens.  (What a kept token
-    pooled from others goes with it.)  The plan's kept tokens must ascend, as the planners make them."""
+    pooled from others goes with it.)  The plan's kept tokens must ascend, as the planners make them.  Inference only: a masked
+    call refuses inputs that require a gradient while gradients are recorded."""
 
     key_range: torch.Tensor | None = None       # int32 [N, 2] or [B, N, 2]
     softcap: float | None = None

@@ -61,11 +61,13 @@ def _rows(t: torch.Tensor) -> torch.Tensor:
     return t.clone(memory_format=torch.contiguous_format)
 
 
-def _check_out(q: torch.Tensor, out: torch.Tensor) -> None:
+def _check_out(q: torch.Tensor, out: torch.Tensor, *inputs: torch.Tensor) -> None:
     if out.shape != q.shape or out.dtype != q.dtype or not _tma_ready(out):
         raise ValueError("out must have q's shape and dtype, a unit channel stride and 16-byte aligned rows")
     if any(s == 0 and n > 1 for s, n in zip(out.stride(), out.shape)):
         raise ValueError("out must not be a broadcast tensor")
+    if out.numel() and any(out.data_ptr() == t.data_ptr() for t in (q, *inputs)):
+        raise ValueError("out must not share memory with the inputs")
 
 
 def _scratch(size: int, device: torch.device) -> torch.Tensor | None:
@@ -150,7 +152,7 @@ def masked_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, log_key_
     rounded to q's type as in ``mass_bias_attention``).  ``key_range`` int32 [Nq, 2] or [B, Nq, 2]: the row sees keys
     [begin, end) (``attention_ranges`` makes them); None: all.  A row without keys gives zeros; what hidden
     keys hold never reaches a row.  ``distance_slope`` [H] with positions [Nq] / [Nk] (or per batch entry), by default
-    token indices with the queries last.  Returns [B, H, Nq, 64] as a view of a token-major buffer, or writes ``out``."""
+    token indices with the queries last.  Returns [B, H, Nq, 64] as a view of a token-major buffer, or writes ``out``, which must not overlap the inputs."""
     if q.ndim != 4 or k.ndim != 4 or v.ndim != 4:
         raise ValueError("q, k and v must be [batch, heads, tokens, channels]")
     B, H, Nq, D = q.shape
@@ -171,7 +173,7 @@ def masked_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, log_key_
     if key_range is not None and (key_range.dtype != torch.int32 or key_range.shape not in ((Nq, 2), (B, Nq, 2))):
         raise ValueError(f"key_range must be int32 [{Nq}, 2] or [{B}, {Nq}, 2]")
     if out is not None:
-        _check_out(q, out)
+        _check_out(q, out, k, v)
     C.require_cuda(q, "masked_attention")
     _same_device("masked_attention", q.device, k, v, log_key_mass, key_range, distance_slope, query_position, key_position, out)
     _refuse_gradients("masked_attention", q, k, v, log_key_mass, distance_slope, query_position, key_position, out)
@@ -251,6 +253,9 @@ class PagedCache:
         # the fields stay what they are, so what every call needs of them is worked out once
         self.__dict__.update(_device=k.device, _heads=heads, _dtype=dtype, _handle=C.CacheHandle(
             *(C.ptr(t) for t in (k, self.v, self.log_mass, *ints)), pages, page, heads, *self.table.shape))
+
+    def __reduce__(self):  # copies and pickles carry the tensors, not the addresses
+        return type(self), (self.k, self.v, self.log_mass, self.table, self.length, self.references)
 
     @classmethod
     def empty(cls, slots: int, pages: int, max_pages: int, *, page_size: int = 64, heads: int = 16, dtype=torch.bfloat16,
@@ -352,7 +357,7 @@ def paged_attention(q: torch.Tensor, cache: PagedCache, sequence, offsets, *, ca
     already (``PagedCache.append``); H is a multiple of the cache's heads.  A row sees the keys up to its own (``causal``) or
     all of its slot, or the keys [begin, end) of ``key_range`` int32 [rows, 2] (frames in causal order).  The cache's log-masses
     are added to the scores; softcap, distance_slope and scale as in ``masked_attention``, positions are token indices.
-    Returns [rows, H, 64] or writes ``out``; rows outside every chunk are not written."""
+    Returns [rows, H, 64] or writes ``out`` (apart from q); rows outside every chunk are not written."""
     if q.ndim != 3 or q.shape[-1] != 64:
         raise ValueError("q must be [rows, heads, 64]")
     rows, H, D = q.shape

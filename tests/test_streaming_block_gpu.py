@@ -239,3 +239,21 @@ def test_recorded_stream_step(pkg, oracle, cuda_device):
     for a, b in ((cache.k, other.k), (cache.v, other.v), (cache.table, other.table), (cache.references, other.references)):
         assert torch.equal(a[:15], b[:15])
     assert pkg.device_error_flags() == 0
+
+
+def test_copies_of_a_cache(pkg, oracle, cuda_device):
+    """A deep copy owns its pages: both go on by themselves."""
+    rng = np.random.default_rng(9)
+    cache = pkg.PagedCache.empty(2, 6, 3, page_size=16, heads=HEADS, device=cuda_device)
+    t = lambda n: torch.from_numpy(rng.standard_normal((n, HEADS, 64)).astype(np.float32)).to(cuda_device, torch.bfloat16)  # noqa: E731
+    k = t(20)
+    cache.append([0], [0, 20], k, k)
+    other = __import__("copy").deepcopy(cache)
+    cache.free([0])
+    cache.append([1], [0, 40], t(40), t(40))
+    q = t(1)
+    ref, bound = attend(oracle, to_np(q), to_np(k), to_np(k), None, "bf16")
+    close(pkg.paged_attention(q, other, [0], [0, 1]), ref, bound)
+    assert other.length.tolist() == [20, 0] and cache.length.tolist() == [0, 40] and pkg.device_error_flags() == 0
+    with pytest.raises(AttributeError):
+        cache.k = other.k

@@ -73,3 +73,7 @@ def test_output_refusals(pkg):
     q = torch.zeros(1, 4, 3, 64)
     with pytest.raises(ValueError, match="broadcast"):
         pkg.masked_attention(q, q, q, out=torch.zeros(1, 1, 1, 64).expand(1, 4, 3, 64))
+    for i in range(3):
+        x = [torch.zeros(1, 4, 3, 64) for _ in range(3)]
+        with pytest.raises(ValueError, match="share memory"):
+            pkg.masked_attention(*x, out=x[i])
