@@ -30,11 +30,12 @@ __all__ = ["PagedCache", "attention_ranges", "masked_attention", "paged_attentio
 _PAGES = (16, 32, 64, 128)
 _Two = ctypes.c_int64 * 2
 _HERE = contextlib.nullcontext()
+_current_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)  # without the check that CUDA is up
 
 
 def _on(device: torch.device):
     """The device made current for a call, where it is not already."""
-    return _HERE if torch.cuda.current_device() == device.index else torch.cuda.device(device)
+    return _HERE if _current_device() == device.index else torch.cuda.device(device)
 
 
 def _refuse_gradients(what: str, *tensors) -> None:
@@ -53,11 +54,14 @@ def _same_device(what: str, device: torch.device, *tensors) -> None:
 def _rows(t: torch.Tensor) -> torch.Tensor:
     """``t``, or a packed copy where the kernels cannot read it: a channel stride, rows that are not 16-byte aligned (a
     packed tensor at an odd offset too), broadcast dimensions."""
-    if t.is_contiguous():
-        if t.data_ptr() % 16 == 0:
+    if t.data_ptr() % 16 == 0:
+        if t.is_contiguous():
             return t
-    elif _tma_ready(t) and 0 not in t.stride():
-        return t
+        stride, per = t.stride(), 16 // t.element_size()
+        if stride[-1] == 1 and not any([s % per or not s for s in stride[:-1]]):
+            return t
+        if _tma_ready(t) and 0 not in stride:
+            return t
     return t.clone(memory_format=torch.contiguous_format)
 
 
@@ -74,11 +78,15 @@ def _scratch(size: int, device: torch.device) -> torch.Tensor | None:
     return torch.empty(size, dtype=torch.uint8, device=device) if size else None
 
 
+def _floats(t: torch.Tensor) -> torch.Tensor:
+    return t if t.dtype is torch.float32 and t.is_contiguous() else t.to(torch.float32).contiguous()
+
+
 def _float_row(what: str, t: torch.Tensor, batch: int, n: int) -> tuple[torch.Tensor, int]:
     """A [n] or [batch, n] tensor as fp32 with its batch stride."""
     if t.shape != (n,) and t.shape != (batch, n):
         raise ValueError(f"{what} must be [{n}] or [{batch}, {n}], got {list(t.shape)}")
-    t = t.to(torch.float32).contiguous()
+    t = _floats(t)
     return t, n if t.ndim == 2 else 0
 
 
@@ -193,7 +201,7 @@ def masked_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, log_key_
             key_range = key_range.contiguous()
             mods.key_range, mods.key_range_sb = key_range.data_ptr(), 2 * Nq if key_range.ndim == 3 else 0
         if distance_slope is not None:
-            distance_slope = distance_slope.to(torch.float32).contiguous()
+            distance_slope = _floats(distance_slope)
             mods.slope = distance_slope.data_ptr()
             if query_position is not None:
                 query_position, mods.q_position_sb = _float_row("query_position", query_position, B, Nq)
@@ -250,9 +258,17 @@ class PagedCache:
             raise ValueError("cache tensors must be contiguous, the pools 16-byte aligned")
         C.require_cuda(k, "PagedCache")
         _same_device("PagedCache", k.device, *every)
-        # the fields stay what they are, so what every call needs of them is worked out once
-        self.__dict__.update(_device=k.device, _heads=heads, _dtype=dtype, _handle=C.CacheHandle(
-            *(C.ptr(t) for t in (k, self.v, self.log_mass, *ints)), pages, page, heads, *self.table.shape))
+        # The fields stay what they are, so what every call needs of them is worked out once.  The bookkeeping calls of one cache
+        # follow one another in any case, so they share one workspace.
+        handle = C.CacheHandle(*(C.ptr(t) for t in (k, self.v, self.log_mass, *ints)), pages, page, heads, *self.table.shape)
+        slots = self.table.shape[0]
+        size = max(C.lib().vb200_cache_append_workspace_size(slots, slots, pages), C.lib().vb200_cache_compact_workspace_size(pages))
+        self.__dict__.update(_device=k.device, _heads=heads, _dtype=dtype, _row=k.shape[2:], _slots=slots, _handle=handle, _sizes={},
+                             _workspace=torch.empty(size, dtype=torch.uint8, device=k.device), _workspace_bytes=size)
+
+    def _scratch(self, size: int) -> torch.Tensor:
+        """The cache's workspace, or a larger one for this call."""
+        return self._workspace if size <= self._workspace_bytes else torch.empty(size, dtype=torch.uint8, device=self._device)
 
     def __reduce__(self):  # copies and pickles carry the tensors, not the addresses
         return type(self), (self.k, self.v, self.log_mass, self.table, self.length, self.references)
@@ -287,14 +303,16 @@ class PagedCache:
         All or nothing: a pool or a table row that is too short leaves the cache as it was (error bit 2).  A slot named
         twice in one call takes its first chunk only (error bit 1).  Without log_mass the tokens have mass 1."""
         dev = self._device
-        if k.ndim != 3 or k.shape[1:] != self.k.shape[2:] or v.shape != k.shape:
+        shape = k.shape
+        if len(shape) != 3 or shape[1:] != self._row or v.shape != shape:
             raise ValueError(f"append: k and v must be [tokens, {self.heads}, 64]")
         if k.dtype != self.k.dtype or v.dtype != self.k.dtype:
             raise ValueError(f"append: the cache holds {self.k.dtype}")
-        if log_mass is not None and self.log_mass is None:
-            raise ValueError("append: the cache holds no log-masses")
-        if log_mass is not None and log_mass.shape != k.shape[:1]:
-            raise ValueError(f"append: log_mass must be [{k.shape[0]}]")
+        if log_mass is not None:
+            if self.log_mass is None:
+                raise ValueError("append: the cache holds no log-masses")
+            if log_mass.shape != shape[:1]:
+                raise ValueError(f"append: log_mass must be [{shape[0]}]")
         _same_device("append", dev, k, v, log_mass)
         _refuse_gradients("append", k, v, log_mass)
         with _on(dev):
@@ -303,13 +321,16 @@ class PagedCache:
             offsets = _int_vector("offsets", offsets, dev, n + 1)
             k, v = _rows(k), _rows(v)
             if log_mass is not None:
-                log_mass = log_mass.to(torch.float32).contiguous()
+                log_mass = _floats(log_mass)
             lib = C.lib()
-            size = lib.vb200_cache_append_workspace_size(n, self.table.shape[0], self.k.shape[0])
-            ws = _scratch(size, dev)
+            size = self._workspace_bytes  # enough for one chunk per slot
+            if n > self._slots:
+                size = lib.vb200_cache_append_workspace_size(n, self._slots, self.k.shape[0])
+            ks, vs = k.stride(), v.stride()
+            ws = self._scratch(size)
             rc = lib.vb200_cache_append(self._handle, self._dtype, sequence.data_ptr(), offsets.data_ptr(), n, k.data_ptr(),
-                                        v.data_ptr(), C.ptr(log_mass), k.shape[0], _Two(*k.stride()[:2]), _Two(*v.stride()[:2]),
-                                        C.ptr(ws), size, C.stream_of(dev))
+                                        v.data_ptr(), C.ptr(log_mass), shape[0], _Two(ks[0], ks[1]), _Two(vs[0], vs[1]),
+                                        ws.data_ptr(), size, C.stream_of(dev))
             C.check(rc, "PagedCache.append")
 
     def fork(self, source, target) -> None:
@@ -321,9 +342,9 @@ class PagedCache:
             target = _int_vector("target", target, dev, source.numel())
             lib = C.lib()
             size = lib.vb200_cache_fork_workspace_size(source.numel(), *self.table.shape)
-            ws = _scratch(size, dev)
-            rc = lib.vb200_cache_fork(self._handle, self._dtype, source.data_ptr(), target.data_ptr(), source.numel(), C.ptr(ws),
-                                      size, C.stream_of(dev))
+            ws = self._scratch(size)
+            rc = lib.vb200_cache_fork(self._handle, self._dtype, source.data_ptr(), target.data_ptr(), source.numel(),
+                                      ws.data_ptr(), size, C.stream_of(dev))
             C.check(rc, "PagedCache.fork")
 
     def free(self, sequence) -> None:
@@ -338,11 +359,9 @@ class PagedCache:
         """Moves the pages in use to the front of the pool and returns their number (int32 [1], on the device)."""
         dev = self._device
         with _on(dev):
-            lib = C.lib()
-            size = lib.vb200_cache_compact_workspace_size(self.k.shape[0])
-            ws = _scratch(size, dev)
             used = torch.empty(1, dtype=torch.int32, device=dev)
-            rc = lib.vb200_cache_compact(self._handle, self._dtype, used.data_ptr(), C.ptr(ws), size, C.stream_of(dev))
+            rc = C.lib().vb200_cache_compact(self._handle, self._dtype, used.data_ptr(), self._workspace.data_ptr(),
+                                             self._workspace_bytes, C.stream_of(dev))
             C.check(rc, "PagedCache.compact")
         return used
 
@@ -358,9 +377,10 @@ def paged_attention(q: torch.Tensor, cache: PagedCache, sequence, offsets, *, ca
     all of its slot, or the keys [begin, end) of ``key_range`` int32 [rows, 2] (frames in causal order).  The cache's log-masses
     are added to the scores; softcap, distance_slope and scale as in ``masked_attention``, positions are token indices.
     Returns [rows, H, 64] or writes ``out`` (apart from q); rows outside every chunk are not written."""
-    if q.ndim != 3 or q.shape[-1] != 64:
+    shape = q.shape
+    if len(shape) != 3 or shape[2] != 64:
         raise ValueError("q must be [rows, heads, 64]")
-    rows, H, D = q.shape
+    rows, H, D = shape
     if H == 0 or H % cache._heads:
         raise ValueError(f"{H} query heads are no multiple of the cache's {cache._heads}")
     if q.dtype != cache.k.dtype:
@@ -373,8 +393,9 @@ def paged_attention(q: torch.Tensor, cache: PagedCache, sequence, offsets, *, ca
         raise ValueError(f"key_range must be int32 [{rows}, 2]")
     if out is not None:
         _check_out(q, out)
-    C.require_cuda(q, "paged_attention")
     dev = cache._device
+    if q.device != dev:
+        C.require_cuda(q, "paged_attention")
     _same_device("paged_attention", dev, q, key_range, distance_slope, out)
     _refuse_gradients("paged_attention", q, distance_slope, out)
     with _on(dev):
@@ -389,10 +410,14 @@ def paged_attention(q: torch.Tensor, cache: PagedCache, sequence, offsets, *, ca
             key_range = key_range.contiguous()
             mods.key_range = key_range.data_ptr()
         if distance_slope is not None:
-            distance_slope = distance_slope.to(torch.float32).contiguous()
+            distance_slope = _floats(distance_slope)
             mods.slope = distance_slope.data_ptr()
         lib = C.lib()
-        size = lib.vb200_paged_attention_workspace_size(cache._dtype, rows, H, cache._handle, n)
+        size = cache._sizes.get((rows, H, n))  # a function of these and of the cache's shape
+        if size is None:
+            size = lib.vb200_paged_attention_workspace_size(cache._dtype, rows, H, cache._handle, n)
+            if len(cache._sizes) < 4096:
+                cache._sizes[rows, H, n] = size
         ws = _scratch(size, dev)
         rc = lib.vb200_paged_attention(cache._dtype, q.data_ptr(), out.data_ptr(), rows, H, D, _Two(q.stride(1), q.stride(0)),
                                        _Two(out.stride(1), out.stride(0)), cache._handle, sequence.data_ptr(), offsets.data_ptr(),
