@@ -249,8 +249,11 @@ def stream_of(device: torch.device) -> int:
     return torch.cuda.current_stream(device).cuda_stream
 
 
+_Three = _c_i64 * 3
+
+
 def strides3(t: torch.Tensor):
-    return (_c_i64 * 3)(*t.stride()[:3])
+    return _Three(*t.stride()[:3])
 
 
 def require_cuda(t: torch.Tensor, what: str) -> None:

@@ -164,8 +164,8 @@ def masked_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, log_key_
     if q.ndim != 4 or k.ndim != 4 or v.ndim != 4:
         raise ValueError("q, k and v must be [batch, heads, tokens, channels]")
     B, H, Nq, D = q.shape
-    Hkv, Nk = k.shape[1], k.shape[2]
-    if D != 64 or k.shape[-1] != 64 or v.shape[-1] != 64:
+    _, Hkv, Nk, _ = k.shape
+    if D != 64 or k.shape[3] != 64 or v.shape[3] != 64:
         raise ValueError("masked_attention supports head_dim=64 only")
     if k.shape != v.shape or k.shape[0] != B or Hkv == 0 or H % Hkv:
         raise ValueError("incompatible q/k/v shapes")
@@ -187,8 +187,8 @@ def masked_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, log_key_
     _refuse_gradients("masked_attention", q, k, v, log_key_mass, distance_slope, query_position, key_position, out)
     with _on(q.device):
         if out is None:
-            out = torch.empty((B, Nq, H, D), device=q.device, dtype=q.dtype).transpose(1, 2)
-        if out.numel() == 0:
+            out = q.new_empty(B, Nq, H, D).transpose(1, 2)
+        if B == 0 or H == 0 or Nq == 0:
             return out
         if Nk == 0:
             return out.zero_()
@@ -210,8 +210,10 @@ def masked_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, log_key_
                 key_position, mods.k_position_sb = _float_row("key_position", key_position, B, Nk)
                 mods.k_position = key_position.data_ptr()
         lib = C.lib()
-        size = lib.vb200_masked_attention_workspace_size(dt, B, H, Hkv, Nq, Nk)
-        ws = _scratch(size, q.device)
+        size, ws = 0, None
+        if dt != C.F32:  # fp32 needs none
+            size = lib.vb200_masked_attention_workspace_size(dt, B, H, Hkv, Nq, Nk)
+            ws = _scratch(size, q.device)
         rc = lib.vb200_masked_attention(dt, q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), B, H, Hkv, Nq, Nk, D,
                                         C.strides3(q), C.strides3(k), C.strides3(v), C.strides3(out), mods, C.ptr(ws), size,
                                         C.stream_of(q.device))
