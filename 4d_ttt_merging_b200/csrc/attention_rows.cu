@@ -735,14 +735,16 @@ int rows_attention(int dtype, bool paged, const AttnView& a, long long most_keys
   const int R = dtype != VB200_F32 ? (mean <= 8 ? 8 : 16) : mean <= 1 ? 1 : mean <= 2 ? 2 : 4;
   const long long blocks = paged ? total / R + a.n_seq : (total + R - 1) / R * a.B;
   const long long items = blocks * a.Hkv;
-  // Split the keys while two CTAs per SM are not filled and a piece keeps at least 256 keys; once more, for even ends
-  // of ragged sequences, while four are not and it keeps 1024 (32 sequences of 500 to 9000 keys: 175 -> 157 us; 8 of 4000,
-  // where it would not: 43 -> 57 us).  Up to 8 parts, the portable size of a cluster (16 gained 5% for one sequence of 32,928
-  // keys).
+  // Split the keys while the GPU is not filled and a piece keeps at least 256 keys.  fp32: up to two CTAs per SM.  16 bits: while
+  // the doubled split leaves room, three CTAs on two SMs; beyond that clusters no longer all fit at once (64 items of 2000 keys:
+  // 17.5 us in 4 parts, 13.3 in 2; 128 of 4000: 38 and 31).  Once more, for even ends of ragged sequences, while there are not
+  // four CTAs per SM and a piece keeps 1024 keys (32 sequences of 500 to 9000: 175 -> 157 us; with twice as many parts 122 ->
+  // 140).  Up to 8 parts, the portable size of a cluster (16 gained 5% for one sequence of 32,928 keys).
   int split = 1;
   const long long sms = sm_count_of_device();
   const long long busy = (paged ? std::max((total + R - 1) / R, seqs) : blocks) * a.Hkv;
-  while (split < 8 && ((busy * split < 2 * sms && most_keys / (2 * split) >= 256) || (busy * split < 4 * sms && most_keys / (2 * split) >= 1024)))
+  const long long fill = dtype == VB200_F32 ? 2 * sms : 3 * sms / 4 + 1;
+  while (split < 8 && ((busy * split < fill && most_keys / (2 * split) >= 256) || (busy * split < 4 * sms && most_keys / (2 * split) >= 1024)))
     split *= 2;
   if (dtype == VB200_F32) return paged ? launch_f32<true>(a, R, items, split, st) : launch_f32<false>(a, R, items, split, st);
   return dtype == VB200_BF16 ? launch_16<__nv_bfloat16>(a, paged, R > 8, items, split, st) : launch_16<__half>(a, paged, R > 8, items, split, st);
