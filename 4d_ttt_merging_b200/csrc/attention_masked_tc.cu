@@ -5,12 +5,12 @@
 //   warps 0-7    two softmax warpgroups, one per query tile, one thread per row (its TMEM lane).  A row's scores sit
 //                in one thread's registers, so the cap, the bias, the distance and the mask are applied once, and
 //                the row's maximum needs no exchange.  A tile of 128 keys is taken in parts of 64, or 32 with a cap.
-//   warp 8       TMA producer (thread 0 has asked for Q): K and V tiles of 128 keys into a ring (dense: one box; paged: a box per page,
-//                pages outside the sequence read a coordinate outside the pool and fill with zeros).
+//   warp 8       TMA producer: K and V tiles of 128 keys into a ring (dense: one box; paged: a box per page, pages outside
+//                the sequence read a coordinate outside the pool and fill with zeros).  Thread 0 has asked for Q before.
 //   warps 9, 10  one MMA stream per query tile: S(j + 1) = Q K_{j+1}^T as soon as S(j) is in registers, then
 //                O += P(j) V_j.
-//   warp 11      per key: bias and position of the tile, into the ring (only when there are any).  Without a cap the bias rides
-//                in the QK product: an extra K=16 chunk holds 1, 1, 1 in columns 0 to 2 of every query row and bias /
+//   warp 11      per key: bias, distance and position of the tile, into the ring (only when there are any).  Without a cap
+//                bias and distance ride in the QK product: an extra K=16 chunk holds 1, 1, 1 in columns 0 to 2 of every query row and bias /
 //                scale, split into three 16-bit values that add up to its 24 bits, in those of the key row (adding it
 //                in the softmax measured 20% slower).
 // TMEM: S_t at 128 t, P_t at 256 + 64 t (16-bit, the A operand of PV), O_t at 384 + 64 t.
@@ -18,8 +18,8 @@
 // Most tiles are seen whole by all rows of a warp and move no row's maximum by 2^8: their probabilities are formed straight from
 // the products, with the maximum as it is, and the tile's maximum is looked at afterwards; the first tile, tiles that the
 // mask cuts and tiles after a miss take their maximum first.  With a cap this lets its polynomial (FMA pipe) run beside the
-// exponentials: 213 -> 154 us (1024 rows, 8192 keys, 37 heads; parts of 64 keys
-// instead of 32 leave the compiler too few registers to interleave them: 186); without a cap 127 -> 117.
+// exponentials: 213 -> 154 us (1024 rows, 8192 keys, 37 heads; parts of 64 keys instead of 32 leave the compiler too few
+// registers to interleave them: 186); without a cap 127 -> 117.
 //
 // The two warps of an SM sub-partition compute their exponentials at the same time and leave the unit idle at the same time
 // (3200 clocks per 256 x 128 scores, 2100 of them in exponentials); making them take turns measured 8% slower, starting one
@@ -42,8 +42,8 @@
 // SMs at a time, 128 of 148 for clusters of 8, and one split for all blocks: a frame of 1041 rows over 33,969 keys took 405 us.)
 //
 // The running maximum is lazy: O is rescaled only when a row's maximum grows by more than 2^8; the new one is set 2^4 above it,
-// so that the next tiles seldom exceed it again (143 -> 137 us, four clips of 2058 keys).  Probabilities are
-// rounded to the value type for the PV product; sums, maxima and O are fp32.
+// so that the next tiles seldom exceed it again (4% for four clips of 2058 keys).  Probabilities are rounded to the value
+// type for the PV product; sums, maxima and O are fp32.
 #include <cudaTypedefs.h>
 
 #include <atomic>
