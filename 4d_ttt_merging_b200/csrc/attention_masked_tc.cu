@@ -23,7 +23,7 @@
 //
 // The two warps of an SM sub-partition compute their exponentials at the same time and leave the unit idle at the same time
 // (3200 clocks per 256 x 128 scores, 2100 of them in exponentials); making them take turns measured 8% slower, starting one
-// half a tile later 6%, and part of the exponentials on the FMA pipe 4%.
+// half a tile later 6%.  An eighth of the exponentials on the FMA pipe is 6% faster.
 //
 // Why this shape: a wait costs 50 to 100 clocks even when what it waits for is long there, a tile's arithmetic 510
 // (two warps per SM sub-partition, bound by the exponential unit) per 64 keys.  64-key steps with a wait for each
@@ -288,17 +288,42 @@ __device__ __forceinline__ float probabilities(const uint32_t (&r)[N], float mul
   return (a0 + a1) + (b0 + b1);
 }
 
+// 2^f on [-1/2, 1/2] as a polynomial of degree 3, fitted here for minimum maximum relative error (7.5e-5: 1/52
+// of what the probability's rounding to bf16 may take, 1/6 for fp16).
+constexpr float kE0 = 0.9999280729920136f, kE1 = 0.6932609862143841f, kE2 = 0.24261113147493726f, kE3 = 0.05517166934152859f;
+constexpr float kLeast = -125.f;  // exponents that the polynomial's integer arithmetic takes
+
+__device__ __forceinline__ float fmin3_nan(float a, float b, float c) {  // NaN if one of them is
+  float d;
+  asm("min.NaN.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
+}
+
+// 2^e for two exponents in [kLeast, 2^8] without the exponential unit: e = n + f, and n is added to the exponent bits.
+__device__ __forceinline__ void exp2_pair(uint64_t e, float& q0, float& q1) {
+  const uint64_t shift = pk2(12582912.f, 12582912.f), t = fadd2(e, shift);  // 1.5 * 2^23: n in the lowest bits
+  const uint64_t f = fadd2(e, ffma2(t, pk2(-1.f, -1.f), shift));
+  uint64_t y = ffma2(pk2(kE3, kE3), f, pk2(kE2, kE2));
+  y = ffma2(y, f, pk2(kE1, kE1));
+  y = ffma2(y, f, pk2(kE0, kE0));
+  float t0, t1, y0, y1;
+  upk2(t, t0, t1);
+  upk2(y, y0, y1);
+  q0 = u2f((f2u(t0) << 23) + f2u(y0));
+  q1 = u2f((f2u(t1) << 23) + f2u(y1));
+}
+
 // The same for keys that every row of the warp sees, straight from the products and with the maximum that the row has so far,
 // so that the exponential unit, the FMA pipe (cap, exponents, sums) and the ALU (maxima) work side by side instead of one
 // after the other.  False for a row whose maximum grows by more than 2^8 or, with a cap, whose scores leave the polynomial's
 // range: then nothing of it holds, and r is as it was.  off: what is added to a score, less the maximum; most: by how much a
-// score may exceed it.
-template <typename T, bool kCap, int N>
+// score may exceed it.  kEvery: one pair in so many takes exp2_pair; a score below its range, or NaN there, is a miss too.
+template <typename T, bool kCap, int kEvery, int N>
 __device__ __forceinline__ bool probabilities_at_once(const uint32_t (&r)[N], const AttnView& a, const CapPoly& k, const float* keys,
                                                       float off, float most, uint32_t* p, float& sum) {
   const uint64_t off2 = pk2(off, off), mul2 = pk2(a.scale, a.scale);
   uint64_t ls[2] = {pk2(0.f, 0.f), pk2(0.f, 0.f)};
-  float top[2] = {-INFINITY, -INFINITY}, far[2] = {0.f, 0.f};
+  float top[2] = {-INFINITY, -INFINITY}, far[2] = {0.f, 0.f}, low[2] = {0.f, 0.f};
 #pragma unroll
   for (int c = 0; c < N; c += 4) {
     float4 key = make_float4(0.f, 0.f, 0.f, 0.f);
@@ -321,7 +346,14 @@ __device__ __forceinline__ bool probabilities_at_once(const uint32_t (&r)[N], co
       float e0, e1;
       upk2(e, e0, e1);
       top[u] = fmax3(top[u], e0, e1);
-      const float q0 = ex2_approx(e0), q1 = ex2_approx(e1);
+      float q0, q1;
+      if (kEvery > 0 && (c / 2 + u) % kEvery == kEvery - 1) {
+        low[u] = fmin3_nan(low[u], e0, e1);
+        exp2_pair(e, q0, q1);
+      } else {
+        q0 = ex2_approx(e0);
+        q1 = ex2_approx(e1);
+      }
       ls[u] = fadd2(ls[u], pk2(q0, q1));
       p[c / 2 + u] = pack2<T>(q0, q1);
     }
@@ -330,7 +362,7 @@ __device__ __forceinline__ bool probabilities_at_once(const uint32_t (&r)[N], co
   upk2(ls[0], a0, a1);
   upk2(ls[1], b0, b1);
   sum = (a0 + a1) + (b0 + b1);
-  return fmaxf(top[0], top[1]) <= most && (!kCap || fmaxf(far[0], far[1]) * a.scale <= k.near_limit);
+  return fmaxf(top[0], top[1]) <= most && low[0] >= kLeast && low[1] >= kLeast && (!kCap || fmaxf(far[0], far[1]) * a.scale <= k.near_limit);
 }
 
 // What three 16-bit values hold of bias / scale; their product with 1 is exact in fp32.
@@ -379,6 +411,10 @@ __global__ void __launch_bounds__(kThreads, 1)
   int* key_hi = key_lo + kQT;
   // keys of a tile that are in registers at a time
   constexpr int kPart = kForm == 2 ? 32 : 64, kParts = kBN / kPart;
+  // one pair of exponentials in this many on the FMA pipe, which idles beside the exponential unit (8232 rows and keys with
+  // masses: 431 us without, 419 one in 16, 405 one in 8, 418 one in 4).  None with a cap, whose polynomial fills the pipe, or with a
+  // distance, whose scores often lie below the polynomial's range (307 -> 337 us for a frame).
+  constexpr int kEvery = kForm <= 1 ? 8 : 0;
   constexpr bool in_product = kForm == 1 || kForm == 3;
   constexpr bool per_key = kForm != 0;  // without a bias and a distance form 2's ring holds zeros
 
@@ -718,7 +754,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           uint32_t p[kPart / 2];
           float sum;
           const bool none = m_run == -INFINITY;
-          if (__all_sync(0xffffffffu, probabilities_at_once<T, kForm == 2>(r, a, poly, keys + g * kPart, none ? add : add - m_run,
+          if (__all_sync(0xffffffffu, probabilities_at_once<T, kForm == 2, kEvery>(r, a, poly, keys + g * kPart, none ? add : add - m_run,
                                                                            none ? -INFINITY : kRescale, p, sum))) {
             l_run += sum;
             if (g == 0) o_at_rest();
