@@ -328,3 +328,29 @@ def test_maxima_that_keep_growing(pkg, oracle, cuda_device, dtype, softcap, grow
     run(pkg, oracle, cuda_device, dtype, q, k, v, softcap=softcap)
     bias = oracle.round_to(rng.standard_normal(1000).astype(np.float32) * 9, "f32")
     run(pkg, oracle, cuda_device, dtype, q, k, v, bias, softcap=softcap)
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+@pytest.mark.parametrize("what", ["far below", "nan", "massless"])
+def test_keys_that_the_polynomial_does_not_take(pkg, oracle, cuda_device, dtype, what):
+    """Keys in tiles that every row sees whole, one in each place of a tile: scores far below the maximum, NaN (whose rows are
+    NaN, and only those), mass 0."""
+    rng, q, k, v = make(41, 1, 2, 1, 300, 1024, dtype, oracle, q_scale=1.0)
+    odd = 256 + 129 * np.arange(5)  # tiles 2 to 6, other places of the tile
+    odd = np.concatenate([odd + i for i in range(0, 24, 3)])
+    bias = np.zeros(1024, np.float32)
+    if what == "far below":
+        bias[odd] = -150.0
+    elif what == "massless":
+        bias[odd] = -np.inf
+    else:
+        k[0, 0, odd[::9]] = np.nan
+        ranges = np.tile(np.array([[0, 1024]], np.int32), (300, 1))
+        ranges[:7, 1] = 256  # these rows do not see them
+        out = pkg.masked_attention(*(gpu(t, cuda_device, TORCH_DTYPE[dtype]) for t in (q, k, v)), key_range=gpu(ranges, cuda_device))
+        out = to_np(out)
+        assert np.isnan(out[:, :, 7:]).all()
+        ref, bound = oracle.streaming.masked_attention(q[:, :, :7], k[:, :, :256], v[:, :, :256], dtype=dtype)
+        check(out[:, :, :7], ref, bound)
+        return
+    run(pkg, oracle, cuda_device, dtype, q, k, v, bias)
