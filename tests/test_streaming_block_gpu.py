@@ -257,3 +257,37 @@ def test_copies_of_a_cache(pkg, oracle, cuda_device):
     assert other.length.tolist() == [20, 0] and cache.length.tolist() == [0, 40] and pkg.device_error_flags() == 0
     with pytest.raises(AttributeError):
         cache.k = other.k
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+def test_hard_merged_clips_and_streams(pkg, oracle, cuda_device, dtype):
+    """A hard-merge plan has no masses: two clips under one mask (a batch), and one clip streamed."""
+    rng = np.random.default_rng(12)
+    N, kept = 2 * FRAME, 60
+    m = block(pkg, cuda_device, dtype)
+    keep = np.stack([np.sort(rng.choice(N, kept, replace=False)) for _ in range(2)])
+    inverse = rng.integers(0, kept, (2, N))
+    for b in range(2):
+        inverse[b, keep[b]] = np.arange(kept)
+    t = lambda a: torch.from_numpy(a).to(cuda_device)  # noqa: E731
+    plan = pkg.TokenPlan(t(keep), t(inverse), N)
+    one = pkg.TokenPlan(t(keep[:1]), t(inverse[:1]), N)
+    x = t(rng.standard_normal((2, N, DIM)).astype(np.float32)).to(TORCH_DTYPE[dtype])
+    ranges = pkg.attention_ranges(N, step=FRAME, device=cuda_device)
+    ab = __import__("importlib").import_module(pkg.__name__ + ".attention_block")
+    cache = pkg.PagedCache.empty(1, 10, 10, page_size=16, heads=HEADS, dtype=TORCH_DTYPE[dtype], masses=False, device=cuda_device)
+    with torch.no_grad():
+        y = m(x, plan, pkg.AttentionMask(key_range=ranges))
+        rows = ab._compact_rows(*ab._dense_rows(m.qkv_projection(x), HEADS, m.q_norm, m.k_norm), plan)
+        z = m.stream(x[:1], cache, [0], token_plan=one)
+        single = ab._compact_rows(*ab._dense_rows(m.qkv_projection(x[:1]), HEADS, m.q_norm, m.k_norm), one)
+    for b in range(2):
+        own = to_np(ranges).astype(int)[keep[b]]
+        seen = np.array([[(keep[b] < lo).sum(), (keep[b] < hi).sum()] for lo, hi in own])
+        q, k, v = (to_np(r[b]).reshape(kept, HEADS, 64) for r in rows)
+        ref, bound = attend(oracle, q, k, v, None, dtype, seen)
+        close(y[b][t(keep[b])], ref, bound)
+    q, k, v = (to_np(r[0]).reshape(kept, HEADS, 64) for r in single)
+    ref, bound = attend(oracle, q, k, v, None, dtype)
+    close(z[0][t(keep[0])], ref, bound)
+    assert cache.length.item() == kept and pkg.device_error_flags() == 0
