@@ -518,12 +518,27 @@ __global__ void __launch_bounds__(kThreads, 1)
   };
 
   // Paged: the tile whose last page the sequence fills in part.  The slots behind the last key hold anything, NaN perhaps, so
-  // warp 11 overwrites their values with zeros before the PV product reads them.  -1: none in this part.
+  // their values are overwritten with zeros before the PV product reads them: by warp 11, which takes the tiles in order, and
+  // without values per key by the producer behind its last tile.  -1: none in this part.
   int tail = -1;
   if (kPaged && (s.keys & (kBN - 1)) != 0) {
     const int j = s.keys / kBN;
     if ((j >= j0[0] && j < j1[0]) || (j >= j0[1] && j < j1[1])) tail = down ? p1 - 1 - j : j - p0;
   }
+
+  // Called by a warp that is in step with the ring: it knows that the fills of the tail's stage before the tail have landed, and
+  // no later one starts before kBarTail.  (A parity says which of two fills has landed, no more: a warp that comes to it from the
+  // start would take another tile for the tail.)  Whole rows, so the swizzle inside a row does not matter.
+  auto clear_tail = [&]() -> bool {
+    const int st = tail % kStages;
+    const bool ok = __all_sync(0xffffffffu, mbar_wait(bar(kBarFull + st), (tail / kStages) & 1, a.err));
+    uint4* v = reinterpret_cast<uint4*>(smem + kOffStage + (2 * st + 1) * kTileBytes);
+    for (int x = (s.keys & (kBN - 1)) * 8 + lane; ok && x < kBN * 8; x += 32) v[x] = make_uint4(0u, 0u, 0u, 0u);
+    fence_proxy_async_smem();
+    __syncwarp();
+    if (lane == 0 && ok) mbar_arrive(bar(kBarTail));
+    return ok;
+  };
 
   // A wait that runs out makes its role go on without waiting (or leave), so that every thread reaches the end and
   // TMEM is freed.
@@ -567,6 +582,8 @@ __global__ void __launch_bounds__(kThreads, 1)
         mbar_wait(bar(kBarQ), 0, a.err);
         for (int u = max(n - kStages, 0); u < n; ++u) mbar_wait(bar(kBarFull + u % kStages), (u / kStages) & 1, a.err);
       }
+      // tiles first to last, so the tail, where there is one, is the last that was asked for
+      if (kPaged && !per_key && ok && tail >= 0) clear_tail();
     } else if (warp < kWarpMma + kQT) {
       // ------------------------------- MMA issuer of query tile t -------------------------------
       const int t = warp - kWarpMma;
@@ -620,15 +637,6 @@ __global__ void __launch_bounds__(kThreads, 1)
       // ------------------------------- per-key bias and position -------------------------------
       const float inv = 1.f / a.scale;  // a.scale = scale * log2(e) without a cap
       bool ok = true;
-      auto clear_tail = [&] {  // whole rows, so the swizzle inside a row does not matter
-        const int st = tail % kStages;
-        ok = __all_sync(0xffffffffu, mbar_wait(bar(kBarFull + st), (tail / kStages) & 1, a.err));
-        uint4* v = reinterpret_cast<uint4*>(smem + kOffStage + (2 * st + 1) * kTileBytes);
-        for (int x = (s.keys & (kBN - 1)) * 8 + lane; ok && x < kBN * 8; x += 32) v[x] = make_uint4(0u, 0u, 0u, 0u);
-        fence_proxy_async_smem();
-        __syncwarp();
-        if (lane == 0 && ok) mbar_arrive(bar(kBarTail));
-      };
       for (int n = 0; per_key && n < n_tiles && ok; ++n) {
         const int j = tile_of(n), st = n % kStages, side = side_of(j);
         float b[4], kp[4];
@@ -676,9 +684,8 @@ __global__ void __launch_bounds__(kThreads, 1)
         if constexpr (in_product) fence_proxy_async_smem();
         __syncwarp();
         if (lane == 0) mbar_arrive(bar(kBarFull + st));
-        if (kPaged && n == tail) clear_tail();
+        if (kPaged && n == tail) ok = clear_tail();
       }
-      if (kPaged && !per_key && tail >= 0) clear_tail();
     }
   } else {
     // ------------------------------- softmax -------------------------------

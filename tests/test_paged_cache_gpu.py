@@ -407,3 +407,32 @@ def test_paged_distance_over_whole_tiles(pkg, oracle, cuda_device, causal, softc
         off = np.abs(to_np(out[a:b]).transpose(1, 0, 2) - want[0]) - bound[0]
         assert off.max() <= 0, off.max()
     assert pkg.device_error_flags() == 0
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+@pytest.mark.parametrize("causal", [True, False])
+@pytest.mark.parametrize("lengths,counts,heads,kv_heads,page", [
+    ([700, 1100], [300, 300], 37, 1, 16),    # 148 row blocks that run whole: the last, partly filled key tile is the 6th and the 9th
+    ([700, 1100], [300, 300], 37, 1, 64),
+    ([1700, 2100], [300, 300], 37, 1, 64),   # the 14th and the 17th
+    ([1700, 2100], [300, 300], 37, 1, 16),
+    ([5900], [1041], 4, 4, 16),              # 20 blocks in 7 parts each: the 7th of its part
+    ([5900], [1041], 8, 2, 64),              # 40 in 3: the 16th
+    ([9273], [1041], 4, 2, 64),              # 20 in 7: the 11th
+])
+@pytest.mark.parametrize("stale", [float("nan"), 100.0])
+def test_last_tile_without_masses(pkg, oracle, cuda_device, dtype, causal, lengths, counts, heads, kv_heads, page, stale):
+    """Long streams in a cache without masses: every value of every tile takes part, what lies behind the last key does not.
+    All values are positive, so a tile's missing values are more than the bound allows."""
+    rng = np.random.default_rng(sum(lengths) + page)
+    cache, ref = pair(pkg, oracle, cuda_device, slots=len(lengths), pages=sum(-(-n // page) for n in lengths), heads=kv_heads,
+                      max_pages=-(-max(lengths) // page) + 1, page=page, dtype=dtype, masses=False)
+    cache.k.fill_(stale), cache.v.fill_(stale)
+    n = sum(lengths)
+    k, v = (oracle.round_to(f(rng.standard_normal((n, kv_heads, 64))).astype(np.float32), dtype) for f in (np.array, np.abs))
+    off = np.concatenate([[0], np.cumsum(lengths)]).tolist()
+    order = list(range(len(lengths)))
+    t = lambda x: torch.from_numpy(x).to(cuda_device, TORCH_DTYPE[dtype])  # noqa: E731
+    cache.append(order, off, t(k), t(v))
+    assert ref.append(order, off, k, v)
+    attend(pkg, oracle, cuda_device, dtype, cache, ref, rng, order, counts, heads, causal=causal, q_scale=1.0)
