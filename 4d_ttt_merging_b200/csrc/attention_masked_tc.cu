@@ -15,7 +15,7 @@
 //                in the softmax measured 20% slower).
 // TMEM: S_t at 128 t, P_t at 256 + 64 t (16-bit, the A operand of PV), O_t at 384 + 64 t.
 //
-// Most tiles are seen whole by all rows of a warp and move no row's maximum by 2^8: their probabilities are formed straight from
+// Most tiles are seen whole by all rows of a warp and move no row's maximum by 2^kRescale: their probabilities are formed straight from
 // the products, with the maximum as it is, and the tile's maximum is looked at afterwards; the first tile, tiles that the
 // mask cuts and tiles after a miss take their maximum first.  With a cap this lets its polynomial (FMA pipe) run beside the
 // exponentials: 213 -> 154 us (1024 rows, 8192 keys, 37 heads; parts of 64 keys instead of 32 leave the compiler too few
@@ -41,9 +41,9 @@
 // does not depend on which one that is.  (Parts in a cluster, joined in distributed shared memory, need whole clusters of
 // SMs at a time, 128 of 148 for clusters of 8, and one split for all blocks: a frame of 1041 rows over 33,969 keys took 405 us.)
 //
-// The running maximum is lazy: O is rescaled only when a row's maximum grows by more than 2^8; the new one is set 2^4 above it,
-// so that the next tiles seldom exceed it again (4% for four clips of 2058 keys).  Probabilities are rounded to the value
-// type for the PV product; sums, maxima and O are fp32.
+// The running maximum is lazy: O is rescaled only when a row's maximum grows by more than 2^8 (fp16: 2^15.9); the new one is set 2^4
+// above it (fp16: 2^4 below), so that the next tiles seldom exceed it again (4% for four clips of 2058 keys).  Probabilities
+// are rounded to the value type for the PV product; sums, maxima and O are fp32.
 #include <cudaTypedefs.h>
 
 #include <atomic>
@@ -62,8 +62,14 @@ constexpr int kTileBytes = kBN * kHeadDim * 2;  // 16 KB: a Q, K or V tile
 constexpr int kSoftmaxWarps = 8;
 constexpr int kWarpProducer = 8, kWarpMma = 9, kWarpKeys = 11;
 constexpr int kThreads = 12 * 32;
-constexpr float kRescale = 8.f;  // P stays <= 2^8
-constexpr float kMargin = 4.f;   // a new maximum leaves this much room; the largest P stays >= 2^-5
+// P stays <= 2^kRescale, and a row's largest P above 2^(-kMargin - 1).  bf16 has fp32's exponents, so a margin above the maximum
+// costs no bits.  fp16 loses what falls below its smallest step 2^-24, so its P reach up to the type's largest value (65,504), and
+// the largest stays above 2^3: a key loses at most 2^-28 of the largest probability per rounding.  (Room to grow is time: 8232 rows and
+// keys with a deviation of 4 take 414 us with -3, 427 with -4, 445 with -5, 498 with -7; 427 with +4 and 2^8 as in bf16.)
+template <typename T>
+constexpr float kRescale = std::is_same<T, __half>::value ? 15.9f : 8.f;
+template <typename T>
+constexpr float kMargin = std::is_same<T, __half>::value ? -4.f : 4.f;
 
 constexpr int kOffQ = 0;
 constexpr int kOffStage = kQT * kTileBytes;
@@ -299,7 +305,7 @@ __device__ __forceinline__ float fmin3_nan(float a, float b, float c) {  // NaN 
   return d;
 }
 
-// 2^e for two exponents in [kLeast, 2^8] without the exponential unit: e = n + f, and n is added to the exponent bits.
+// 2^e for two exponents in [kLeast, kRescale] without the exponential unit: e = n + f, and n is added to the exponent bits.
 __device__ __forceinline__ void exp2_pair(uint64_t e, float& q0, float& q1) {
   const uint64_t shift = pk2(12582912.f, 12582912.f), t = fadd2(e, shift);  // 1.5 * 2^23: n in the lowest bits
   const uint64_t f = fadd2(e, ffma2(t, pk2(-1.f, -1.f), shift));
@@ -315,7 +321,7 @@ __device__ __forceinline__ void exp2_pair(uint64_t e, float& q0, float& q1) {
 
 // The same for keys that every row of the warp sees, straight from the products and with the maximum that the row has so far,
 // so that the exponential unit, the FMA pipe (cap, exponents, sums) and the ALU (maxima) work side by side instead of one
-// after the other.  False for a row whose maximum grows by more than 2^8 or, with a cap, whose scores leave the polynomial's
+// after the other.  False for a row whose maximum grows by more than 2^most or, with a cap, whose scores leave the polynomial's
 // range: then nothing of it holds, and r is as it was.  off: what is added to a score, less the maximum; most: by how much a
 // score may exceed it.  kEvery: one pair in so many takes exp2_pair; a score below its range, or NaN there, is a miss too.
 template <typename T, bool kCap, int kEvery, int N>
@@ -762,7 +768,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           float sum;
           const bool none = m_run == -INFINITY;
           if (__all_sync(0xffffffffu, probabilities_at_once<T, kForm == 2, kEvery>(r, a, poly, keys + g * kPart, none ? add : add - m_run,
-                                                                           none ? -INFINITY : kRescale, p, sum))) {
+                                                                           none ? -INFINITY : kRescale<T>, p, sum))) {
             l_run += sum;
             if (g == 0) o_at_rest();
             store(g, p);
@@ -783,11 +789,11 @@ __global__ void __launch_bounds__(kThreads, 1)
         const float mul = form_scores<kForm == 2>(r, a, poly, keys + h * kPart, apart, slope, pos, be.x - first, be.y - first,
                                                   first < all_lo || first + kPart > all_hi);
         const float m_new = fmaf(max_of(r), mul, add);
-        const bool grow = m_new > m_run + kRescale;
+        const bool grow = m_new > m_run + kRescale<T>;
         const bool need = __any_sync(0xffffffffu, grow);
         float f = 1.f;  // what O, and the probabilities of the parts before, are to be multiplied by
         if (need) {
-          const float m_tgt = grow ? ceilf(m_new) + kMargin : m_run;
+          const float m_tgt = grow ? ceilf(m_new) + kMargin<T> : m_run;
           f = grow ? ex2_approx(m_run - m_tgt) : 1.f;
           l_run *= f;
           m_run = m_tgt;
@@ -806,7 +812,7 @@ __global__ void __launch_bounds__(kThreads, 1)
               tmem_st32x32b_x16(o_addr + c, o);
             }
           }
-          // by a power of two, so exactly
+          // by a power of two: exactly, but for what fp16 holds in less than 11 bits, which rounds to its step once more
 #pragma unroll 1
           for (int c = 0; c < h * (kPart / 2); c += 16) {
             uint32_t o[16];

@@ -346,6 +346,11 @@ __device__ __forceinline__ void mma16816(float (&d)[4], const uint32_t (&a)[4], 
 }
 
 constexpr int kRing = 3;  // steps of 16 keys in a warp's ring
+constexpr float kRoom = 8.f;  // a row's maximum grows by up to 2^8 before O is rescaled
+// A new maximum has P = 2^kUp.  fp16 loses what falls below its smallest step 2^-24, so its P go up to 2^(7 + 8), near the top of
+// the type; bf16 has fp32's exponents.
+template <typename T>
+constexpr float kUp = std::is_same<T, __half>::value ? 7.f : 0.f;
 constexpr int kSide = 16 * kHeadDim * 2;  // K or V of a step: 16 rows of 128 bytes, 128-byte swizzle
 constexpr int kRowsRing = kRowWarps * kRing * 2 * kSide;
 constexpr int kRowsSmem = kRowsRing + 1024;  // slack for the alignment of the swizzle
@@ -573,15 +578,16 @@ __global__ void __launch_bounds__(kRowWarps * 32, 2) few_rows_kernel(const __gri
         mx[r] = fmaxf(mx[r], y);
       }
       // Lazy running maximum: O is rescaled when some row's grows by more than 2^8.  The lanes' own maxima tell whether one
-      // does; only then are they brought together.
-      if (__any_sync(0xffffffffu, mx[0] > m[n][0] + 8.f || mx[1] > m[n][1] + 8.f)) {
+      // does; only then are they brought together.  m: the maximum less kUp.
+      constexpr float most = kRoom + kUp<T>;
+      if (__any_sync(0xffffffffu, mx[0] > m[n][0] + most || mx[1] > m[n][1] + most)) {
 #pragma unroll
         for (int r = 0; r < 2; ++r) {
 #pragma unroll
           for (int d = 4; d < 32; d <<= 1) mx[r] = fmaxf(mx[r], __shfl_xor_sync(0xffffffffu, mx[r], d));
-          if (mx[r] > m[n][r] + 8.f) {
-            const float f = ex2_approx(m[n][r] - mx[r]);
-            m[n][r] = mx[r];
+          if (mx[r] > m[n][r] + most) {
+            const float f = ex2_approx(m[n][r] - (mx[r] - kUp<T>));
+            m[n][r] = mx[r] - kUp<T>;
             l[n][r] *= f;
 #pragma unroll
             for (int j = 0; j < 4; ++j) {

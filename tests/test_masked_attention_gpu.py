@@ -354,3 +354,38 @@ def test_keys_that_the_polynomial_does_not_take(pkg, oracle, cuda_device, dtype,
         check(out[:, :, :7], ref, bound)
         return
     run(pkg, oracle, cuda_device, dtype, q, k, v, bias)
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+@pytest.mark.parametrize("heads,queries", [(2, 300), (1, 2)])
+@pytest.mark.parametrize("top", [[0], [20000], [32927], range(5, 32928, 144)], ids=["first", "inside", "last", "many"])
+@pytest.mark.parametrize("depth", [12.0, 13.0, 14.5])
+@pytest.mark.parametrize("softcap", [None, 60.0])
+def test_small_probabilities_add_up(pkg, oracle, cuda_device, dtype, heads, queries, top, depth, softcap):
+    """Keys that stand 12 to 14.5 nats above the other ones of 32,928, which have one score, so that their probabilities round the
+    same way.  The high keys' values are 0, so the output is what the small probabilities add up to.
+
+    Tolerance, relative to the output (all values are positive): each probability and the result are rounded once, 2 * eps / 2 and 1%
+    for the second order; the exponential may be a polynomial (2^-13), and the sum that it is divided by too; scores are sums of one
+    product and zeros, at most 16 long and rounded 16 times; sums of n terms round at most n / 16 + 128 times.  Besides, fp16
+    rounds to its step 2^-24: with the largest probability kept above 2^3, each of at most four roundings takes 2^-25 / 2^3 of it
+    from a key's."""
+    n, top = 32928, list(top)
+    q, k = np.zeros((1, heads, queries, 64), np.float32), np.zeros((1, 1, n, 64), np.float32)
+    q[..., 0] = 8.0
+    k[0, 0, :, 0] = -depth
+    k[0, 0, top, 0] = 0.0
+    v = oracle.round_to((np.abs(np.random.default_rng(queries).standard_normal((1, 1, n, 64))) + 0.5).astype(np.float32), dtype)
+    v[0, 0, top] = 0.0
+    td = TORCH_DTYPE[dtype]
+    got = to_np(pkg.masked_attention(*(gpu(t, cuda_device, td) for t in (q, k, v)), softcap=softcap))
+    x = k[0, 0, :, 0].astype(np.float64)
+    x = x if softcap is None else softcap * np.tanh(x / softcap)
+    p = np.exp(x) / np.exp(x).sum()
+    want = p @ v[0, 0].astype(np.float64)
+    half, u = oracle.streaming.EPS_HALF[dtype], 2.0 ** -24
+    rel = 2.02 * half + 2 * (2.0 ** -13 + 16 * 16 * u + (n / 16 + 128) * u + (0 if softcap is None else softcap * 2.0 ** -21))
+    # the result's own smallest step: 2^-25
+    step = 4 * 2.0 ** -28 * p.max() * v[0, 0].sum(0) + 2.0 ** -25 if dtype == "f16" else 0.0
+    assert (np.abs(got - want) <= rel * want + step).all(), np.abs(got / want - 1).max()
+    assert pkg.device_error_flags() == 0
