@@ -10,7 +10,9 @@
   fp32;
 * sums over the keys round 2^-24 per addition, at most keys / 16 + 128 in a row;
 * 16-bit types round each probability (eps / 2) before the product with the values, and the result once (eps / 2);
-  fp16 also loses what falls below its smallest step 2^-24 of a probability (the largest probability of a row is at least 2^-8).
+  fp16 besides rounds to its smallest step 2^-24: the kernels keep a row's largest probability, before it is divided by the sum, above 2^3
+  and round a probability at most four times (once, and once for each time that the maximum grows while its tile is in work), so a key
+  loses at most 4 * 2^-25 / 2^3 of the row's largest, or what two roundings take of its own; the result rounds to 2^-25.
 """
 from __future__ import annotations
 
@@ -78,7 +80,7 @@ def masked_attention(q, k, v, bias=None, ranges=None, *, scale=0.125, softcap=No
             else:
                 bound[b, h] += half * np.abs(o)
             if dtype == "f16":  # absolute step of small probabilities and of small results
-                bound[b, h] += 2.0 ** -24 * (2.0 ** 8 * np.abs(np.where(see.any(0)[:, None], vz, 0.0)).sum(0, keepdims=True) + 1.0)
+                bound[b, h] += np.minimum(2 * p, 2.0 ** -26 * p.max(1, keepdims=True)) @ np.abs(vz) + 2.0 ** -25
     return out, bound
 
 

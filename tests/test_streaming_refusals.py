@@ -154,3 +154,25 @@ def test_oracle_cache_keeps_tokens(oracle):
             assert len(k) == len(want[s]) and all((x == y).all() for x, y in zip(k, want[s])) and (v == -k).all()
         count = np.bincount([p for row in c.held for p in row], minlength=20)
         assert count.tolist() == c.refs
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+def test_oracle_bound_is_narrow(oracle, dtype):
+    """Over long keys the bound stays a few roundings of the output: values that are missing from it, one tile's of 127 keys, are
+    outside."""
+    rng = np.random.default_rng(2)
+    n = 8000
+    q, k = rng.standard_normal((1, 1, 3, 64)), rng.standard_normal((1, 1, n, 64))
+    v = np.abs(rng.standard_normal((1, 1, n, 64)))
+    out, bound = oracle.streaming.masked_attention(q, k, v, dtype=dtype)
+    assert (bound < 3 * 2 * oracle.streaming.EPS_HALF[dtype] * out).all()
+    less = v.copy()
+    less[:, :, :127] = 0
+    lost, _ = oracle.streaming.masked_attention(q, k, less, dtype=dtype)
+    assert (np.abs(lost - out) > bound).all()
+    bias = np.full(n, -14.0)
+    bias[9] = 12.0
+    v[0, 0, 9] = 0  # the output is what keys 26 nats below the top add up to
+    out, bound = oracle.streaming.masked_attention(q, k, v, bias, dtype=dtype)
+    # at most two roundings of the whole, the result's step, and what the other roundings take as above
+    assert (bound <= (2 + 3 * 2 * oracle.streaming.EPS_HALF[dtype]) * out + 2.0 ** -25).all()
