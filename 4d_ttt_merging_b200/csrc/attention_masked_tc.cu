@@ -12,7 +12,8 @@
 //   warp 11      per key: bias, distance and position of the tile, into the ring (only when there are any).  Without a cap
 //                bias and distance ride in the QK product: an extra K=16 chunk holds 1, 1, 1 in columns 0 to 2 of every query row and bias /
 //                scale, split into three 16-bit values that add up to its 24 bits, in those of the key row (adding it
-//                in the softmax measured 20% slower).
+//                in the softmax measured 20% slower).  fp16, whose largest value is 65,504: 2^15 and 2^6 in columns 3 and 4 for the
+//                upper parts of larger ones.
 // TMEM: S_t at 128 t, P_t at 256 + 64 t (16-bit, the A operand of PV), O_t at 384 + 64 t.
 //
 // Most tiles are seen whole by all rows of a warp and move no row's maximum by 2^kRescale: their probabilities are formed straight from
@@ -371,9 +372,11 @@ __device__ __forceinline__ bool probabilities_at_once(const uint32_t (&r)[N], co
   return fmaxf(top[0], top[1]) <= most && low[0] >= kLeast && low[1] >= kLeast && (!kCap || fmaxf(far[0], far[1]) * a.scale <= k.near_limit);
 }
 
-// What three 16-bit values hold of bias / scale; their product with 1 is exact in fp32.
+// What the chunk's 16-bit values hold of bias / scale; their products are exact in fp32.  fp16: up to kPlainBias in columns 0 to 2,
+// beyond it 2^15 c3 + 2^6 c4 + what is left, where c3 and c4 take 11 bits each.
 template <typename T>
-constexpr float kMostBias = std::is_same<T, __nv_bfloat16>::value ? 1e30f : 60000.f;
+constexpr float kMostBias = std::is_same<T, __nv_bfloat16>::value ? 1e30f : 1.9e9f;
+constexpr float kPlainBias = 60000.f;
 
 // kForm: 0 plain scores; 1 with a bias, in the product; 2 with a cap, bias and distance in the softmax; 3 with a distance and no
 // cap, in the product like a bias.
@@ -388,6 +391,9 @@ constexpr float kMostBias = std::is_same<T, __nv_bfloat16>::value ? 1e30f : 6000
 // A bias that does not fit in the product: one below the range (the type's lowest value, say) hides its key there, as -inf
 // does, and a row that ends with no probability, or with a maximum so low that such a key might count, is computed again
 // by exact_row; one above the range, or NaN, makes its scores infinite or NaN, and exact_row computes those rows too.
+// In the rows that stay, a key that such a bias hides could count only if its q.k were half the range, and then the rounding of its
+// fp32 sum, 64 * 2^-24 of that, is 14 nats or more.  That holds from scales of 2^-8 (fp16) and 2^-76 (bf16) on; calls with smaller
+// ones go to the few-row kernel.
 template <typename T, bool kPaged, int kForm>
 __global__ void __launch_bounds__(kThreads, 1)
     masked_attention_tc_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_constant__ CUtensorMap tmap_k,
@@ -450,11 +456,11 @@ __global__ void __launch_bounds__(kThreads, 1)
     tmem_relinquish();
   }
   if constexpr (in_product) {
-    // the query rows' chunk: 1, 1, 1 in columns 0 to 2; the key rows' chunks: zero beyond column 3
-    const uint32_t one = kBF16 ? 0x3F80u : 0x3C00u;
+    // the query rows' chunk: 1, 1, 1 in columns 0 to 2, fp16 also 2^15 and 2^6; the key rows' chunks: zero beyond
+    const uint32_t one = kBF16 ? 0x3F80u : 0x3C00u, upper = kBF16 ? 0u : 0x7800u, middle = kBF16 ? 0u : 0x5400u;
     for (int x = threadIdx.x; x < (1 + kStages) * kExtraBytes / 16; x += kThreads) {
       const bool q = x < kExtraBytes / 16 && ((x >> 3) & 1) == 0;
-      *reinterpret_cast<uint4*>(smem + kOffExtra + 16 * x) = make_uint4(q ? one | one << 16 : 0u, q ? one : 0u, 0u, 0u);
+      *reinterpret_cast<uint4*>(smem + kOffExtra + 16 * x) = make_uint4(q ? one | one << 16 : 0u, q ? one | upper << 16 : 0u, q ? middle : 0u, 0u);
     }
     fence_proxy_async_smem();  // generic writes become visible to the tensor core
   }
@@ -672,8 +678,14 @@ __global__ void __launch_bounds__(kThreads, 1)
           const float away = side > 0 ? slope * static_cast<float>(k - (kBN - 1)) : side < 0 ? -slope * static_cast<float>(k) : 0.f;
           if (down) dst[kBN + k] = kp[u];
           if constexpr (in_product) {
-            float x = fmaf(b[u], kLog2E, away) * inv, mid = 0.f, lo = 0.f;
+            float x = fmaf(b[u], kLog2E, away) * inv, mid = 0.f, lo = 0.f, c3 = 0.f, c4 = 0.f;
             if (fabsf(x) <= kMostBias<T>) {
+              if (!kBF16 && fabsf(x) > kPlainBias) {
+                c3 = to_f32<T>(from_f32<T>(x * 0x1p-15f));
+                x = fmaf(c3, -0x1p15f, x);
+                c4 = to_f32<T>(from_f32<T>(x * 0x1p-6f));
+                x = fmaf(c4, -0x1p6f, x);
+              }
               const float hi = to_f32<T>(from_f32<T>(x));
               mid = to_f32<T>(from_f32<T>(x - hi));
               lo = x - hi - mid;
@@ -681,8 +693,9 @@ __global__ void __launch_bounds__(kThreads, 1)
             } else {
               x = x < 0.f ? -INFINITY : x > 0.f ? INFINITY : x;
             }
-            *reinterpret_cast<uint2*>(smem + kOffExtra + (1 + st) * kExtraBytes + (k >> 3) * 256 + (k & 7) * 16) =
-                make_uint2(pack2<T>(x, mid), pack2<T>(lo, 0.f));
+            uint8_t* chunk = smem + kOffExtra + (1 + st) * kExtraBytes + (k >> 3) * 256 + (k & 7) * 16;
+            if constexpr (kBF16) *reinterpret_cast<uint2*>(chunk) = make_uint2(pack2<T>(x, mid), pack2<T>(lo, 0.f));
+            else *reinterpret_cast<uint4*>(chunk) = make_uint4(pack2<T>(x, mid), pack2<T>(lo, c3), pack2<T>(c4, 0.f), 0u);
           } else {
             dst[k] = bias_log2(b[u]) + away;
           }

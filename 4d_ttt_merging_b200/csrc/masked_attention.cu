@@ -79,6 +79,12 @@ bool few_rows(int dtype, int64_t rows, int64_t group, int64_t heads_and_sequence
   return dtype == VB200_F32 || rows * group <= 16 || (rows * group + 15) / 16 * heads_and_sequences <= 32;
 }
 
+// The tile kernel adds bias and distance inside the QK product, where what it can hold of them shrinks with the scale
+// (attention_masked_tc.cu); below these scales the few-row kernel, which adds them in fp32, takes the call whatever its rows.
+bool bias_beyond_product(int dtype, const vb200_score_mods* m, bool bias) {
+  return m->softcap == 0.f && (bias || m->slope != nullptr) && m->scale < (dtype == VB200_F16 ? 0x1p-8f : 0x1p-76f);
+}
+
 }  // namespace
 
 int rows_map(CUtensorMap* map, const void* base, int dtype, long long n, long long heads, long long batch, long long sn, long long sh,
@@ -170,7 +176,8 @@ extern "C" int vb200_masked_attention(int dtype, const void* q, const void* k, c
   a.bias = mods->key_bias, a.bias_sb = mods->key_bias_sb;
   a.qpos = mods->q_position, a.qpos_sb = mods->q_position_sb;
   a.kpos = mods->k_position, a.kpos_sb = mods->k_position_sb;
-  if (few_rows(dtype, Nq, a.group, Hkv * B)) return rows_attention(dtype, false, a, Nk, static_cast<cudaStream_t>(stream));
+  if (few_rows(dtype, Nq, a.group, Hkv * B) || bias_beyond_product(dtype, mods, a.bias != nullptr))
+    return rows_attention(dtype, false, a, Nk, static_cast<cudaStream_t>(stream));
   return tile_attention(dtype, false, a, Nk, workspace, workspace_bytes, static_cast<cudaStream_t>(stream));
 }
 
@@ -217,6 +224,7 @@ extern "C" int vb200_paged_attention(int dtype, const void* q, void* out, int64_
   a.page_shift = cache->page_size == 16 ? 4 : cache->page_size == 32 ? 5 : cache->page_size == 64 ? 6 : 7;
   a.max_pages = static_cast<int>(cache->max_pages), a.causal = causal;
   const int64_t most = cache->max_pages * cache->page_size;
-  if (few_rows(dtype, (rows + n - 1) / n, a.group, cache->kv_heads * n)) return rows_attention(dtype, true, a, most, static_cast<cudaStream_t>(stream));
+  if (few_rows(dtype, (rows + n - 1) / n, a.group, cache->kv_heads * n) || bias_beyond_product(dtype, mods, a.bias != nullptr))
+    return rows_attention(dtype, true, a, most, static_cast<cudaStream_t>(stream));
   return tile_attention(dtype, true, a, most, workspace, workspace_bytes, static_cast<cudaStream_t>(stream));
 }

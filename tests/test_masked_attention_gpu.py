@@ -389,3 +389,31 @@ def test_small_probabilities_add_up(pkg, oracle, cuda_device, dtype, heads, quer
     step = 4 * 2.0 ** -28 * p.max() * v[0, 0].sum(0) + 2.0 ** -25 if dtype == "f16" else 0.0
     assert (np.abs(got - want) <= rel * want + step).all(), np.abs(got / want - 1).max()
     assert pkg.device_error_flags() == 0
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f16", "f32"])
+@pytest.mark.parametrize("queries", [300, 2])
+@pytest.mark.parametrize("scale", [1e-30, 1e-5, 2.0 ** -9, 1 / 64, 0.125])
+@pytest.mark.parametrize("dist", [False, True])
+def test_biases_at_any_scale(pkg, oracle, cuda_device, dtype, queries, scale, dist):
+    """Biases and distances of ordinary size beside products of any scale: bias / scale leaves the range of fp16 and of bf16."""
+    rng, q, k, v = make(51, 1, 2, 2, queries, 400, dtype, oracle)
+    bias = rng.choice([0.0, -0.7, -1.3, 1.0, -30.0], 400).astype(np.float32)
+    slope = np.array([0.01, 0.3], np.float32) if dist else None
+    run(pkg, oracle, cuda_device, dtype, q, k, v, bias, slope=slope, scale=scale)
+    if dist:
+        run(pkg, oracle, cuda_device, dtype, q, k, v, slope=slope, scale=scale)
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f16", "f32"])
+@pytest.mark.parametrize("queries", [300, 2])
+@pytest.mark.parametrize("size", [160.0, 248.0, 504.0])
+def test_biases_that_products_outweigh(pkg, oracle, cuda_device, dtype, queries, size):
+    """Keys whose products with the queries are as large as their bias is low (3,200 to 31,752 nats), beside keys without either."""
+    rng, q, k, v = make(52, 1, 2, 2, queries, 400, dtype, oracle, q_scale=1.0)
+    bias = np.zeros(400, np.float32)
+    q[..., 0] = size
+    k[..., 0] = 0.0
+    k[:, :, 7::50, 0] = size
+    bias[7::50] = -size * size / 8 + rng.uniform(-2, 2, 8)
+    run(pkg, oracle, cuda_device, dtype, q, k, v, bias)
