@@ -81,7 +81,7 @@ constexpr int kOffKeys = kOffExtra + (1 + kStages) * kExtraBytes;  // [stage][2]
 constexpr int kOffBar = kOffKeys + kStages * 2 * kBN * 4;
 constexpr int kBarQ = 0, kBarFull = 1, kBarEmpty = kBarFull + kStages, kBarS = kBarEmpty + kStages, kBarSFree = kBarS + kQT,
               kBarP = kBarSFree + kQT, kBarO = kBarP + kQT, kBarTail = kBarO + kQT, kNumBars = kBarTail + 1;
-constexpr int kOffMisc = kOffBar + kNumBars * 8;  // TMEM base; per query tile: first and last key
+constexpr int kOffMisc = kOffBar + kNumBars * 8;  // TMEM base; per query tile: first and last key; whether this part is the last
 constexpr int kSmemBytes = kOffMisc + 32 + 1024;
 constexpr int kMaxSplit = 8;
 constexpr size_t kPartBytes = static_cast<size_t>(kQT) * kBM * (kHeadDim + 2) * 4;  // O, then (maximum, sum), of a block's rows
@@ -421,6 +421,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   auto bar = [=](int i) -> uint32_t { return sbase + kOffBar + 8 * i; };
   int* key_lo = reinterpret_cast<int*>(smem + kOffMisc + 8);
   int* key_hi = key_lo + kQT;
+  volatile int* last_part = key_hi + kQT;
   // keys of a tile that are in registers at a time
   constexpr int kPart = kForm == 2 ? 32 : 64, kParts = kBN / kPart;
   // one pair of exponentials in this many on the FMA pipe, which idles beside the exponential unit (8232 rows and keys with
@@ -889,9 +890,9 @@ __global__ void __launch_bounds__(kThreads, 1)
       __threadfence();
       named_bar_sync(1, kSoftmaxWarps * 32);
       if (threadIdx.x == 0)
-        *reinterpret_cast<volatile int*>(key_lo) = atomicAdd(w.counters + (item - w.n_full), 1u) == static_cast<unsigned>(split - 1);
+        *last_part = atomicAdd(w.counters + (item - w.n_full), 1u) == static_cast<unsigned>(split - 1);
       named_bar_sync(1, kSoftmaxWarps * 32);
-      if (write && *reinterpret_cast<volatile int*>(key_lo) != 0) {
+      if (write && *last_part != 0) {
         __threadfence();
         float f[kMaxSplit];
         m_run = -INFINITY;

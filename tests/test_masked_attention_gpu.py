@@ -417,3 +417,21 @@ def test_biases_that_products_outweigh(pkg, oracle, cuda_device, dtype, queries,
     k[:, :, 7::50, 0] = size
     bias[7::50] = -size * size / 8 + rng.uniform(-2, 2, 8)
     run(pkg, oracle, cuda_device, dtype, q, k, v, bias)
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+@pytest.mark.parametrize("mass", [False, True])
+def test_parts_without_keys(pkg, oracle, cuda_device, dtype, mass):
+    """A block in parts whose rows see a few keys at both ends, so that the parts in between have no tile and reach the
+    joining at once: the same bits every time, and right."""
+    rng, q, k, v = make(61, 1, 4, 4, 256, 9000, dtype, oracle)
+    bias = np.log(rng.integers(1, 9, 9000)).astype(np.float32) if mass else None
+    r = np.zeros((256, 2), np.int32)
+    r[:128] = np.sort(rng.integers(0, 130, (128, 2)), 1)
+    r[128:] = np.sort(rng.integers(8800, 9001, (128, 2)), 1)
+    first = run(pkg, oracle, cuda_device, dtype, q, k, v, bias, r)
+    td = TORCH_DTYPE[dtype]
+    args = [gpu(t, cuda_device, td) for t in (q, k, v)]
+    b, kr = gpu(bias, cuda_device), gpu(r, cuda_device)
+    outs = [pkg.masked_attention(*args, b, key_range=kr) for _ in range(200)]
+    assert all(torch.equal(o, first) for o in outs) and pkg.device_error_flags() == 0
