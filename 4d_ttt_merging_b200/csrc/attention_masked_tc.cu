@@ -163,13 +163,7 @@ __device__ __forceinline__ uint32_t pack2(float lo, float hi) {
   return sizeof(T) == 2 && std::is_same<T, __nv_bfloat16>::value ? pack_bf16x2(lo, hi) : pack_f16x2(lo, hi);
 }
 
-// tanh(y) / y as a polynomial in y^2, fitted here for minimum maximum relative error (least squares reweighted to equal
-// ripples): degree 3 for |y| <= 1/2 (5e-7), degree 5 for |y| <= 1 (6e-7); 7e-7 evaluated in fp32.
-constexpr double kTanhNear[4] = {0.999999463558197, -0.33326318860054016, 0.13190296292304993, -0.04440222308039665};
-constexpr double kTanhFar[6] = {0.9999994039535522,    -0.3332904279232025,  0.13281433284282684,
-                                -0.051605671644210815, 0.016743112355470657, -0.0030670592095702887};
-
-// The same for cap * log2(e) * tanh(r s) / r in r^2, each coefficient twice for the packed instructions.
+// The polynomials of tanh for cap * log2(e) * tanh(r s) / r in r^2, each coefficient twice for the packed instructions.
 // A polynomial whose coefficients leave the range of normal numbers (a cap far from the scale) has limit -1 and is not used.
 struct CapPoly {
   uint64_t near_[4], far_[6];

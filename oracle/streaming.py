@@ -5,7 +5,7 @@
 
 * a score x_j is a dot product of 64 products in fp32: at most 64 * 2^-24 * sum_d |q_d k_jd| * scale off; forming it in the
   log2 domain with cap, bias and distance rounds it at most 8 more times, 2^-24 of its size (of the sizes of its terms) each;
-  the cap's tanh is good to 2^-21 absolute, times the cap;
+  the cap's tanh is good to 2^-20 relative and 2^-21 absolute, times the cap;
 * e^x then is off by that much relative, plus 2^-13 where 16-bit types allow a polynomial exponential (7.5e-5), 2^-21 for
   fp32;
 * sums over the keys round 2^-24 per addition, at most keys / 16 + 128 in a row;
@@ -47,7 +47,7 @@ def masked_attention(q, k, v, bias=None, ranges=None, *, scale=0.125, softcap=No
                 err = 64 * u * abs(scale) * (np.abs(q[b, h]) @ np.abs(kk).T) + 8 * u * np.abs(x)
                 if softcap:
                     x = softcap * np.tanh(x / softcap)
-                    err += softcap * 2.0 ** -21
+                    err += np.minimum(softcap * 2.0 ** -21, np.abs(x) * 2.0 ** -20)
                 if m is not None:
                     x = x + m[None]
                     err += 8 * u * np.abs(m)[None]

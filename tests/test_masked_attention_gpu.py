@@ -435,3 +435,17 @@ def test_parts_without_keys(pkg, oracle, cuda_device, dtype, mass):
     b, kr = gpu(bias, cuda_device), gpu(r, cuda_device)
     outs = [pkg.masked_attention(*args, b, key_range=kr) for _ in range(200)]
     assert all(torch.equal(o, first) for o in outs) and pkg.device_error_flags() == 0
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f16", "f32"])
+@pytest.mark.parametrize("queries", [300, 2])
+@pytest.mark.parametrize("softcap", [50.0, 3e3, 3e4, 1e5, 1e6, 1e9, 1e30])
+def test_scores_far_below_the_cap(pkg, oracle, cuda_device, dtype, queries, softcap):
+    """A cap that scores hardly reach, down to one that changes nothing, leaves them their bits."""
+    rng, q, k, v = make(71, 1, 2, 2, queries, 300, dtype, oracle)
+    run(pkg, oracle, cuda_device, dtype, q, k, v, softcap=softcap)
+    run(pkg, oracle, cuda_device, dtype, q, k, v, np.log(rng.integers(1, 9, 300)).astype(np.float32), softcap=softcap)
+    k[0, 0, 5], k[0, 1, 200] = np.nan, np.nan  # exact_row: the rows that do not see these keys
+    r = np.tile(np.array([[6, 200]], np.int32), (queries, 1))
+    v[0, 0, 5], v[0, 1, 200] = np.nan, np.nan
+    run(pkg, oracle, cuda_device, dtype, q, k, v, None, r, softcap=softcap)
