@@ -660,8 +660,7 @@ __global__ void __launch_bounds__(kThreads, 1)
               at = (static_cast<long long>(id) << a.page_shift) + (key & ((1 << a.page_shift) - 1));
             }
             if (a.bias != nullptr && there) b[u] = __ldg(a.bias + at);
-            if (down)
-              kp[u] = !kPaged && a.kpos != nullptr ? __ldg(a.kpos + s.batch * a.kpos_sb + key) : static_cast<float>(key);
+            if (down) kp[u] = key_position<kPaged>(a, s, position_origin<kPaged>(a, s, row_first), key);
           }
         }
         if (n >= kStages) ok = __all_sync(0xffffffffu, mbar_wait(bar(kBarEmpty + st), (n / kStages - 1) & 1, a.err));
@@ -710,7 +709,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     const uint32_t p_addr = tmem + lane_off + kTmemP + t * kHeadDim;
     const uint32_t o_addr = tmem + lane_off + kTmemO + t * kHeadDim;
     const int i = row_first + t * kBM + row;  // token of the sequence
-    const float pos = by_side ? static_cast<float>(pos_first + t * kBM + row) : down && valid ? row_position<kPaged>(a, s, i) : 0.f;
+    const float pos = by_side ? static_cast<float>(t * kBM + row) : down && valid ? row_position<kPaged>(a, s, position_origin<kPaged>(a, s, row_first), i) : 0.f;
     // keys that every row of the warp sees
     const int all_lo = __reduce_max_sync(0xffffffffu, valid ? be.x : 0);
     const int all_hi = __reduce_min_sync(0xffffffffu, valid ? be.y : 0x7fffffff);
@@ -740,7 +739,8 @@ __global__ void __launch_bounds__(kThreads, 1)
       const float* keys = reinterpret_cast<const float*>(smem + kOffKeys) + st * 2 * kBN;
       const int key0 = j * kBN;
       // what the row's own distance adds to every score of the tile
-      const float add = side == 0 ? 0.f : -slope * fabsf(pos - static_cast<float>(side > 0 ? key0 + kBN - 1 : key0));
+      const float rel = static_cast<float>(key0 - pos_first);
+      const float add = side == 0 ? 0.f : -slope * (side > 0 ? pos - (rel + static_cast<float>(kBN - 1)) : rel - pos);
       uint32_t r[kPart];
       auto load = [&](int h) {
 #pragma unroll

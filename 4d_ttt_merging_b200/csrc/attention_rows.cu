@@ -86,6 +86,7 @@ __global__ void __launch_bounds__(kRowWarps * 32, R <= 2 ? 3 : 2) rows_attention
   const long long pair0 = static_cast<long long>(blk) * R;
   const int pairs = static_cast<int>(min(static_cast<long long>(R), static_cast<long long>(s.rows) * a.group - pair0));
 
+  const int origin = position_origin<kPaged>(a, s, static_cast<int>(pair0 / a.group));
   if (threadIdx.x < R) {
     const int r = threadIdx.x;
     int2 be = make_int2(0, 0);
@@ -94,7 +95,7 @@ __global__ void __launch_bounds__(kRowWarps * 32, R <= 2 ? 3 : 2) rows_attention
       const int i = static_cast<int>((pair0 + r) / a.group), g = static_cast<int>((pair0 + r) % a.group);
       be = row_range<kPaged>(a, s, i);
       if (a.slope != nullptr) {
-        p = row_position<kPaged>(a, s, i);
+        p = row_position<kPaged>(a, s, origin, i);
         sl = __ldg(a.slope + hk * a.group + g) * kLog2E;
       }
     }
@@ -175,8 +176,7 @@ __global__ void __launch_bounds__(kRowWarps * 32, R <= 2 ? 3 : 2) rows_attention
         kr[u].load(kb + koff + static_cast<long long>(at0 + off) * a.k_sn);
         vr[u].load(vb_ + voff + static_cast<long long>(at0 + off) * a.v_sn);
         bs[u] = bias == nullptr ? 0.f : bias_log2(__ldg(bias + boff + at0 + off));
-        kp[u] = !dist ? 0.f : (!kPaged && a.kpos != nullptr ? __ldg(a.kpos + s.batch * a.kpos_sb + key0 + off)
-                                                            : static_cast<float>(key0 + off));
+        kp[u] = !dist ? 0.f : key_position<kPaged>(a, s, origin, key0 + off);
       } else {
         kr[u].zero();
         vr[u].zero();
@@ -395,6 +395,7 @@ __global__ void __launch_bounds__(kRowWarps * 32, 2) few_rows_kernel(const __gri
   const int pairs = static_cast<int>(min(static_cast<long long>(kRows), static_cast<long long>(s.rows) * a.group - pair0));
   auto token_of = [&](int r) { return static_cast<int>((pair0 + r) / a.group); };
   auto head_of = [&](int r) { return hk * a.group + static_cast<int>((pair0 + r) % a.group); };
+  const int origin = position_origin<kPaged>(a, s, token_of(0));
   if (threadIdx.x < kRows) bad[threadIdx.x] = 0;
   const uint32_t bars = smem_u32(&full_bar[warp][0]);
   if (lane == 0) {
@@ -435,7 +436,7 @@ __global__ void __launch_bounds__(kRowWarps * 32, 2) few_rows_kernel(const __gri
         const int2 x = row_range<kPaged>(a, s, token_of(r));
         be[n][e] = x;
         if (a.slope != nullptr) {
-          pos[n][e] = row_position<kPaged>(a, s, token_of(r));
+          pos[n][e] = row_position<kPaged>(a, s, origin, token_of(r));
           slp[n][e] = __ldg(a.slope + head_of(r)) * kLog2E;
         }
         if (x.y > x.x) {
@@ -544,10 +545,7 @@ __global__ void __launch_bounds__(kRowWarps * 32, 2) few_rows_kernel(const __gri
     float kp[2] = {0.f, 0.f};
     if (a.slope != nullptr) {
 #pragma unroll
-      for (int u = 0; u < 2; ++u) {
-        const int key = key0 + 8 * u + g;
-        kp[u] = !kPaged && a.kpos != nullptr ? __ldg(a.kpos + s.batch * a.kpos_sb + min(key, s.keys - 1)) : static_cast<float>(key);
-      }
+      for (int u = 0; u < 2; ++u) kp[u] = key_position<kPaged>(a, s, origin, min(key0 + 8 * u + g, s.keys - 1));  // beyond: hidden
     }
     uint32_t p[kN][2];
 #pragma unroll

@@ -112,10 +112,22 @@ __device__ __forceinline__ int2 row_range(const AttnView& a, const AttnSeq& s, i
   return e > b ? make_int2(b, e) : make_int2(0, 0);
 }
 
+// Positions in fp32.  Token indices are counted from that of a row of the block (its first, say): fp32 holds every whole number up
+// to 2^24 only, and in a longer sequence the distances between neighbours would be lost; counted so, a distance d is off by
+// 2^-24 d at most.  Positions that are given stand as they are.
 template <bool kPaged>
-__device__ __forceinline__ float row_position(const AttnView& a, const AttnSeq& s, int i) {
+__device__ __forceinline__ int position_origin(const AttnView& a, const AttnSeq& s, int row) {
+  return !kPaged && (a.qpos != nullptr || a.kpos != nullptr) ? 0 : s.keys - s.rows + row;
+}
+template <bool kPaged>
+__device__ __forceinline__ float row_position(const AttnView& a, const AttnSeq& s, int origin, int i) {
   if (!kPaged && a.qpos != nullptr) return __ldg(a.qpos + s.batch * a.qpos_sb + i);
-  return static_cast<float>(s.keys - s.rows + i);
+  return static_cast<float>(s.keys - s.rows + i - origin);
+}
+template <bool kPaged>
+__device__ __forceinline__ float key_position(const AttnView& a, const AttnSeq& s, int origin, int j) {
+  if (!kPaged && a.kpos != nullptr) return __ldg(a.kpos + s.batch * a.kpos_sb + j);
+  return static_cast<float>(j - origin);
 }
 
 // Page of a key tile's slot, or `pages` (outside the pool) with the error word set when the table
@@ -160,7 +172,8 @@ __device__ __noinline__ void exact_row(const AttnView& a, AttnSeq s, int i, int 
   const int lane = threadIdx.x & 31, hk = head / a.group;
   const int2 be = row_range<kPaged>(a, s, i);
   const float slope = a.slope == nullptr ? 0.f : __ldg(a.slope + head) * kLog2E;
-  const float pos = row_position<kPaged>(a, s, i);
+  const int origin = position_origin<kPaged>(a, s, i);
+  const float pos = row_position<kPaged>(a, s, origin, i);
   const T* q = static_cast<const T*>(a.q) + s.batch * a.q_sb + head * a.q_sh + static_cast<long long>(s.row0 + i) * a.q_sn + 2 * lane;
   const float q0 = to_f32<T>(q[0]) * a.scale, q1 = to_f32<T>(q[1]) * a.scale;
   float m = -INFINITY, l = 0.f, o0 = 0.f, o1 = 0.f;
@@ -182,7 +195,7 @@ __device__ __noinline__ void exact_row(const AttnView& a, AttnSeq s, int i, int 
         vo = s.batch * a.v_sb + j * a.v_sn;
         if (a.bias != nullptr) b = bias_log2(__ldg(a.bias + s.batch * a.bias_sb + j));
       }
-      kp = !kPaged && a.slope != nullptr && a.kpos != nullptr ? __ldg(a.kpos + s.batch * a.kpos_sb + j) : static_cast<float>(j);
+      if (a.slope != nullptr) kp = key_position<kPaged>(a, s, origin, j);
     }
     for (unsigned some = __ballot_sync(0xffffffffu, b != -INFINITY); some != 0; some &= some - 1) {
       const int from = __ffs(some) - 1;

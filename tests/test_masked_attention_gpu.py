@@ -449,3 +449,31 @@ def test_scores_far_below_the_cap(pkg, oracle, cuda_device, dtype, queries, soft
     r = np.tile(np.array([[6, 200]], np.int32), (queries, 1))
     v[0, 0, 5], v[0, 1, 200] = np.nan, np.nan
     run(pkg, oracle, cuda_device, dtype, q, k, v, None, r, softcap=softcap)
+
+
+@pytest.mark.parametrize("dtype,queries,page", [("bf16", 600, 0), ("f16", 600, 0), ("bf16", 3, 0), ("f32", 3, 0), ("bf16", 600, 64), ("f16", 2, 128)])
+@pytest.mark.parametrize("softcap", [None, 20.0])
+def test_distances_beyond_24_bits(pkg, oracle, cuda_device, dtype, queries, page, softcap):
+    """More than 2^24 keys, dense and paged: the distances among the last tokens are whole numbers that fp32 positions of the
+    sequence do not hold."""
+    td, near = TORCH_DTYPE[dtype], 1800
+    n = (1 << 24) + (1 << 20) + 3
+    k, v = (torch.zeros(1, 1, -(-n // 128) * 128, 64, device=cuda_device, dtype=td) for _ in range(2))
+    rng, qn, kn, vn = make(81, 1, 1, 1, queries, near, dtype, oracle, q_scale=1.0)
+    k[:, :, n - near:n], v[:, :, n - near:n] = gpu(kn, cuda_device, td), gpu(vn, cuda_device, td)
+    first = near - queries + np.arange(queries)
+    r = np.stack([np.maximum(first - 900, 0), first + 1], 1).astype(np.int32)
+    r[::3, 1] = near  # keys behind the row too
+    slope = np.array([0.75], np.float32)
+    q, kr, sl = gpu(qn, cuda_device, td), gpu(r + (n - near), cuda_device, torch.int32), gpu(slope, cuda_device)
+    if page:
+        pools = [t.view(-1, page, 1, 64) for t in (k, v)]
+        pages = pools[0].shape[0]
+        ints = lambda x: x.to(device=cuda_device, dtype=torch.int32)  # noqa: E731
+        cache = pkg.PagedCache(*pools, None, ints(torch.arange(pages).view(1, pages)), ints(torch.tensor([n])), ints(torch.ones(pages)))
+        out = pkg.paged_attention(q[0].transpose(0, 1), cache, [0], [0, queries], key_range=kr, distance_slope=sl, softcap=softcap)
+        out = out.transpose(0, 1)[None]
+    else:
+        out = pkg.masked_attention(q, k[:, :, :n], v[:, :, :n], key_range=kr, distance_slope=sl, softcap=softcap)
+    check(out, *oracle.streaming.masked_attention(qn, kn, vn, None, r, slope=slope, softcap=softcap, dtype=dtype))
+    assert pkg.device_error_flags() == 0
