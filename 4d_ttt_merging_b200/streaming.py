@@ -65,12 +65,48 @@ def _rows(t: torch.Tensor) -> torch.Tensor:
     return t.clone(memory_format=torch.contiguous_format)
 
 
-def _check_out(q: torch.Tensor, out: torch.Tensor, *inputs: torch.Tensor) -> None:
+def _runs(t: torch.Tensor) -> tuple[int, list[tuple[int, int]]]:
+    """Bytes of the contiguous runs that a tensor consists of, and the (byte stride, count) of the dimensions that place them."""
+    es = t.element_size()
+    run, outer = es, []
+    for s, n in sorted((s * es, n) for s, n in zip(t.stride(), t.shape) if n > 1 and s):
+        if s <= run and not outer:
+            run += s * (n - 1)
+        else:
+            outer.append((s, n))
+    return run, outer
+
+
+def _share_memory(a: torch.Tensor, b: torch.Tensor) -> bool:
+    """Whether two tensors have a byte in common.  Views of one buffer may interleave without that."""
+    if not a.numel() or not b.numel() or a.device != b.device:
+        return False
+    at, bt = a.data_ptr(), b.data_ptr()
+    reach = lambda t: t.element_size() * (1 + sum([s * (n - 1) for s, n in zip(t.stride(), t.shape)]))  # noqa: E731
+    if at + reach(a) <= bt or bt + reach(b) <= at:
+        return False
+    (ra, oa), (rb, ob) = _runs(a), _runs(b)
+    pitch = math.gcd(*(s for s, _ in oa + ob))
+    if pitch and ra <= (bt - at) % pitch <= pitch - rb:  # runs at different places of one pitch
+        return False
+
+    def starts(t, outer):
+        x = torch.tensor([t - min(at, bt)])
+        for s, n in outer:
+            x = (x[:, None] + s * torch.arange(n)).flatten()
+        return x.sort().values
+
+    xa, xb = starts(at, oa), starts(bt, ob)
+    before = torch.searchsorted(xa, xb + rb) - 1  # the last run of a that starts before a run of b ends
+    return bool(((before >= 0) & (xa[before.clamp(min=0)] + ra > xb)).any())
+
+
+def _check_out(q: torch.Tensor, out: torch.Tensor, *inputs: torch.Tensor | None) -> None:
     if out.shape != q.shape or out.dtype != q.dtype or not _tma_ready(out):
         raise ValueError("out must have q's shape and dtype, a unit channel stride and 16-byte aligned rows")
     if any(s == 0 and n > 1 for s, n in zip(out.stride(), out.shape)):
         raise ValueError("out must not be a broadcast tensor")
-    if out.numel() and any(out.data_ptr() == t.data_ptr() for t in (q, *inputs)):
+    if any(isinstance(t, torch.Tensor) and _share_memory(out, t) for t in (q, *inputs)):
         raise ValueError("out must not share memory with the inputs")
 
 
@@ -160,7 +196,7 @@ def masked_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, log_key_
     rounded to q's type as in ``mass_bias_attention``).  ``key_range`` int32 [Nq, 2] or [B, Nq, 2]: the row sees keys
     [begin, end) (``attention_ranges`` makes them); None: all.  A row without keys gives zeros; what hidden
     keys hold never reaches a row.  ``distance_slope`` [H] with positions [Nq] / [Nk] (or per batch entry), by default
-    token indices with the queries last.  Returns [B, H, Nq, 64] as a view of a token-major buffer, or writes ``out``, which must not overlap the inputs."""
+    token indices with the queries last.  Returns [B, H, Nq, 64] as a view of a token-major buffer, or writes ``out``, which must not share memory with the inputs."""
     if q.ndim != 4 or k.ndim != 4 or v.ndim != 4:
         raise ValueError("q, k and v must be [batch, heads, tokens, channels]")
     B, H, Nq, D = q.shape
@@ -181,7 +217,7 @@ def masked_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, log_key_
     if key_range is not None and (key_range.dtype != torch.int32 or key_range.shape not in ((Nq, 2), (B, Nq, 2))):
         raise ValueError(f"key_range must be int32 [{Nq}, 2] or [{B}, {Nq}, 2]")
     if out is not None:
-        _check_out(q, out, k, v)
+        _check_out(q, out, k, v, log_key_mass, key_range, distance_slope, query_position, key_position)
     C.require_cuda(q, "masked_attention")
     _same_device("masked_attention", q.device, k, v, log_key_mass, key_range, distance_slope, query_position, key_position, out)
     _refuse_gradients("masked_attention", q, k, v, log_key_mass, distance_slope, query_position, key_position, out)
@@ -378,7 +414,8 @@ def paged_attention(q: torch.Tensor, cache: PagedCache, sequence, offsets, *, ca
     already (``PagedCache.append``); H is a multiple of the cache's heads.  A row sees the keys up to its own (``causal``) or
     all of its slot, or the keys [begin, end) of ``key_range`` int32 [rows, 2] (frames in causal order).  The cache's log-masses
     are added to the scores; softcap, distance_slope and scale as in ``masked_attention``, positions are token indices.
-    Returns [rows, H, 64] or writes ``out`` (apart from q); rows outside every chunk are not written."""
+    Returns [rows, H, 64] or writes ``out``, which must not share memory with q, the cache or another input; rows outside every chunk
+    are not written."""
     shape = q.shape
     if len(shape) != 3 or shape[2] != 64:
         raise ValueError("q must be [rows, heads, 64]")
@@ -394,7 +431,7 @@ def paged_attention(q: torch.Tensor, cache: PagedCache, sequence, offsets, *, ca
     if key_range is not None and (key_range.dtype != torch.int32 or key_range.shape != (rows, 2)):
         raise ValueError(f"key_range must be int32 [{rows}, 2]")
     if out is not None:
-        _check_out(q, out)
+        _check_out(q, out, cache.k, cache.v, cache.log_mass, cache.table, cache.length, key_range, distance_slope, sequence, offsets)
     dev = cache._device
     if q.device != dev:
         C.require_cuda(q, "paged_attention")

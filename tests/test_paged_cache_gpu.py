@@ -436,3 +436,15 @@ def test_last_tile_without_masses(pkg, oracle, cuda_device, dtype, causal, lengt
     cache.append(order, off, t(k), t(v))
     assert ref.append(order, off, k, v)
     attend(pkg, oracle, cuda_device, dtype, cache, ref, rng, order, counts, heads, causal=causal, q_scale=1.0)
+
+
+def test_outputs_in_the_cache_are_refused(pkg, cuda_device):
+    cache = pkg.PagedCache.empty(2, 4, 4, page_size=16, heads=2, device=cuda_device)
+    x = torch.zeros(3, 3, 2, 64, device=cuda_device, dtype=torch.bfloat16)
+    seq, off = (torch.tensor(t, device=cuda_device, dtype=torch.int32) for t in ([0], [0, 2]))
+    q = x[:2, 0]
+    for bad in (x[1:, 0], cache.k[1, :2], cache.v[3, 5:7], q):
+        with pytest.raises(ValueError, match="share memory"):
+            pkg.paged_attention(q, cache, seq, off, out=bad)
+    assert pkg.paged_attention(q, cache, seq, off, out=x[:2, 2]).data_ptr() == x[0, 2].data_ptr()
+    assert pkg.device_error_flags() == 0

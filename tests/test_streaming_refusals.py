@@ -3,6 +3,7 @@ the oracle of the cache."""
 from __future__ import annotations
 
 import ctypes
+import importlib
 
 import numpy as np
 import pytest
@@ -176,3 +177,56 @@ def test_oracle_bound_is_narrow(oracle, dtype):
     out, bound = oracle.streaming.masked_attention(q, k, v, bias, dtype=dtype)
     # at most two roundings of the whole, the result's step, and what the other roundings take as above
     assert (bound <= (2 + 3 * 2 * oracle.streaming.EPS_HALF[dtype]) * out + 2.0 ** -25).all()
+
+
+def _bytes(t):
+    at = torch.zeros(1, dtype=torch.int64) + t.data_ptr()
+    for s, n in zip(t.stride(), t.shape):
+        at = (at[:, None] + s * t.element_size() * torch.arange(n)).flatten()
+    return {int(x) + i for x in at for i in range(t.element_size())}
+
+
+def test_shared_memory_is_seen(pkg):
+    """Against the sets of bytes, over views of one buffer."""
+    share = importlib.import_module(pkg.__name__ + ".streaming")._share_memory
+    rng = np.random.default_rng(7)
+    base = torch.zeros(600, dtype=torch.bfloat16)
+    found = 0
+    for _ in range(600):
+        views = []
+        for _ in range(2):
+            while True:
+                shape, stride = rng.integers(1, 5, 3).tolist(), rng.choice([0, 1, 2, 4, 7, 8, 16, 24, 48], 3).tolist()
+                first, last = int(rng.integers(0, 120)), sum(s * (n - 1) for s, n in zip(stride, shape))
+                if first + last < 600:
+                    break
+            views.append(base.as_strided(shape, stride, first))
+        want = bool(_bytes(views[0]) & _bytes(views[1]))
+        assert share(*views) == want, [(v.shape, v.stride(), v.storage_offset()) for v in views]
+        found += want
+    assert 100 < found < 500
+
+
+def test_outputs_that_share_memory(pkg):
+    """Refused where an output has a byte of an input, taken where views of one buffer lie side by side."""
+    f = pkg.masked_attention
+    buf = torch.zeros(1, 9, 4, 2, 64)  # tokens of q | k | v | out
+    q, k, v, out = (buf[:, :, i].transpose(1, 2) for i in range(4))
+    heads = torch.zeros(1, 8, 9, 64)   # heads of q | k | v | out
+    tokens = torch.zeros(1, 2, 36, 64)  # every head: tokens of q | k | v | out
+    for x in ((q, k, v, out), heads.chunk(4, 1), tokens.chunk(4, 2)):
+        with pytest.raises(RuntimeError, match="CUDA"):  # as far as a call comes without one
+            f(*x[:3], out=x[3])
+        for i in range(3):
+            with pytest.raises(ValueError, match="share memory"):
+                f(*x[:3], out=x[i])
+    rows = torch.zeros(1, 2, 10, 64)
+    for a, b in ((rows[:, :, :9], rows[:, :, 1:]), (rows[:, :, 1:], rows[:, :, :9])):
+        with pytest.raises(ValueError, match="share memory"):
+            f(a, k, v, out=b)
+        with pytest.raises(ValueError, match="share memory"):
+            f(q, a, v, out=b)
+        with pytest.raises(ValueError, match="share memory"):
+            f(q, k, a, out=b)
+    with pytest.raises(ValueError, match="share memory"):
+        f(q, k, v, log_key_mass=rows.view(-1)[-9:], out=rows[:, :, 1:])
