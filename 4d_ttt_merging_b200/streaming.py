@@ -10,8 +10,8 @@ operators for what lies next to that:
   fork, free and compact them on the device without host synchronisation;
 * ``paged_attention``    a chunk of new tokens per stream (a frame, or one token) over that cache.
 
-They have no backward pass: tensors that require a gradient are refused while gradients are recorded.  The reference
-has no counterpart (its inference is one clip, batch one).
+They have no derivatives: tensors that require a gradient are refused while gradients are recorded, and so are the dual tensors
+of forward-mode differentiation.  The reference has no counterpart (its inference is one clip, batch one).
 """
 from __future__ import annotations
 
@@ -21,6 +21,7 @@ import math
 from dataclasses import dataclass
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _clib as C
 from .ops import _tma_ready
@@ -43,6 +44,10 @@ def _refuse_gradients(what: str, *tensors) -> None:
         for t in tensors:
             if t is not None and t.requires_grad:
                 raise RuntimeError(f"{what} has no backward pass: call it under torch.no_grad() or detach its inputs")
+    if forward_ad._current_level >= 0:  # inside dual_level(); tangents are carried under no_grad() too
+        for t in tensors:
+            if t is not None and forward_ad.unpack_dual(t).tangent is not None:
+                raise RuntimeError(f"{what} has no forward-mode derivative: its inputs must not be dual tensors")
 
 
 def _same_device(what: str, device: torch.device, *tensors) -> None:
@@ -352,7 +357,7 @@ class PagedCache:
             if log_mass.shape != shape[:1]:
                 raise ValueError(f"append: log_mass must be [{shape[0]}]")
         _same_device("append", dev, k, v, log_mass)
-        _refuse_gradients("append", k, v, log_mass)
+        _refuse_gradients("append", k, v, log_mass, self.k, self.v, self.log_mass)
         with _on(dev):
             sequence = _int_vector("sequence", sequence, dev)
             n = sequence.numel()
@@ -436,7 +441,7 @@ def paged_attention(q: torch.Tensor, cache: PagedCache, sequence, offsets, *, ca
     if q.device != dev:
         C.require_cuda(q, "paged_attention")
     _same_device("paged_attention", dev, q, key_range, distance_slope, out)
-    _refuse_gradients("paged_attention", q, distance_slope, out)
+    _refuse_gradients("paged_attention", q, distance_slope, out, cache.k, cache.v, cache.log_mass)
     with _on(dev):
         sequence = _int_vector("sequence", sequence, dev)
         n = sequence.numel()

@@ -448,3 +448,24 @@ def test_outputs_in_the_cache_are_refused(pkg, cuda_device):
             pkg.paged_attention(q, cache, seq, off, out=bad)
     assert pkg.paged_attention(q, cache, seq, off, out=x[:2, 2]).data_ptr() == x[0, 2].data_ptr()
     assert pkg.device_error_flags() == 0
+
+
+def test_derivatives_are_refused(pkg, cuda_device):
+    cache = pkg.PagedCache.empty(2, 4, 4, page_size=16, heads=2, device=cuda_device)
+    x = torch.zeros(1, 2, 64, device=cuda_device, dtype=torch.bfloat16)
+    dense = torch.zeros(1, 2, 5, 64, device=cuda_device)
+    ad = torch.autograd.forward_ad
+    with ad.dual_level():
+        dual = ad.make_dual(x, torch.ones_like(x))
+        for call in (lambda: cache.append([0], [0, 1], dual, x), lambda: pkg.paged_attention(dual, cache, [0], [0, 1]),
+                     lambda: pkg.masked_attention(dense, ad.make_dual(dense, dense), dense)):
+            with pytest.raises(RuntimeError, match="forward-mode"):
+                call()
+    assert cache.length.tolist() == [0, 0]
+    cache.v.requires_grad_()
+    for call in (lambda: cache.append([0], [0, 1], x, x), lambda: pkg.paged_attention(x, cache, [0], [0, 1])):
+        with pytest.raises(RuntimeError, match="no backward"):
+            call()
+    with torch.no_grad():
+        cache.append([0], [0, 1], x, x)
+    assert cache.length.tolist() == [1, 0] and pkg.device_error_flags() == 0

@@ -230,3 +230,20 @@ def test_outputs_that_share_memory(pkg):
             f(q, k, a, out=b)
     with pytest.raises(ValueError, match="share memory"):
         f(q, k, v, log_key_mass=rows.view(-1)[-9:], out=rows[:, :, 1:])
+
+
+def test_derivatives_are_refused(pkg):
+    refuse = importlib.import_module(pkg.__name__ + ".streaming")._refuse_gradients
+    t = torch.zeros(2)
+    refuse("call", t, None)
+    with pytest.raises(RuntimeError, match="no backward"):
+        refuse("call", t, torch.zeros(2, requires_grad=True))
+    with torch.no_grad():
+        refuse("call", torch.zeros(2, requires_grad=True))
+    with torch.autograd.forward_ad.dual_level():
+        refuse("call", t, None)
+        dual = torch.autograd.forward_ad.make_dual(t, torch.ones(2))
+        with pytest.raises(RuntimeError, match="forward-mode"):
+            refuse("call", t, dual)
+        with torch.no_grad(), pytest.raises(RuntimeError, match="forward-mode"):
+            refuse("call", dual)
