@@ -33,7 +33,7 @@ import torch.nn.functional as F
 from torch import nn
 
 from .ops import head_layernorm, mass_bias_attention, row_gather
-from .streaming import PagedCache, masked_attention, paged_attention
+from .streaming import PagedCache, _positive, _refuse_gradients, masked_attention, paged_attention
 from .token_plan import WeightedBilinearTokenPlan
 
 __all__ = ["AttentionMask", "GlobalAttention", "compute_attention"]
@@ -306,6 +306,7 @@ class GlobalAttention(nn.Module):
                 raise ValueError("stream: with a token plan all rows are one chunk")
         elif offsets is None and streams != 1:
             raise ValueError("stream: offsets are needed for several streams")
+        _positive("softcap", softcap)  # what the attention would refuse is refused before the cache takes anything
         qkv = self._qkv(x, token_plan)
         log_mass = None
         if token_plan is None:
@@ -319,6 +320,7 @@ class GlobalAttention(nn.Module):
             log_mass = getattr(token_plan, "key_log_mass", None)
             log_mass = None if log_mass is None else log_mass.reshape(-1)
         q, k, v = (t.to(cache.k.dtype) for t in (q, k, v))  # LayerNorm gives fp32 under autocast
+        _refuse_gradients("stream", q, k, v, log_mass)
         # made on the device, so that the step can be recorded into a graph
         chunk = lambda n: torch.arange(2, device=x.device, dtype=torch.int32) * n if offsets is None else offsets
         cache.append(sequence, chunk(k.shape[0]), k, v, log_mass)

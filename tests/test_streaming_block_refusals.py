@@ -77,3 +77,23 @@ def test_output_refusals(pkg):
         x = [torch.zeros(1, 4, 3, 64) for _ in range(3)]
         with pytest.raises(ValueError, match="share memory"):
             pkg.masked_attention(*x, out=x[i])
+
+
+def test_a_refused_stream_step_leaves_the_cache(pkg):
+    """What the attention would refuse after the append is refused before it."""
+    m = pkg.GlobalAttention(128, 2)
+
+    class Cache:
+        k = torch.zeros(4, 16, 2, 64)
+
+        def append(self, *args):
+            raise AssertionError("the cache was written")
+
+    x = torch.zeros(1, 6, 128)
+    for cap in (0.0, -1.0, float("nan")):
+        with torch.no_grad(), pytest.raises(ValueError, match="softcap"):
+            m.stream(x, Cache(), [0], softcap=cap)
+    m.requires_grad_(False)
+    m.q_norm.weight.requires_grad_()  # the queries alone require a gradient
+    with pytest.raises(RuntimeError, match="no backward"):
+        m.stream(x, Cache(), [0])
