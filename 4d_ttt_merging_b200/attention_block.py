@@ -290,7 +290,8 @@ class GlobalAttention(nn.Module):
         stream.  Rows see the past and their whole chunk, or with ``causal`` no later token.  With a token plan, x is the
         new frames of one stream, merged among themselves: the cache takes its merged keys with their masses.
         Special queries of a plan attend over merged keys here (the past is kept in that form only), so plans with
-        ``dense_special_queries`` are refused, as is ``causal`` with a plan.  Returns [1, N, C].
+        ``dense_special_queries`` are refused, as is ``causal`` with a plan.  Returns [1, N, C]; rows outside every chunk (a padded
+        batch) come out as rows without keys do.
 
         A pool without room for the chunks leaves the cache as it was and shows in ``device_error_flags()`` (bit 2); the
         rows then attend over the past alone."""
@@ -324,6 +325,7 @@ class GlobalAttention(nn.Module):
         # made on the device, so that the step can be recorded into a graph
         chunk = lambda n: torch.arange(2, device=x.device, dtype=torch.int32) * n if offsets is None else offsets
         cache.append(sequence, chunk(k.shape[0]), k, v, log_mass)
-        attn = paged_attention(q, cache, sequence, chunk(q.shape[0]), causal=causal, softcap=softcap)
+        out = None if offsets is None else q.new_zeros(q.shape)  # the attention leaves rows outside the chunks as they are
+        attn = paged_attention(q, cache, sequence, chunk(q.shape[0]), causal=causal, softcap=softcap, out=out)
         y = self.proj(attn.reshape(1, attn.shape[0], -1).to(qkv.dtype))
         return y if token_plan is None else token_plan.restore(y)

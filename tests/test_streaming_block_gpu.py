@@ -291,3 +291,20 @@ def test_hard_merged_clips_and_streams(pkg, oracle, cuda_device, dtype):
     ref, bound = attend(oracle, q, k, v, None, dtype)
     close(z[0][t(keep[0])], ref, bound)
     assert cache.length.item() == kept and pkg.device_error_flags() == 0
+
+
+def test_rows_outside_the_chunks(pkg, oracle, cuda_device):
+    """A padded batch: rows before the first chunk and behind the last are those of a row without keys, whatever memory they got."""
+    m = block(pkg, cuda_device, "bf16")
+    cache = pkg.PagedCache.empty(3, 20, 8, page_size=16, heads=HEADS, device=cuda_device)
+    n, cut = 300, [4, 20, 20, 50]
+    x = torch.randn(1, n, DIM, generator=torch.Generator().manual_seed(4)).to(cuda_device, torch.bfloat16)
+    with torch.no_grad():
+        for _ in range(3):
+            stale = [torch.full((n, HEADS, 64), float("nan"), device=cuda_device, dtype=torch.bfloat16) for _ in range(8)]
+            del stale
+            y = m.stream(x, cache, [2, 1, 0], cut, causal=True)
+            empty = m.proj(torch.zeros(1, DIM, device=cuda_device, dtype=torch.bfloat16))
+            outside = torch.cat([y[0, :4], y[0, 50:]])
+            assert torch.equal(outside, empty.expand_as(outside)) and bool(torch.isfinite(y).all())
+    assert cache.length.tolist() == [90, 0, 48] and pkg.device_error_flags() == 0
