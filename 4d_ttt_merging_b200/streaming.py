@@ -29,6 +29,7 @@ from .ops import _tma_ready
 __all__ = ["PagedCache", "attention_ranges", "masked_attention", "paged_attention"]
 
 _PAGES = (16, 32, 64, 128)
+_WIDE = (torch.int64, torch.uint32, torch.uint64)
 _Two = ctypes.c_int64 * 2
 _HERE = contextlib.nullcontext()
 _current_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)  # without the check that CUDA is up
@@ -141,14 +142,21 @@ def _positive(what: str, value: float | None) -> float:
 
 
 def _int_vector(what: str, t, device: torch.device, n: int | None = None) -> torch.Tensor:
-    """A 1-D int32 device tensor; lists and other integer tensors are converted."""
+    """A 1-D int32 device tensor; lists and other integer tensors are converted.  Values beyond int32 are refused on the host and
+    become its ends on the device, which are out of every range, so that none of them turns into another slot or row."""
     if isinstance(t, torch.Tensor) and t.dtype is torch.int32 and t.device == device and t.ndim == 1 and t.is_contiguous() and (
             n is None or t.numel() == n):
         return t
     if not isinstance(t, torch.Tensor):
         t = torch.tensor(t, dtype=None if len(t) else torch.int32)
-    if t.ndim != 1 or t.dtype.is_floating_point or t.dtype == torch.bool or (n is not None and t.numel() != n):
+    if t.ndim != 1 or t.dtype.is_floating_point or t.dtype.is_complex or t.dtype == torch.bool or (n is not None and t.numel() != n):
         raise ValueError(f"{what} must be a 1-D integer tensor" + ("" if n is None else f" of {n} entries"))
+    if t.dtype in _WIDE:
+        t = t.to(torch.int64)  # an unsigned value beyond int64 becomes a negative one
+        if t.is_cuda:
+            t = t.clamp(-2 ** 31, 2 ** 31 - 1)
+        elif t.numel() and not (-2 ** 31 <= int(t.min()) and int(t.max()) < 2 ** 31):
+            raise ValueError(f"{what} has values that int32 does not hold")
     return t.to(device=device, dtype=torch.int32).contiguous()
 
 
@@ -164,8 +172,8 @@ def attention_ranges(queries: int, keys: int | None = None, *, documents: torch.
 
     Everything is computed on the device of ``documents`` (else ``device``), without host synchronisation."""
     keys = queries if keys is None else keys
-    if queries < 0 or keys < queries:
-        raise ValueError("attention_ranges: 0 <= queries <= keys is required")
+    if queries < 0 or keys < queries or keys >= 2 ** 31:
+        raise ValueError("attention_ranges: 0 <= queries <= keys < 2^31 is required")
     if (step is not None and step < 1) or (window is not None and window < 1) or prefix < 0:
         raise ValueError("attention_ranges: step and window are at least 1, prefix at least 0")
     if documents is not None:

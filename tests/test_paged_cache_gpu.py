@@ -469,3 +469,20 @@ def test_derivatives_are_refused(pkg, cuda_device):
     with torch.no_grad():
         cache.append([0], [0, 1], x, x)
     assert cache.length.tolist() == [1, 0] and pkg.device_error_flags() == 0
+
+
+def test_integers_beyond_32_bits(pkg, oracle, cuda_device):
+    """On the device they name no slot and no row: an error bit, and the cache as it was."""
+    rng, cache, ref = filled(pkg, oracle, cuda_device, "bf16", 16, 2, [20, 30])
+    t = lambda *x: torch.tensor(x, device=cuda_device)  # noqa: E731
+    k = torch.zeros(4, 2, 64, device=cuda_device, dtype=torch.bfloat16)
+    before = cache.length.clone(), cache.table.clone()
+    for call in (lambda: cache.append(t(2 ** 32), t(0, 4), k, k), lambda: cache.append(t(0), t(2 ** 32, 2 ** 32 + 4), k, k),
+                 lambda: cache.fork(t(2 ** 32 + 1), t(2)), lambda: cache.fork(t(1), t(2 ** 33 + 2)), lambda: cache.free(t(-2 ** 32))):
+        call()
+        assert pkg.device_error_flags() == 2
+        assert torch.equal(cache.length, before[0]) and torch.equal(cache.table, before[1])
+    out = torch.full((4, 2, 64), 7.0, device=cuda_device, dtype=torch.bfloat16)
+    pkg.paged_attention(k, cache, t(2 ** 32), t(0, 4), out=out)
+    pkg.paged_attention(k, cache, t(0), t(2 ** 32, 2 ** 32 + 4), out=out)
+    assert pkg.device_error_flags() == 2 and bool((out == 7).all())

@@ -247,3 +247,18 @@ def test_derivatives_are_refused(pkg):
             refuse("call", t, dual)
         with torch.no_grad(), pytest.raises(RuntimeError, match="forward-mode"):
             refuse("call", dual)
+
+
+def test_integers_beyond_32_bits(pkg):
+    """Slots and offsets that int32 does not hold are refused on the host; nothing wraps round to another slot."""
+    f = importlib.import_module(pkg.__name__ + ".streaming")._int_vector
+    cpu = torch.device("cpu")
+    for good in ([1, 2], [], range(3), np.array([1, -5]), torch.tensor([2 ** 31 - 1, -2 ** 31]), torch.tensor([1, 7], dtype=torch.uint32),
+                 torch.tensor([3], dtype=torch.uint8)):
+        assert f("sequence", good, cpu).tolist() == [int(x) for x in good] and f("sequence", good, cpu).dtype == torch.int32
+    for bad in ([2 ** 32], [0, 2 ** 31], [-2 ** 31 - 1], torch.tensor([2 ** 40]), torch.tensor([2 ** 32 - 1], dtype=torch.uint32),
+                torch.tensor([2 ** 63 + 1], dtype=torch.uint64), torch.zeros(2, dtype=torch.complex64), torch.zeros(2, dtype=torch.bool)):
+        with pytest.raises(ValueError, match="sequence"):
+            f("sequence", bad, cpu)
+    with pytest.raises(ValueError, match="2\\^31"):
+        pkg.attention_ranges(1, 2 ** 31)
