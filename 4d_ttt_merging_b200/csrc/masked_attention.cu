@@ -56,6 +56,7 @@ int fill_mods(const vb200_score_mods* m, AttnView& a) {
   } else {
     a.scale = m->scale * kLog2E;
     a.cap = 0.f;
+    VB200_REQUIRE(std::isfinite(a.scale), "attention: scale out of range");
   }
   return VB200_OK;
 }

@@ -262,3 +262,16 @@ def test_integers_beyond_32_bits(pkg):
             f("sequence", bad, cpu)
     with pytest.raises(ValueError, match="2\\^31"):
         pkg.attention_ranges(1, 2 ** 31)
+
+
+def test_scales_that_overflow_are_refused(pkg):
+    """A scale is held with a factor log2(e): the largest finite ones would become infinite, and every result NaN."""
+    lib, C = pkg.load_library(), pkg._clib
+    s = (ctypes.c_int64 * 3)(64, 64, 64)
+    two = (ctypes.c_int64 * 2)(64, 64)
+    cache = C.CacheHandle(k=16, v=16, table=16, length=16, references=16, pages=4, page_size=16, kv_heads=2, slots=2, max_pages=4)
+    for mods in (C.ScoreMods(scale=3e38), C.ScoreMods(scale=3e38, softcap=1e-3)):
+        assert lib.vb200_masked_attention(1, 16, 16, 16, 16, 1, 4, 2, 3, 5, 64, s, s, s, s, mods, None, 0, None) == C.EINVAL
+        assert b"out of range" in lib.vb200_last_error()
+        assert lib.vb200_paged_attention(1, 16, 16, 2, 4, 64, two, two, cache, 16, 16, 1, 1, mods, None, 0, None) == C.EINVAL
+        assert b"out of range" in lib.vb200_last_error()
