@@ -461,10 +461,11 @@ __global__ void __launch_bounds__(kRowWarps * 32, 2) few_rows_kernel(const __gri
   const int slot_mask = (1 << a.page_shift) - 1;
   auto page_at = [&](int c) -> int { return kPaged && c < c1 ? page_of(a, s, (lo + 16 * c) >> a.page_shift) : a.pages; };
   // TMA of step c (16 keys of one page) into place `at` of the warp's ring; past the tensor, or a page that there is not,
-  // reads zeros
+  // reads zeros.  After a wait that ran out nothing more is asked for: what is in flight was asked for before that wait.
   const uint32_t mine = smem_u32(ring) + warp * kRing * 2 * kSide;
+  bool ok = true;
   auto fetch = [&](int c, int page, int at) {
-    if (c < c1 && lane == 0) {
+    if (ok && c < c1 && lane == 0) {
       const uint32_t dst = mine + at * 2 * kSide, bar = bars + 8 * at;
       const int key0 = lo + 16 * c;
       mbar_arrive_expect_tx(bar, 2 * kSide);
@@ -498,7 +499,6 @@ __global__ void __launch_bounds__(kRowWarps * 32, 2) few_rows_kernel(const __gri
 
   // page numbers are looked up one step before their tiles are asked for, biases one step before they are used
   int here[kRing], cur = 0, phase = 0;
-  bool ok = true;
 #pragma unroll
   for (int k = 0; k < kRing - 1; ++k) {
     here[k] = page_at(c0 + warp + k * kRowWarps);
