@@ -289,10 +289,7 @@ __device__ __forceinline__ float probabilities(const uint32_t (&r)[N], float mul
   return (a0 + a1) + (b0 + b1);
 }
 
-// 2^f on [-1/2, 1/2] as a polynomial of degree 3, fitted here for minimum maximum relative error (7.5e-5: 1/52
-// of what the probability's rounding to bf16 may take, 1/6 for fp16).
-constexpr float kE0 = 0.9999280729920136f, kE1 = 0.6932609862143841f, kE2 = 0.24261113147493726f, kE3 = 0.05517166934152859f;
-constexpr float kLeast = -125.f;  // exponents that the polynomial's integer arithmetic takes
+constexpr float kLeast = -125.f;  // the lowest exponent that exp2_pair takes; its 7.5e-5 are 1/52 of what rounding to bf16 may take, 1/6 for fp16
 
 __device__ __forceinline__ float fmin3_nan(float a, float b, float c) {  // NaN if one of them is
   float d;
@@ -300,21 +297,7 @@ __device__ __forceinline__ float fmin3_nan(float a, float b, float c) {  // NaN 
   return d;
 }
 
-// 2^e for two exponents in [kLeast, kRescale] without the exponential unit: e = n + f, and n is added to the exponent bits.
-__device__ __forceinline__ void exp2_pair(uint64_t e, float& q0, float& q1) {
-  const uint64_t shift = pk2(12582912.f, 12582912.f), t = fadd2(e, shift);  // 1.5 * 2^23: n in the lowest bits
-  const uint64_t f = fadd2(e, ffma2(t, pk2(-1.f, -1.f), shift));
-  uint64_t y = ffma2(pk2(kE3, kE3), f, pk2(kE2, kE2));
-  y = ffma2(y, f, pk2(kE1, kE1));
-  y = ffma2(y, f, pk2(kE0, kE0));
-  float t0, t1, y0, y1;
-  upk2(t, t0, t1);
-  upk2(y, y0, y1);
-  q0 = u2f((f2u(t0) << 23) + f2u(y0));
-  q1 = u2f((f2u(t1) << 23) + f2u(y1));
-}
-
-// The same for keys that every row of the warp sees, straight from the products and with the maximum that the row has so far,
+// Probabilities of keys that every row of the warp sees, straight from the products and with the maximum that the row has so far,
 // so that the exponential unit, the FMA pipe (cap, exponents, sums) and the ALU (maxima) work side by side instead of one
 // after the other.  False for a row whose maximum grows by more than 2^most or, with a cap, whose scores leave the polynomial's
 // range: then nothing of it holds, and r is as it was.  off: what is added to a score, less the maximum; most: by how much a

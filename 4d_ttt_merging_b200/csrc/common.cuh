@@ -315,19 +315,17 @@ __device__ __forceinline__ float fmax3(float a, float b, float c) {
   return d;
 }
 
-// 2^e for two values on the FMA pipe (no MUFU), for e <= 64.  Method: round-to-nearest
+// 2^e for two values on the FMA pipe (no MUFU), for -125 <= e <= 64.  Method: round-to-nearest
 // split e = n + f with the 1.5 * 2^23 shifter (n lands in the low mantissa bits of
 // t = e + 1.5 * 2^23, f = e - n in [-1/2, 1/2]); 2^f by a degree-3 polynomial fitted here for
 // minimum maximum relative error on [-1/2, 1/2] (Remez exchange, 7.5e-5 with fp32 Horner);
-// 2^n applied by adding n to the exponent field (t's bits shifted left by 23).  Inputs below
-// -125 are clamped, giving about 2^-125 instead of a denormal or zero.
-__device__ __forceinline__ void exp2_poly2(float e0, float e1, float& p0, float& p1) {
+// 2^n applied by adding n to the exponent field (t's bits shifted left by 23).
+__device__ __forceinline__ void exp2_pair(uint64_t e, float& p0, float& p1) {
   constexpr float kShift = 12582912.0f;  // 1.5 * 2^23
   constexpr float kC0 = 0.99992805719375610f;
   constexpr float kC1 = 0.69326096773147583f;
   constexpr float kC2 = 0.24261112511157990f;
   constexpr float kC3 = 0.05517166852951050f;
-  const uint64_t e = pk2(fmaxf(e0, -125.f), fmaxf(e1, -125.f));
   const uint64_t t = fadd2(e, pk2(kShift, kShift));
   const uint64_t neg_n = ffma2(t, pk2(-1.f, -1.f), pk2(kShift, kShift));  // shifter - t = -n
   const uint64_t f = fadd2(e, neg_n);
@@ -339,6 +337,10 @@ __device__ __forceinline__ void exp2_poly2(float e0, float e1, float& p0, float&
   upk2(t, tlo, thi);
   p0 = __uint_as_float(__float_as_uint(plo) + (__float_as_uint(tlo) << 23));
   p1 = __uint_as_float(__float_as_uint(phi) + (__float_as_uint(thi) << 23));
+}
+// The same for any e <= 64: inputs below -125 give about 2^-125 instead of a denormal or zero.
+__device__ __forceinline__ void exp2_poly2(float e0, float e1, float& p0, float& p1) {
+  exp2_pair(pk2(fmaxf(e0, -125.f), fmaxf(e1, -125.f)), p0, p1);
 }
 
 __device__ __forceinline__ uint32_t pack_bf16x2(float lo, float hi) {
