@@ -54,7 +54,7 @@ def masked_attention(q, k, v, bias=None, ranges=None, *, scale=0.125, softcap=No
                 if slope is not None:
                     d = float(slope[h]) * np.abs(at(qpos, Nq, Nk - Nq)[:, None] - at(kpos, Nk, 0)[None])
                     x = x - d
-                    err += 8 * u * d
+                    err += 8 * u * np.abs(d)  # slopes may be negative
             x = np.where(see, x, -np.inf)
             top = x.max(1, keepdims=True)
             p = np.exp(x - np.where(np.isneginf(top), 0.0, top))

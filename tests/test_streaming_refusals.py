@@ -275,3 +275,12 @@ def test_scales_that_overflow_are_refused(pkg):
         assert b"out of range" in lib.vb200_last_error()
         assert lib.vb200_paged_attention(1, 16, 16, 2, 4, 64, two, two, cache, 16, 16, 1, 1, mods, None, 0, None) == C.EINVAL
         assert b"out of range" in lib.vb200_last_error()
+
+
+def test_oracle_bound_of_a_growing_bias(oracle):
+    """A distance bias of either sign rounds by its size: a negative slope takes nothing from the bound."""
+    rng = np.random.default_rng(3)
+    q, k, v = np.zeros((1, 1, 4, 64)), rng.standard_normal((1, 1, 900, 64)), rng.standard_normal((1, 1, 900, 64))
+    out, bound = oracle.streaming.masked_attention(q, k, v, slope=[-2.0])
+    # the keys that count lie 890 tokens away and more: their bias and the row's maximum, each 1,780, round 8 times
+    assert (bound > 2 * 8 * 2.0 ** -24 * 1700 * np.abs(out)).all()
