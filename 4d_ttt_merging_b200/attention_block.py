@@ -294,7 +294,7 @@ class GlobalAttention(nn.Module):
         batch) come out as rows without keys do.
 
         A pool without room for the chunks leaves the cache as it was and shows in ``device_error_flags()`` (bit 2); the
-        rows then attend over the past alone."""
+        rows then attend over the past alone, and with ``causal``, as if its last tokens were theirs, over part of it."""
         if x.ndim != 3 or x.shape[0] != 1:
             raise ValueError("stream: x must be [1, tokens, channels]")
         streams = len(sequence)

@@ -20,7 +20,9 @@
 // the products, with the maximum as it is, and the tile's maximum is looked at afterwards; the first tile, tiles that the
 // mask cuts and tiles after a miss take their maximum first.  With a cap this lets its polynomial (FMA pipe) run beside the
 // exponentials: 213 -> 154 us (1024 rows, 8192 keys, 37 heads; parts of 64 keys instead of 32 leave the compiler too few
-// registers to interleave them: 186); without a cap 127 -> 117.
+// registers to interleave them: 186); without a cap 127 -> 117.  Scores beyond half the cap, and keys of mass 0 in the places
+// whose exponential the FMA pipe takes, send their part of a tile the other way: 8232 rows and keys of 16 heads take 582 us
+// with scores within half the cap, 1420 beyond it; without a cap 404, with one such key in every 64 485 us.
 //
 // The two warps of an SM sub-partition compute their exponentials at the same time and leave the unit idle at the same time
 // (3200 clocks per 256 x 128 scores, 2100 of them in exponentials); making them take turns measured 8% slower, starting one
@@ -35,7 +37,8 @@
 // Work that is skipped: key tiles outside the union of the rows' intervals.  Masks are evaluated in the tiles that
 // some row of a warp sees in part only.  A hidden key has probability 0; what its value holds still meets that 0 in
 // the PV product, so a row that comes out with a value that is not finite is computed again, key by key, by its
-// warp (exact_row): rows are right whatever the hidden values are, and finite inputs pay one test per row.
+// warp (exact_row): rows are right whatever the hidden values are, and finite inputs pay one test per row.  Those that do not
+// pay much more: 1041 rows of 16 heads over 5000 keys 65 us, with NaN in the 100 values behind them 184 ms.
 //
 // The last, partly filled wave of blocks is split over the keys (up to 8 parts a block).  Every part writes O, maximum
 // and sum to the workspace and counts itself; the part that comes last joins all of them in order, so the result
@@ -362,7 +365,8 @@ constexpr float kPlainBias = 60000.f;
 // slope |pos - ref|, one number per row, plus slope |ref - key|, one per key, with ref the tile's key nearest to the rows:
 // the second is a bias like any other, and the first goes where the maximum is subtracted.  The few tiles among the rows'
 // own positions, tiles of explicit positions and negative slopes take the distance key by key in the softmax.  (All tiles key
-// by key: 195 us instead of 112 without a distance, six streams of 42 to 542 new tokens over 1900 to 9600.)  With a distance the
+// by key 251 us, so 180, without a distance 160: six streams of 42 to 542 new tokens over 1900 to 9600; a frame of 1041 tokens over
+// 32,928 keys 414, 311, 277.)  With a distance the
 // tiles are taken last to first: a causal row then meets its largest scores first, and its maximum hardly ever grows.
 //
 // A bias that does not fit in the product: one below the range (the type's lowest value, say) hides its key there, as -inf

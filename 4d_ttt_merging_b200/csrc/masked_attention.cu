@@ -76,6 +76,10 @@ bool aligned(const void* p, const int64_t* s, std::initializer_list<int64_t> siz
 // its tiles are nearly empty and the heads of a group read their keys one by one; or at most 32 blocks of 16 pairs in
 // all, where either kernel leaves SMs idle and the lighter one ends sooner (17 rows, 16 heads, 1041 keys: 12 against 18 us,
 // 16,464 keys: 29 against 35; 33 rows and 4116 keys, beyond the rule: 27 against 20).
+//
+// The rule sees the mean of a paged call's rows (the host does not know the chunks), so a call that mixes long chunks with single
+// tokens takes one kernel for all: 32 streams of 500 to 9000 keys, 16 heads, take 121 us with a token each; with one chunk
+// of 300 rows among them 213 (by itself 27), with one of 1041 rows 190 (45).  Such calls are better made apart.
 bool few_rows(int dtype, int64_t rows, int64_t group, int64_t heads_and_sequences) {
   return dtype == VB200_F32 || rows * group <= 16 || (rows * group + 15) / 16 * heads_and_sequences <= 32;
 }
@@ -224,6 +228,9 @@ extern "C" int vb200_paged_attention(int dtype, const void* q, void* out, int64_
   a.n_seq = static_cast<int>(n), a.slots = static_cast<int>(cache->slots), a.pages = static_cast<int>(cache->pages);
   a.page_shift = cache->page_size == 16 ? 4 : cache->page_size == 32 ? 5 : cache->page_size == 64 ? 6 : 7;
   a.max_pages = static_cast<int>(cache->max_pages), a.causal = causal;
+  // What the splits over the keys are planned for: the host does not know the lengths, so a short stream in a table with room for
+  // many keys is split like a long one.  Room for 65,536: 8 chunks of 300 rows over 1100 keys 43 -> 90 us, 1041 rows over 2701
+  // 45 -> 64; decode, and a frame over 32,928 keys, as with a table that is just wide enough.
   const int64_t most = cache->max_pages * cache->page_size;
   if (few_rows(dtype, (rows + n - 1) / n, a.group, cache->kv_heads * n) || bias_beyond_product(dtype, mods, a.bias != nullptr))
     return rows_attention(dtype, true, a, most, static_cast<cudaStream_t>(stream));

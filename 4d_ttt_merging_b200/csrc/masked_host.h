@@ -19,7 +19,8 @@ int rows_map(CUtensorMap* map, const void* base, int dtype, long long n, long lo
              long long sb, int box);
 int pool_map(CUtensorMap* map, const void* base, int dtype, const AttnView& a, int box);
 
-// The FMA-pipe kernel: any type, any number of rows; most_keys bounds the keys of a sequence.
+// The kernels for few rows (bf16, fp16: warp-level matrix instructions) and for fp32 (FMA pipe); they take any number of rows.
+// most_keys bounds the keys of a sequence.
 int rows_attention(int dtype, bool paged, const AttnView& a, long long most_keys, cudaStream_t st);
 
 // The tensor-core kernel: bf16 and fp16.  Without the workspace its last wave runs unsplit.

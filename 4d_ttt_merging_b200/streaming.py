@@ -208,7 +208,8 @@ def masked_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, log_key_
     one type (fp32, bf16 or fp16), any strides.  ``log_key_mass`` [Nk] or [B, Nk] is added in fp32 (it is not
     rounded to q's type as in ``mass_bias_attention``).  ``key_range`` int32 [Nq, 2] or [B, Nq, 2]: the row sees keys
     [begin, end) (``attention_ranges`` makes them); None: all.  A row without keys gives zeros; what hidden
-    keys hold never reaches a row.  ``distance_slope`` [H] with positions [Nq] / [Nk] (or per batch entry), by default
+    keys hold never reaches a row (in 16 bits, infinite or NaN values near a row's keys cost a thousand times its time: keep a
+    buffer behind its valid keys finite).  Capped 16-bit scores are fastest within half the cap.  ``distance_slope`` [H] with positions [Nq] / [Nk] (or per batch entry), by default
     token indices with the queries last.  Returns [B, H, Nq, 64] as a view of a token-major buffer, or writes ``out``, which must not share memory with the inputs."""
     if q.ndim != 4 or k.ndim != 4 or v.ndim != 4:
         raise ValueError("q, k and v must be [batch, heads, tokens, channels]")
@@ -426,7 +427,8 @@ def paged_attention(q: torch.Tensor, cache: PagedCache, sequence, offsets, *, ca
     Rows offsets[i] .. offsets[i + 1] of q [rows, H, 64] are the last tokens of slot sequence[i] and are in the cache
     already (``PagedCache.append``); H is a multiple of the cache's heads.  A row sees the keys up to its own (``causal``) or
     all of its slot, or the keys [begin, end) of ``key_range`` int32 [rows, 2] (frames in causal order).  The cache's log-masses
-    are added to the scores; softcap, distance_slope and scale as in ``masked_attention``, positions are token indices.
+    are added to the scores; softcap, distance_slope and scale as in ``masked_attention``, positions are token indices.  One call
+    takes one kernel by its mean chunk, so single tokens and long chunks are better given in calls of their own.
     Returns [rows, H, 64] or writes ``out``, which must not share memory with q, the cache or another input; rows outside every chunk
     are not written."""
     shape = q.shape

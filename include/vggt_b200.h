@@ -120,8 +120,10 @@ VB200_API int vb200_exp2_poly(const float* x, float* y, int64_t n, void* stream)
  * out_i = sum_j e^{x_ij} v_j / sum_j e^{x_ij} over the keys j in [begin_i, end_i) of the row; a row
  * without keys gives 0.  What the other keys hold (infinities, NaN) never reaches the row.  Forward only.
  * head_dim 64; H is a multiple of Hkv, query head h reads key head h / (H / Hkv).  BF16 / F16 run on
- * tcgen05 (or the FMA pipe for few rows per key head), F32 on the FMA pipe; statistics and sums in fp32,
- * in 16 bits the probabilities are rounded to the value type before the PV product.
+ * tcgen05 (few rows per key head, and biases beside scales below 2^-8 (F16) or 2^-76 (BF16), on the warp-level
+ * matrix instructions), F32 on the FMA pipe; statistics and sums in fp32, in 16 bits the probabilities are rounded
+ * to the value type before the PV product.  A row whose tiles hold hidden values that are infinite or NaN is computed
+ * again key by key, which takes a thousand times as long: keep values behind the keys in use finite.
  * No reference counterpart: the reference's global attention sees one clip at a time, all of it. */
 typedef struct {
   const float* key_bias;     /* natural log, added to the score; NULL: none.  Dense calls only:    */
