@@ -486,3 +486,40 @@ def test_integers_beyond_32_bits(pkg, oracle, cuda_device):
     pkg.paged_attention(k, cache, t(2 ** 32), t(0, 4), out=out)
     pkg.paged_attention(k, cache, t(0), t(2 ** 32, 2 ** 32 + 4), out=out)
     assert pkg.device_error_flags() == 2 and bool((out == 7).all())
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+@pytest.mark.parametrize("heads,rows", [(4, 300), (2, 3)])
+@pytest.mark.parametrize("paged", [False, True])
+@pytest.mark.parametrize("softcap,dist,mass", [(None, False, False), (8.0, True, True), (None, True, True), (30.0, False, True)])
+def test_rows_beside_hidden_values(pkg, oracle, cuda_device, dtype, heads, rows, paged, softcap, dist, mass):
+    """Every row's tiles hold values that are NaN and hidden from it, so every row is computed a second time: intervals from one
+    key to 900, in a dense tensor and over pages, with all that changes a score."""
+    n, td = 1000, TORCH_DTYPE[dtype]
+    rng = np.random.default_rng(rows + heads)
+    k, v, m = tokens(rng, n, 2, dtype, oracle)
+    m[::17] = -np.inf
+    hide = np.ones(n, bool)
+    hide[40:940] = False
+    k[hide], v[hide] = np.nan, np.nan
+    r = np.sort(rng.integers(40, 940, (rows, 2)), 1).astype(np.int32)
+    r[::5] = [40, 940]
+    r[1::7, 1] = r[1::7, 0] + 1
+    q = oracle.round_to((rng.standard_normal((rows, heads, 64)) * 2).astype(np.float32), dtype)
+    slope = (2.0 ** -np.arange(1, heads + 1)).astype(np.float32) if dist else None
+    m = m if mass else None
+    t = lambda x, d=td: None if x is None else torch.from_numpy(np.ascontiguousarray(x)).to(cuda_device, d)  # noqa: E731
+    kw = dict(key_range=t(r, torch.int32), softcap=softcap, distance_slope=t(slope, torch.float32))
+    if paged:
+        cache = pkg.PagedCache.empty(2, 70, 65, page_size=16, heads=2, dtype=td, masses=mass, device=cuda_device)
+        cache.append([1], [0, n], t(k), t(v), t(m, torch.float32))
+        got = pkg.paged_attention(t(q), cache, [1], [0, rows], **kw).transpose(0, 1)[None]
+    else:
+        dense = lambda x: t(x.swapaxes(0, 1)[None])  # noqa: E731
+        got = pkg.masked_attention(dense(q), dense(k), dense(v), t(m, torch.float32), **kw)
+    want, bound = oracle.streaming.masked_attention(*(x[None].swapaxes(1, 2) for x in (q, np.where(hide[:, None, None], 0, k), np.where(hide[:, None, None], 0, v))),
+                                                    m, r, softcap=softcap, slope=slope, dtype=dtype)
+    got = to_np(got)
+    assert np.isfinite(got).all()
+    assert (np.abs(got - want) <= bound).all(), (np.abs(got - want) - bound).max()
+    assert pkg.device_error_flags() == 0
