@@ -83,13 +83,18 @@ def _runs(t: torch.Tensor) -> tuple[int, list[tuple[int, int]]]:
     return run, outer
 
 
+def _extent(t: torch.Tensor) -> tuple[int, int]:
+    """The addresses from a tensor's first byte to behind its last."""
+    at, n = t.data_ptr(), t.numel()
+    if n and not t.is_contiguous():
+        n = 1 + sum([s * (n - 1) for s, n in zip(t.stride(), t.shape)])
+    return at, at + n * t.element_size()
+
+
 def _share_memory(a: torch.Tensor, b: torch.Tensor) -> bool:
     """Whether two tensors have a byte in common.  Views of one buffer may interleave without that."""
-    if not a.numel() or not b.numel() or a.device != b.device:
-        return False
-    at, bt = a.data_ptr(), b.data_ptr()
-    reach = lambda t: t.element_size() * (1 + sum([s * (n - 1) for s, n in zip(t.stride(), t.shape)]))  # noqa: E731
-    if at + reach(a) <= bt or bt + reach(b) <= at:
+    (at, ae), (bt, be) = _extent(a), _extent(b)
+    if ae <= bt or be <= at or at == ae or bt == be or a.device != b.device:
         return False
     (ra, oa), (rb, ob) = _runs(a), _runs(b)
     pitch = math.gcd(*(s for s, _ in oa + ob))
@@ -107,12 +112,18 @@ def _share_memory(a: torch.Tensor, b: torch.Tensor) -> bool:
     return bool(((before >= 0) & (xa[before.clamp(min=0)] + ra > xb)).any())
 
 
-def _check_out(q: torch.Tensor, out: torch.Tensor, *inputs: torch.Tensor | None) -> None:
+def _check_out(q: torch.Tensor, out: torch.Tensor, *inputs: torch.Tensor | None, apart: tuple[tuple[int, int], ...] = ()) -> None:
+    """``apart``: extents of contiguous inputs on out's device."""
     if out.shape != q.shape or out.dtype != q.dtype or not _tma_ready(out):
         raise ValueError("out must have q's shape and dtype, a unit channel stride and 16-byte aligned rows")
     if any(s == 0 and n > 1 for s, n in zip(out.stride(), out.shape)):
         raise ValueError("out must not be a broadcast tensor")
-    if any(isinstance(t, torch.Tensor) and _share_memory(out, t) for t in (q, *inputs)):
+    first, last = _extent(out)
+    shared = any([a < last and first < b for a, b in apart]) and first < last
+    for t in (q, *inputs):  # most inputs start behind the output's last byte or end before its first
+        if not shared and isinstance(t, torch.Tensor) and t.data_ptr() < last:
+            shared = _share_memory(out, t)
+    if shared:
         raise ValueError("out must not share memory with the inputs")
 
 
@@ -142,7 +153,8 @@ def _positive(what: str, value: float | None) -> float:
 
 
 def _int_vector(what: str, t, device: torch.device, n: int | None = None) -> torch.Tensor:
-    """A 1-D int32 device tensor; lists and other integer tensors are converted.  Values beyond int32 are refused on the host and
+    """A 1-D int32 device tensor; lists and other integer tensors are converted (16 us of a call for int64 on the device, 8 of them
+    for the values below; int32 is taken as it is).  Values beyond int32 are refused on the host and
     become its ends on the device, which are out of every range, so that none of them turns into another slot or row."""
     if isinstance(t, torch.Tensor) and t.dtype is torch.int32 and t.device == device and t.ndim == 1 and t.is_contiguous() and (
             n is None or t.numel() == n):
@@ -315,7 +327,7 @@ class PagedCache:
         handle = C.CacheHandle(*(C.ptr(t) for t in (k, self.v, self.log_mass, *ints)), pages, page, heads, *self.table.shape)
         slots = self.table.shape[0]
         size = max(C.lib().vb200_cache_append_workspace_size(slots, slots, pages), C.lib().vb200_cache_compact_workspace_size(pages))
-        self.__dict__.update(_device=k.device, _heads=heads, _dtype=dtype, _row=k.shape[2:], _slots=slots, _handle=handle, _sizes={},
+        self.__dict__.update(_extents=tuple(_extent(t) for t in every if t is not self.references), _device=k.device, _heads=heads, _dtype=dtype, _row=k.shape[2:], _slots=slots, _handle=handle, _sizes={},
                              _workspace=torch.empty(size, dtype=torch.uint8, device=k.device), _workspace_bytes=size)
 
     def _scratch(self, size: int) -> torch.Tensor:
@@ -446,7 +458,7 @@ def paged_attention(q: torch.Tensor, cache: PagedCache, sequence, offsets, *, ca
     if key_range is not None and (key_range.dtype != torch.int32 or key_range.shape != (rows, 2)):
         raise ValueError(f"key_range must be int32 [{rows}, 2]")
     if out is not None:
-        _check_out(q, out, cache.k, cache.v, cache.log_mass, cache.table, cache.length, key_range, distance_slope, sequence, offsets)
+        _check_out(q, out, key_range, distance_slope, sequence, offsets, apart=cache._extents if out.device == cache._device else ())
     dev = cache._device
     if q.device != dev:
         C.require_cuda(q, "paged_attention")
